@@ -140,6 +140,81 @@ int mmf_hgrn_scan(mmf_ctx* ctx, float* out, const float* i, const float* f, size
 int mmf_rmsnorm_swishgate(mmf_ctx* ctx, float* out, const float* g, const float* o,
                           const float* w, size_t rows, size_t cols, float eps);
 
+/* ---- layer operators: a recurrent low-bit layer, dev pointers -----------------------------
+ * Operators of layers like the engine's own that it does not run itself: the norm before a
+ * product with its residual and 8-bit codes, products with 4-bit weights, and a selective
+ * state space token mixer (short convolution, scan). No counterparts in the reference.
+ *
+ * Rows may be fp32, bf16 or fp16 (the MMF_* types below), at any address aligned to their type,
+ * and ld elements apart (0: as long as a row; never less). Sums, states and scales are fp32 or
+ * wider, and each output is rounded to its type once, to nearest even. Outputs may not overlap
+ * other tensors of the call unless said otherwise (MMF_ERR_ARG where the addresses show it).
+ * Nothing is allocated by these calls but what mmf_workspace_bytes counts, so that they can be
+ * captured into a graph of the context's stream. Calls with no rows do nothing.
+ *
+ * Several sequences stand one after the other in the rows. lens (host, may be NULL) holds their
+ * `seqs` lengths, which sum to rows and may be 0; with NULL all have rows / seqs rows, so that
+ * rows == seqs is one token of each. A sequence's state row is read and then replaced by the state
+ * after its last row; a sequence of no rows keeps its own. Without a state (NULL) sequences
+ * start from zeros. */
+enum { MMF_F32 = 0, MMF_BF16 = 1, MMF_F16 = 2, MMF_I8 = 3 };
+
+/* The residual's addition, the RMS norm and the next product's int8 codes:
+ *   h = x + res (res may be NULL: h = x), y = h / sqrt(mean(h^2) + eps) * w,
+ *   m = max(max|y| of the row, 1e-5), scales[row] = m / 127, codes = round(y * 127 / m)
+ * (ties to even), the codes that MMF_INT8_ABSMAX takes of a row up to the rounding of its fp32
+ * steps; here they are taken in 64 bits. h (of x's type; may be NULL, and may be x or res itself
+ * with the same stride) and y (of x's type, may be NULL) are stored where given; the norm is taken
+ * of the sum before its rounding. A row whose sums or weights hold an infinity or NaN has codes 0
+ * and the scale NaN. */
+int mmf_add_rmsnorm_q8(mmf_ctx* ctx, int dtype, int8_t* codes, float* scales, const void* x, const void* res, void* h,
+                       void* y, const float* w, size_t rows, size_t cols, size_t ldx, size_t ldres, size_t ldh,
+                       size_t ldy, size_t ldcodes, float eps);
+
+/* Register weights [N, K] of 4 bits (host memory): codes [N, ceil(K/2)], two a byte, the even input's
+ * in the low half; scales [N, G] in fp16 (their bits) and zero points [N, G] in 0..15 (NULL: 8
+ * throughout), G = ceil(K / group) groups of `group` inputs, a multiple of 32 (0: one group a row).
+ * A weight is (code - zero) * scale. They are repacked on the device; the id is mmf_w4_linear's. */
+int mmf_w4_register(mmf_ctx* ctx, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, size_t N,
+                    size_t K, size_t group, int* w4_id);
+int mmf_w4_shape(mmf_ctx* ctx, int w4_id, size_t* N, size_t* K, size_t* group);
+/* Free registered weights; the id is invalid afterwards (calls that pass it fail with MMF_ERR_ARG). */
+int mmf_w4_release(mmf_ctx* ctx, int w4_id);
+/* out [rows, N] = x [rows, K] times the transposed weights, from one token to long prompts. x of
+ * dtype MMF_F32, MMF_BF16, MMF_F16, or MMF_I8 with xscales [rows] (else NULL): the codes and scales
+ * of mmf_add_rmsnorm_q8. out is of out_dtype (a float type). The weights enter every sum as the
+ * integers they are, with no rounding, and the scale multiplies a group's fp32 sum (int8 x: its
+ * exact integer sum). A row that holds an infinity or NaN has no finite output; finite inputs
+ * should stay below 1e36. */
+int mmf_w4_linear(mmf_ctx* ctx, int w4_id, int dtype, const void* x, const float* xscales, int out_dtype, void* out,
+                  size_t rows, size_t ldx, size_t ldo);
+
+/* Short causal convolution over each of D channels, width 1..8:
+ *   out[t, d] = act(bias[d] + sum_j w[d, j] * x[t - width + 1 + j, d])
+ * with act = silu if `silu`, w [D, width], bias [D] (may be NULL), state [seqs, width - 1, D] the
+ * inputs before a sequence's first row, oldest first (all fp32). */
+int mmf_short_conv(mmf_ctx* ctx, int dtype, void* out, const void* x, const float* w, const float* bias, float* state,
+                   const size_t* lens, size_t seqs, size_t rows, size_t D, size_t width, int silu, size_t ldx,
+                   size_t ldo);
+
+/* Selective state space scan over D channels with N states each (1..128). Row by row of a sequence,
+ *   dt' = dt + dt_bias[d] (through softplus if `softplus`)
+ *   h[n, d] = exp(dt' * A[d, n]) * h[n, d] + dt' * B[n] * u[d]
+ *   out[d] = (sum_n C[n] * h[n, d] + skip[d] * u[d]) * silu(z[d])
+ * out, u, dt, z [rows, D] and B, C [rows, N] of dtype; A [D, N], skip [D], dt_bias [D] and state
+ * [seqs, N, D] in fp32. z, skip, dt_bias and state may be NULL. */
+typedef struct {
+  int dtype, softplus;
+  void* out;
+  const void *u, *dt, *B, *C, *z;
+  const float *A, *skip, *dt_bias;
+  float* state;
+  const size_t* lens;
+  size_t seqs, rows, D, N;
+  size_t ldo, ldu, lddt, ldb, ldc, ldz;
+} mmf_scan_args;
+int mmf_selective_scan(mmf_ctx* ctx, const mmf_scan_args* args);
+
 /* ---- model (model.hpp:33-120) ----------------------------------------------------------- */
 typedef struct {
   size_t vocab_size, hidden_size, num_hidden_layers, intermediate_size; /* config.hpp:8-21 */

@@ -24,6 +24,7 @@ LIB_PATH = os.path.join(HERE, "_lib", "libmmfree_hip.so")
 MKBLOB = os.path.join(HERE, "_lib", "mmfree-mkblob")
 
 FLOAT, FIXED_Q510, INT8_ABSMAX = 0, 1, 2
+F32, BF16, F16, I8 = 0, 1, 2, 3  # row types of the layer operators
 MODES = {"float": FLOAT, "fixed": FIXED_Q510, "int8": INT8_ABSMAX}
 
 _vp = C.c_void_p
@@ -35,6 +36,12 @@ _fp = C.POINTER(C.c_float)
 class MmfConfig(C.Structure):
     _fields_ = [("vocab_size", _sz), ("hidden_size", _sz), ("num_hidden_layers", _sz),
                 ("intermediate_size", _sz), ("use_lower_bound", C.c_int), ("rms_norm_eps", C.c_float)]
+
+
+class MmfScanArgs(C.Structure):
+    _fields_ = ([("dtype", C.c_int), ("softplus", C.c_int)]
+                + [(n, _vp) for n in ("out", "u", "dt", "B", "C", "z", "A", "skip", "dt_bias", "state", "lens")]
+                + [(n, _sz) for n in ("seqs", "rows", "D", "N", "ldo", "ldu", "lddt", "ldb", "ldc", "ldz")])
 
 
 TOKEN_CB = C.CFUNCTYPE(None, _vp, C.c_int64)
@@ -75,6 +82,13 @@ def load_library(path: str = LIB_PATH):
         "mmf_swiglu": (i, [_vp, _vp, _vp, _vp, _sz]),
         "mmf_hgrn_scan": (i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp]),
         "mmf_rmsnorm_swishgate": (i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, C.c_float]),
+        "mmf_add_rmsnorm_q8": (i, [_vp, i] + [_vp] * 7 + [_sz] * 7 + [C.c_float]),
+        "mmf_w4_register": (i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, C.POINTER(i)]),
+        "mmf_w4_shape": (i, [_vp, i, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),
+        "mmf_w4_release": (i, [_vp, i]),
+        "mmf_w4_linear": (i, [_vp, i, i, _vp, _vp, i, _vp, _sz, _sz, _sz]),
+        "mmf_short_conv": (i, [_vp, i] + [_vp] * 6 + [_sz] * 4 + [i, _sz, _sz]),
+        "mmf_selective_scan": (i, [_vp, C.POINTER(MmfScanArgs)]),
         "mmf_model_begin": (i, [_vp, C.POINTER(MmfConfig)]),
         "mmf_model_tensor": (i, [_vp, C.c_char_p, i, C.POINTER(_sz), i, _vp]),
         "mmf_model_finalize": (i, [_vp, i, i]),
@@ -119,6 +133,13 @@ def _ptr(x):
 def _np(a, dtype):
     a = np.ascontiguousarray(a, dtype=dtype)
     return a, a.ctypes.data_as(C.c_void_p)
+
+
+def _lens(lens, seqs):
+    """(size_t array of sequence lengths or None, their number)."""
+    if lens is None:
+        return None, seqs
+    return C.cast((_sz * len(lens))(*[int(n) for n in lens]), _vp), len(lens)
 
 
 class Engine:
@@ -226,6 +247,57 @@ class Engine:
 
     def rmsnorm_swishgate(self, out, g, o, w, rows, cols, eps=1e-6):
         self._chk(self.lib.mmf_rmsnorm_swishgate(self.h, _ptr(out), _ptr(g), _ptr(o), _ptr(w), rows, cols, eps))
+
+    # ---- layer operators: rows of dtype F32, BF16 or F16, strides in elements (0: the row's length) ----
+    def add_rmsnorm_q8(self, codes, scales, x, w, rows, cols, res=None, h=None, y=None, eps=1e-6, dtype=F32, ldx=0,
+                       ldres=0, ldh=0, ldy=0, ldcodes=0):
+        """h = x + res, its RMS norm as int8 codes with a scale per row (mmf_add_rmsnorm_q8)."""
+        self._chk(self.lib.mmf_add_rmsnorm_q8(self.h, dtype, _ptr(codes), _ptr(scales), _ptr(x), _ptr(res), _ptr(h),
+                                              _ptr(y), _ptr(w), rows, cols, ldx, ldres, ldh, ldy, ldcodes, eps))
+
+    def register_w4(self, codes, scales, zeros=None, K=None, group=128) -> int:
+        """4-bit weights: codes uint8 [N, ceil(K/2)], scales float16 and zeros uint8 (or None: 8) [N, ceil(K/group)]."""
+        codes, cp = _np(codes, np.uint8)
+        scales, sp = _np(scales, np.float16)
+        N, K = codes.shape[0], 2 * codes.shape[1] if K is None else K
+        groups = -(-K // group) if group else 1
+        if codes.shape != (N, (K + 1) // 2) or scales.shape != (N, groups):
+            raise ValueError(f"codes {codes.shape} and scales {scales.shape} are not those of {N} x {K} in groups of {group}")
+        zp = None
+        if zeros is not None:
+            zeros, zp = _np(zeros, np.uint8)
+            if zeros.shape != scales.shape:
+                raise ValueError(f"zeros {zeros.shape} differ from scales {scales.shape}")
+        wid = C.c_int()
+        self._chk(self.lib.mmf_w4_register(self.h, cp, sp, zp, N, K, group, C.byref(wid)))
+        return wid.value
+
+    def w4_shape(self, wid):
+        n, k, g = _sz(), _sz(), _sz()
+        self._chk(self.lib.mmf_w4_shape(self.h, wid, C.byref(n), C.byref(k), C.byref(g)))
+        return n.value, k.value, g.value
+
+    def w4_release(self, wid):
+        self._chk(self.lib.mmf_w4_release(self.h, wid))
+
+    def w4_linear(self, wid, x, out, rows, dtype=F32, out_dtype=F32, scales=None, ldx=0, ldo=0):
+        """out [rows, N] = x [rows, K] times 4-bit weights; dtype I8: codes with their scales [rows]."""
+        self._chk(self.lib.mmf_w4_linear(self.h, wid, dtype, _ptr(x), _ptr(scales), out_dtype, _ptr(out), rows, ldx, ldo))
+
+    def short_conv(self, out, x, w, rows, D, width, bias=None, state=None, lens=None, seqs=1, silu=True, dtype=F32,
+                   ldx=0, ldo=0):
+        """Short causal convolution of sequences of the lengths lens (None: `seqs` equal ones)."""
+        lp, n = _lens(lens, seqs)
+        self._chk(self.lib.mmf_short_conv(self.h, dtype, _ptr(out), _ptr(x), _ptr(w), _ptr(bias), _ptr(state), lp, n,
+                                          rows, D, width, int(silu), ldx, ldo))
+
+    def selective_scan(self, out, u, dt, A, B, C, rows, D, N, skip=None, z=None, dt_bias=None, state=None, lens=None,
+                       seqs=1, softplus=True, dtype=F32, ldo=0, ldu=0, lddt=0, ldb=0, ldc=0, ldz=0):
+        """Selective state space scan of sequences of the lengths lens (None: `seqs` equal ones)."""
+        lp, n = _lens(lens, seqs)
+        a = MmfScanArgs(dtype, int(softplus), _ptr(out), _ptr(u), _ptr(dt), _ptr(B), _ptr(C), _ptr(z), _ptr(A),
+                        _ptr(skip), _ptr(dt_bias), _ptr(state), lp, n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
+        self._chk(self.lib.mmf_selective_scan(self.h, a))
 
     # ---- model ----
     def load_blob(self, path_or_blob, mode=FLOAT, frac_bits=10):

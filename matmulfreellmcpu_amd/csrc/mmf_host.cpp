@@ -21,6 +21,7 @@
 
 #include "../../include/mmfree_hip.h"
 #include "mmf_internal.hpp"
+#include "mmf_layer_dev.hpp"
 
 using namespace mmf;
 
@@ -94,6 +95,13 @@ struct Proj {
   ProjDev d;
   void* mem = nullptr;   // pk | tail | rowsum | normw in one allocation
   void* mem4 = nullptr;  // pk4 (float-mode models only)
+};
+
+// 4-bit weights (mmf_w4_register): codes and scales in one allocation.
+struct W4 {
+  W4Geom g{};
+  void* mem = nullptr;
+  const uint32_t *codes = nullptr, *scales = nullptr;
 };
 
 struct DevTensor {
@@ -196,6 +204,7 @@ struct mmf_ctx {
   hipStream_t stream = nullptr;
   std::string err;
   std::vector<Proj> projs;
+  std::vector<W4> w4s;
   Model model;
   DBuf raw;  // staging for int8 weights before the repack
   DBuf opy, opq, opct, opsa, opstate;
@@ -1067,6 +1076,8 @@ void mmf_destroy(mmf_ctx* c) {
     if (p.mem) (void)hipFree(p.mem);
     if (p.mem4) (void)hipFree(p.mem4);
   }
+  for (auto& w : c->w4s)
+    if (w.mem) (void)hipFree(w.mem);
   for (auto& kv : c->model.tensors)
     if (kv.second.p) (void)hipFree(kv.second.p);
   Model& m = c->model;
@@ -1518,6 +1529,109 @@ int mmf_rmsnorm_swishgate(mmf_ctx* c, float* out, const float* g, const float* o
   return guard(c, [&] {
     if (rows && cols)
       MMF_HIP(launch_swishgate(g, o, w, out, static_cast<int>(rows), static_cast<int>(cols), eps, c->stream));
+  });
+}
+
+// ---- layer operators ----------------------------------------------------------------------
+extern "C++" {
+static void refuse(const char* why) {
+  if (why) fail(MMF_ERR_ARG, why);
+}
+static const W4& w4_of(mmf_ctx* c, int id) {
+  if (id < 0 || id >= static_cast<int>(c->w4s.size())) fail(MMF_ERR_ARG, "invalid w4_id " + std::to_string(id));
+  if (!c->w4s[id].mem) fail(MMF_ERR_ARG, "w4_id " + std::to_string(id) + " was released");
+  return c->w4s[id];
+}
+}  // extern "C++"
+
+int mmf_add_rmsnorm_q8(mmf_ctx* c, int dtype, int8_t* codes, float* scales, const void* x, const void* res, void* h,
+                       void* y, const float* w, size_t rows, size_t cols, size_t ldx, size_t ldres, size_t ldh,
+                       size_t ldy, size_t ldcodes, float eps) {
+  return guard(c, [&] {
+    NormQArgs a{dtype, x, res, w, h, y, codes, scales, rows, cols, ldx, ldres, ldh, ldy, ldcodes, eps};
+    refuse(check(a));
+    MMF_HIP(launch_normq(a, c->stream));
+  });
+}
+
+int mmf_w4_register(mmf_ctx* c, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, size_t N, size_t K,
+                    size_t group, int* w4_id) {
+  return guard(c, [&] {
+    if (!codes || !scales || !w4_id) fail(MMF_ERR_ARG, "null argument");
+    refuse(check_w4(N, K, group));
+    W4 w;
+    w.g = w4_geom(N, K, group);
+    const size_t groups = (K + w.g.group - 1) / w.g.group, nc = N * ((K + 1) / 2), ns = N * groups * 2,
+                 nz = zeros ? N * groups : 0;
+    for (size_t i = 0; i < nz; ++i)
+      if (zeros[i] > 15) fail(MMF_ERR_ARG, "zero points must be 0..15");
+    char* raw = static_cast<char*>(c->raw.get((nc + 15) / 16 * 16 + ns + nz));
+    char* raw_s = raw + (nc + 15) / 16 * 16;
+    MMF_HIP(hipMemcpyAsync(raw, codes, nc, hipMemcpyHostToDevice, c->stream));
+    MMF_HIP(hipMemcpyAsync(raw_s, scales, ns, hipMemcpyHostToDevice, c->stream));
+    if (nz) MMF_HIP(hipMemcpyAsync(raw_s + ns, zeros, nz, hipMemcpyHostToDevice, c->stream));
+    c->w4s.reserve(c->w4s.size() + 1);  // so that nothing below throws away the allocation
+    MMF_HIP(hipMalloc(&w.mem, w4_code_bytes(w.g) + w4_scale_bytes(w.g)));
+    w.codes = static_cast<const uint32_t*>(w.mem);
+    w.scales = w.codes + w4_code_bytes(w.g) / 4;
+    hipError_t e = launch_w4_pack(reinterpret_cast<const uint8_t*>(raw), reinterpret_cast<const uint16_t*>(raw_s),
+                                  nz ? reinterpret_cast<const uint8_t*>(raw_s + ns) : nullptr, w.g,
+                                  const_cast<uint32_t*>(w.codes), const_cast<uint32_t*>(w.scales), c->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(c->stream);  // the caller's arrays have been read
+    if (e != hipSuccess) {
+      (void)hipFree(w.mem);
+      MMF_HIP(e);
+    }
+    c->w4s.push_back(w);
+    *w4_id = static_cast<int>(c->w4s.size() - 1);
+  });
+}
+
+int mmf_w4_shape(mmf_ctx* c, int id, size_t* N, size_t* K, size_t* group) {
+  return guard(c, [&] {
+    const W4& w = w4_of(c, id);
+    if (N) *N = w.g.N;
+    if (K) *K = w.g.K;
+    if (group) *group = w.g.group;
+  });
+}
+
+int mmf_w4_release(mmf_ctx* c, int id) {
+  return guard(c, [&] {
+    (void)w4_of(c, id);
+    MMF_HIP(hipStreamSynchronize(c->stream));
+    MMF_HIP(hipFree(c->w4s[id].mem));
+    c->w4s[id] = W4{};
+  });
+}
+
+int mmf_w4_linear(mmf_ctx* c, int id, int dtype, const void* x, const float* xscales, int out_dtype, void* out,
+                  size_t rows, size_t ldx, size_t ldo) {
+  return guard(c, [&] {
+    const W4& w = w4_of(c, id);
+    W4Args a{dtype, out_dtype, x, xscales, out, rows, ldx, ldo};
+    refuse(check(a, w.g.N, w.g.K));
+    MMF_HIP(launch_w4(a, w.g, w.codes, w.scales, c->stream));
+  });
+}
+
+int mmf_short_conv(mmf_ctx* c, int dtype, void* out, const void* x, const float* w, const float* bias, float* state,
+                   const size_t* lens, size_t seqs, size_t rows, size_t D, size_t width, int silu, size_t ldx,
+                   size_t ldo) {
+  return guard(c, [&] {
+    ConvArgs a{dtype, silu, out, x, w, bias, state, lens, seqs, rows, D, width, ldx, ldo};
+    refuse(check(a));
+    MMF_HIP(launch_conv(a, c->stream));
+  });
+}
+
+int mmf_selective_scan(mmf_ctx* c, const mmf_scan_args* s) {
+  return guard(c, [&] {
+    if (!s) fail(MMF_ERR_ARG, "null argument");
+    ScanArgs a{s->dtype, s->softplus, s->out, s->u, s->dt, s->B, s->C, s->z, s->A, s->skip, s->dt_bias, s->state,
+               s->lens, s->seqs, s->rows, s->D, s->N, s->ldo, s->ldu, s->lddt, s->ldb, s->ldc, s->ldz};
+    refuse(check(a));
+    MMF_HIP(launch_sel_scan(a, c->stream));
   });
 }
 

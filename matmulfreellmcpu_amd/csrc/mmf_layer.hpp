@@ -1,0 +1,286 @@
+// mmf_layer.hpp -- the operators of a recurrent low-bit layer: arguments, checks and launch plans.
+//
+// Plain C++ without HIP, so that the checks and the plans also compile, and are tested, on a host
+// without a device. The kernels are in mmf_normq.hip, mmf_w4.hip, mmf_conv.hip and mmf_scan.hip.
+// A row tensor is `rows` rows of `cols` elements, ld elements apart (ld >= cols), at any address
+// that its element type is aligned at.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#ifdef __HIPCC__
+#define MMF_HD __host__ __device__
+#else
+#define MMF_HD
+#endif
+
+namespace mmf {
+
+enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2, kI8 = 3 };
+
+inline size_t dtype_size(int t) { return t == kF32 ? 4 : t == kI8 ? 1 : 2; }
+inline bool float_type(int t) { return t == kF32 || t == kBF16 || t == kF16; }
+
+constexpr size_t kMaxRows = size_t{1} << 24;  // of one call, as mmf_bitlinear
+constexpr size_t kMaxCols = size_t{1} << 20;  // channels, columns
+constexpr size_t kMaxLd = size_t{1} << 31;
+
+// A row tensor's memory.
+struct RowsOf {
+  const void* p;
+  size_t ld, cols, esize;
+};
+
+inline bool rows_aligned(const RowsOf& a) { return reinterpret_cast<uintptr_t>(a.p) % a.esize == 0; }
+
+// Whether two row tensors of `rows` rows share an element. Tensors that are column ranges of one
+// buffer (the same ld) overlap only if their columns do; others are compared by their whole ranges.
+inline bool rows_overlap(const RowsOf& a, const RowsOf& b, size_t rows) {
+  if (!rows || !a.p || !b.p || !a.cols || !b.cols) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+  const uintptr_t ea = pa + ((rows - 1) * a.ld + a.cols) * a.esize, eb = pb + ((rows - 1) * b.ld + b.cols) * b.esize;
+  if (ea <= pb || eb <= pa) return false;
+  const size_t step = a.ld * a.esize;
+  if (step != b.ld * b.esize) return true;
+  const size_t d = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;
+  return d < a.cols * a.esize || d + b.cols * b.esize > step;
+}
+inline bool same_rows(const RowsOf& a, const RowsOf& b) { return a.p == b.p && a.ld == b.ld && a.esize == b.esize; }
+
+// ---- residual addition, RMS norm and int8 codes ------------------------------------------------
+struct NormQArgs {
+  int dtype;             // of x, res, h, y
+  const void *x, *res;   // res may be null
+  const float* w;        // [cols]
+  void *h, *y;           // may be null
+  int8_t* codes;
+  float* scales;         // [rows]
+  size_t rows, cols, ldx, ldres, ldh, ldy, ldcodes;
+  float eps;
+};
+
+// The reason why a call is refused, or null. A zero ld means cols.
+inline const char* check(NormQArgs& a) {
+  if (!float_type(a.dtype)) return "dtype must be MMF_F32, MMF_BF16 or MMF_F16";
+  if (a.rows > kMaxRows) return "too many rows";
+  if (a.cols > kMaxCols) return "rows are too long";
+  for (size_t* ld : {&a.ldx, &a.ldres, &a.ldh, &a.ldy, &a.ldcodes}) {
+    if (!*ld) *ld = a.cols;
+    if (*ld < a.cols || *ld > kMaxLd) return "a row stride is smaller than the row, or too large";
+  }
+  if (!a.rows || !a.cols) return nullptr;
+  if (!a.x || !a.w || !a.codes || !a.scales) return "null argument";
+  const size_t es = dtype_size(a.dtype);
+  const RowsOf x{a.x, a.ldx, a.cols, es}, r{a.res, a.ldres, a.cols, es}, h{a.h, a.ldh, a.cols, es},
+      y{a.y, a.ldy, a.cols, es}, c{a.codes, a.ldcodes, a.cols, 1}, s{a.scales, 1, 1, 4}, w{a.w, a.cols, a.cols, 4};
+  for (const RowsOf& t : {x, r, h, y, s, w})
+    if (!rows_aligned(t)) return "a pointer is not aligned to its type";
+  for (const RowsOf& in : {x, r})
+    if (a.h && !same_rows(h, in) && rows_overlap(h, in, a.rows)) return "h overlaps an input (it may be x or res itself)";
+  for (const RowsOf& in : {x, r, h})
+    if (rows_overlap(y, in, a.rows) || rows_overlap(c, in, a.rows)) return "an output overlaps another tensor of the call";
+  if (rows_overlap(y, c, a.rows)) return "an output overlaps another tensor of the call";
+  return nullptr;
+}
+
+// ---- products with 4-bit weights ----------------------------------------------------------------
+// Weights laid out for the kernels. Outputs go in tiles of 16 and inputs in chunks of 128, padded:
+//   codes [ntile][chunk][lane 0..63][word 0..3]: lane l holds output 16 ntile + l % 16, and word j
+//     the 8 inputs from 128 chunk + w4_k(step, j, l / 16). Element e of a word sits at bits
+//     3 + 4 w4_nibble(e) (rotated by 3, so that one AND and one OR make two 16-bit floats of it).
+//   scales [ntile][w4_subs * nchunk][16]: the fp16 scale in the low half, the zero point above it.
+// step is the kernel's scale granularity, 32, 64 or 128 inputs: the largest that divides the group
+// (of rows that are one group: 128).
+struct W4Geom {
+  int N, K, group, step, nt, nc, ns;  // tiles of 16 outputs, chunks of 128 inputs, scales a tile row
+};
+inline W4Geom w4_geom(size_t N, size_t K, size_t group) {
+  W4Geom g;
+  g.N = static_cast<int>(N);
+  g.K = static_cast<int>(K);
+  g.group = static_cast<int>(group ? group : K);
+  g.step = !group || group >= K || group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32;
+  g.nt = static_cast<int>((N + 15) / 16);
+  g.nc = static_cast<int>((K + 127) / 128);
+  g.ns = g.nc * (128 / g.step);
+  return g;
+}
+// First input (within its chunk) of word j of a lane of lane group q = lane / 16. With scales every 32
+// inputs a matrix instruction's 32 inputs are neighbours; otherwise each lane's 16 of a half chunk are.
+MMF_HD inline constexpr int w4_k(int step, int j, int q) {
+  return step == 32 ? 32 * j + 8 * q : 64 * (j >> 1) + 16 * q + 8 * (j & 1);
+}
+// Nibble of element e (0..7) of a word: neighbours 2p and 2p + 1 are nibbles p and p + 4, the same bits
+// of the word's two halves, so that one mask makes a pair of 16-bit floats of them.
+MMF_HD inline constexpr int w4_nibble(int e) { return 4 * (e & 1) + (e >> 1); }
+MMF_HD inline size_t w4_code_bytes(const W4Geom& g) { return static_cast<size_t>(g.nt) * g.nc * 1024; }
+MMF_HD inline size_t w4_scale_bytes(const W4Geom& g) { return static_cast<size_t>(g.nt) * g.ns * 64; }
+
+inline const char* check_w4(size_t N, size_t K, size_t group) {
+  if (!N || !K || N > kMaxCols || K > kMaxCols) return "invalid 4-bit weight shape";
+  if (group % 32) return "the group must be a multiple of 32 inputs, or 0 for whole rows";
+  return nullptr;
+}
+
+struct W4Args {
+  int dtype, out_dtype;
+  const void* x;
+  const float* xscales;  // MMF_I8: a scale per row
+  void* out;
+  size_t rows, ldx, ldo;
+};
+inline const char* check(W4Args& a, size_t N, size_t K) {
+  if (!float_type(a.dtype) && a.dtype != kI8) return "dtype must be MMF_F32, MMF_BF16, MMF_F16 or MMF_I8";
+  if (!float_type(a.out_dtype)) return "out_dtype must be MMF_F32, MMF_BF16 or MMF_F16";
+  if (a.rows > kMaxRows) return "too many rows";
+  if (!a.ldx) a.ldx = K;
+  if (!a.ldo) a.ldo = N;
+  if (a.ldx < K || a.ldo < N || a.ldx > kMaxLd || a.ldo > kMaxLd)
+    return "a row stride is smaller than the row, or too large";
+  if (!a.rows) return nullptr;
+  if (!a.x || !a.out) return "null argument";
+  if ((a.dtype == kI8) != (a.xscales != nullptr)) return "int8 rows need their scales, and other rows have none";
+  const RowsOf x{a.x, a.ldx, K, dtype_size(a.dtype)}, o{a.out, a.ldo, N, dtype_size(a.out_dtype)},
+      s{a.xscales, 1, 1, 4};
+  if (!rows_aligned(x) || !rows_aligned(o) || !rows_aligned(s)) return "a pointer is not aligned to its type";
+  if (rows_overlap(x, o, a.rows) || rows_overlap(s, o, a.rows)) return "the output overlaps an input";
+  return nullptr;
+}
+
+// ---- packed sequences ---------------------------------------------------------------------------
+// Rows of several sequences, one after the other. A launch takes up to kSeqs sequences, whose first
+// rows and first tiles travel as a kernel argument; sequences of one length need no table.
+constexpr int kSeqs = 240;
+struct SeqTab {
+  int n;                  // sequences of this launch
+  int len, tiles;         // of each, where all are alike (len > 0)
+  int row[kSeqs + 1];     // else: first row of each, from the launch's first
+  int tile[kSeqs + 1];    // first tile of each
+};
+
+inline const char* check_seqs(const size_t* lens, size_t seqs, size_t rows) {
+  if (seqs > kMaxRows) return "too many sequences";
+  if (!seqs) return rows ? "rows without a sequence" : nullptr;
+  if (!lens) return rows % seqs ? "the rows do not divide into the sequences" : nullptr;
+  size_t sum = 0;
+  for (size_t i = 0; i < seqs; ++i) {
+    if (lens[i] > rows) return "a sequence is longer than the rows";
+    sum += lens[i];
+    if (sum > rows) return "the sequences' lengths exceed the rows";
+  }
+  return sum == rows ? nullptr : "the sequences' lengths do not sum to the rows";
+}
+
+// The table of sequences [first, first + n) with tiles of `step` rows; returns its rows, and tiles
+// in *ntiles.
+inline size_t fill_seqs(SeqTab& t, const size_t* lens, size_t rows, size_t seqs, size_t first, int n, int step,
+                        int* ntiles) {
+  t.n = n;
+  const size_t l0 = lens ? lens[first] : rows / seqs;
+  bool alike = true;
+  for (int i = 1; lens && i < n; ++i) alike = alike && lens[first + i] == l0;
+  t.len = alike ? static_cast<int>(l0) : 0;
+  t.tiles = static_cast<int>((l0 + step - 1) / step);
+  if (alike) {
+    *ntiles = n * t.tiles;
+    return n * l0;
+  }
+  int r = 0, k = 0;
+  for (int i = 0; i < n; ++i) {
+    t.row[i] = r;
+    t.tile[i] = k;
+    r += static_cast<int>(lens[first + i]);
+    k += static_cast<int>((lens[first + i] + step - 1) / step);
+  }
+  t.row[n] = r;
+  t.tile[n] = k;
+  *ntiles = k;
+  return r;
+}
+
+// ---- short causal convolution -------------------------------------------------------------------
+constexpr size_t kMaxWidth = 8;
+struct ConvArgs {
+  int dtype, silu;
+  void* out;
+  const void* x;
+  const float *w, *bias;  // [D, width], [D] or null
+  float* state;           // [seqs, width - 1, D] or null
+  const size_t* lens;
+  size_t seqs, rows, D, width, ldx, ldo;
+};
+inline const char* check(ConvArgs& a) {
+  if (!float_type(a.dtype)) return "dtype must be MMF_F32, MMF_BF16 or MMF_F16";
+  if (a.rows > kMaxRows) return "too many rows";
+  if (a.D > kMaxCols) return "too many channels";
+  if (!a.width || a.width > kMaxWidth) return "the width must be 1..8";
+  if (!a.ldx) a.ldx = a.D;
+  if (!a.ldo) a.ldo = a.D;
+  if (a.ldx < a.D || a.ldo < a.D || a.ldx > kMaxLd || a.ldo > kMaxLd)
+    return "a row stride is smaller than the row, or too large";
+  if (const char* e = check_seqs(a.lens, a.seqs, a.rows)) return e;
+  if (!a.rows || !a.D) return nullptr;
+  if (!a.out || !a.x || !a.w) return "null argument";
+  const size_t es = dtype_size(a.dtype), held = (a.width - 1) * a.D;
+  const RowsOf x{a.x, a.ldx, a.D, es}, o{a.out, a.ldo, a.D, es}, w{a.w, 1, 1, 4}, b{a.bias, 1, 1, 4},
+      s{a.state, 1, 1, 4};
+  for (const RowsOf& t : {x, o, w, b, s})
+    if (!rows_aligned(t)) return "a pointer is not aligned to its type";
+  if (rows_overlap(x, o, a.rows)) return "the output overlaps the input";
+  const RowsOf whole{a.state, a.seqs * held, a.seqs * held, 4};
+  for (const RowsOf& t : {x, o}) {
+    const size_t all = (a.rows - 1) * t.ld + t.cols;
+    if (rows_overlap(whole, RowsOf{t.p, all, all, es}, 1)) return "the state overlaps another tensor of the call";
+  }
+  return nullptr;
+}
+
+// ---- selective state space scan -----------------------------------------------------------------
+constexpr size_t kMaxStates = 128;
+struct ScanArgs {
+  int dtype, softplus;
+  void* out;
+  const void *u, *dt, *B, *C, *z;       // z may be null
+  const float *A, *skip, *dt_bias;      // [D, N], [D] or null, [D] or null
+  float* state;                         // [seqs, N, D] or null
+  const size_t* lens;
+  size_t seqs, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz;
+};
+inline const char* check(ScanArgs& a) {
+  if (!float_type(a.dtype)) return "dtype must be MMF_F32, MMF_BF16 or MMF_F16";
+  if (a.rows > kMaxRows) return "too many rows";
+  if (a.D > kMaxCols) return "too many channels";
+  if (!a.N || a.N > kMaxStates) return "the states per channel must be 1..128";
+  for (size_t* ld : {&a.ldo, &a.ldu, &a.lddt, &a.ldz}) {
+    if (!*ld) *ld = a.D;
+    if (*ld < a.D || *ld > kMaxLd) return "a row stride is smaller than the row, or too large";
+  }
+  for (size_t* ld : {&a.ldb, &a.ldc}) {
+    if (!*ld) *ld = a.N;
+    if (*ld < a.N || *ld > kMaxLd) return "a row stride is smaller than the row, or too large";
+  }
+  if (const char* e = check_seqs(a.lens, a.seqs, a.rows)) return e;
+  if (!a.rows || !a.D) return nullptr;
+  if (!a.out || !a.u || !a.dt || !a.A || !a.B || !a.C) return "null argument";
+  const size_t es = dtype_size(a.dtype);
+  const RowsOf o{a.out, a.ldo, a.D, es};
+  const RowsOf ins[] = {{a.u, a.ldu, a.D, es}, {a.dt, a.lddt, a.D, es}, {a.B, a.ldb, a.N, es}, {a.C, a.ldc, a.N, es},
+                        {a.z, a.ldz, a.D, es}};
+  const size_t held = a.seqs * a.N * a.D;
+  const RowsOf whole{a.state, held, held, 4};
+  if (!rows_aligned(o)) return "a pointer is not aligned to its type";
+  for (const RowsOf& t : ins) {
+    if (!rows_aligned(t)) return "a pointer is not aligned to its type";
+    if (rows_overlap(o, t, a.rows)) return "the output overlaps an input";
+    const size_t all = (a.rows - 1) * t.ld + t.cols;
+    if (rows_overlap(whole, RowsOf{t.p, all, all, es}, 1)) return "the state overlaps another tensor of the call";
+  }
+  for (const float* p : {a.A, a.skip, a.dt_bias, static_cast<const float*>(a.state)})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return "a pointer is not aligned to its type";
+  const size_t all = (a.rows - 1) * a.ldo + a.D;
+  if (rows_overlap(whole, RowsOf{a.out, all, all, es}, 1)) return "the state overlaps another tensor of the call";
+  return nullptr;
+}
+
+}  // namespace mmf

@@ -1,0 +1,212 @@
+// Checks and plans of the layer operators (csrc/mmf_layer.hpp) on the host: prints a line for every
+// expectation that does not hold and exits with their number.
+#include <cstdio>
+#include <cstring>
+#include <set>
+#include <vector>
+
+#include "../matmulfreellmcpu_amd/csrc/mmf_layer.hpp"
+
+using namespace mmf;
+
+static int bad = 0;
+static void want(const char* what, const char* got, const char* part) {
+  const bool ok = part ? got && std::strstr(got, part) : !got;
+  if (!ok) {
+    std::printf("%s: got '%s', wanted '%s'\n", what, got ? got : "accepted", part ? part : "accepted");
+    ++bad;
+  }
+}
+static void is(const char* what, long got, long expect) {
+  if (got != expect) {
+    std::printf("%s: got %ld, wanted %ld\n", what, got, expect);
+    ++bad;
+  }
+}
+
+// addresses only: nothing here is read
+template <class T> static T* at(uintptr_t a) { return reinterpret_cast<T*>(a); }
+
+static NormQArgs norm() {
+  return {kF32, at<float>(0x10000), at<float>(0x20000), at<float>(0x900), at<float>(0x30000), nullptr,
+          at<int8_t>(0x40000), at<float>(0x50000), 4, 100, 0, 0, 0, 0, 0, 1e-6f};
+}
+static void norms() {
+  auto go = [](const char* what, const char* part, auto&& change) {
+    NormQArgs a = norm();
+    change(a);
+    want(what, check(a), part);
+  };
+  go("norm", nullptr, [](NormQArgs&) {});
+  go("norm type", "dtype", [](NormQArgs& a) { a.dtype = kI8; });
+  go("norm type below", "dtype", [](NormQArgs& a) { a.dtype = -1; });
+  go("norm stride", "stride", [](NormQArgs& a) { a.ldx = 99; });
+  go("norm wide stride", "stride", [](NormQArgs& a) { a.ldcodes = size_t{1} << 32; });
+  go("norm null x", "null", [](NormQArgs& a) { a.x = nullptr; });
+  go("norm null codes", "null", [](NormQArgs& a) { a.codes = nullptr; });
+  go("norm null scales", "null", [](NormQArgs& a) { a.scales = nullptr; });
+  go("norm null w", "null", [](NormQArgs& a) { a.w = nullptr; });
+  go("norm no rows", nullptr, [](NormQArgs& a) { a.rows = 0, a.x = nullptr; });
+  go("norm no columns", nullptr, [](NormQArgs& a) { a.cols = 0; });
+  go("norm many rows", "rows", [](NormQArgs& a) { a.rows = kMaxRows + 1; });
+  go("norm long rows", "long", [](NormQArgs& a) { a.cols = kMaxCols + 1; });
+  go("norm odd address", "aligned", [](NormQArgs& a) { a.x = at<char>(0x10002); });
+  go("norm bf16 at 2 bytes", nullptr, [](NormQArgs& a) { a.dtype = kBF16, a.x = at<char>(0x10002); });
+  go("norm no residual", nullptr, [](NormQArgs& a) { a.res = nullptr; });
+  go("norm h in place of x", nullptr, [](NormQArgs& a) { a.h = const_cast<void*>(a.x); });
+  go("norm h in place of res", nullptr, [](NormQArgs& a) { a.h = const_cast<void*>(a.res); });
+  go("norm h shifted", "overlaps", [](NormQArgs& a) { a.h = at<float>(0x20004); });
+  go("norm h in place, other stride", "overlaps", [](NormQArgs& a) { a.h = const_cast<void*>(a.x), a.ldh = 101; });
+  go("norm y on x", "overlaps", [](NormQArgs& a) { a.y = const_cast<void*>(a.x); });
+  go("norm y on h", "overlaps", [](NormQArgs& a) { a.y = a.h; });
+  go("norm codes on x", "overlaps", [](NormQArgs& a) { a.codes = at<int8_t>(0x10010); });
+  go("norm codes on y", "overlaps", [](NormQArgs& a) { a.y = at<float>(0x60000), a.codes = at<int8_t>(0x60001); });
+  go("norm neighbours in one buffer", nullptr,
+     [](NormQArgs& a) { a.ldx = a.ldh = 200, a.h = at<float>(0x10000 + 400); });
+  go("norm touching neighbours", "overlaps",
+     [](NormQArgs& a) { a.ldx = a.ldh = 200, a.h = at<float>(0x10000 + 396); });
+}
+
+static void products() {
+  want("w4 shape", check_w4(100, 77, 32), nullptr);
+  want("w4 whole rows", check_w4(100, 77, 0), nullptr);
+  want("w4 no outputs", check_w4(0, 77, 32), "shape");
+  want("w4 no inputs", check_w4(7, 0, 32), "shape");
+  want("w4 too large", check_w4(kMaxCols + 1, 7, 32), "shape");
+  want("w4 group", check_w4(7, 100, 48), "group");
+  auto go = [](const char* what, const char* part, auto&& change) {
+    W4Args a{kF32, kF32, at<float>(0x10000), nullptr, at<float>(0x20000), 4, 0, 0};
+    change(a);
+    want(what, check(a, 100, 64), part);
+  };
+  go("w4", nullptr, [](W4Args&) {});
+  go("w4 type", "dtype", [](W4Args& a) { a.dtype = 4; });
+  go("w4 out type", "out_dtype", [](W4Args& a) { a.out_dtype = kI8; });
+  go("w4 int8 without scales", "scales", [](W4Args& a) { a.dtype = kI8; });
+  go("w4 int8", nullptr, [](W4Args& a) { a.dtype = kI8, a.xscales = at<float>(0x900); });
+  go("w4 scales without int8", "scales", [](W4Args& a) { a.xscales = at<float>(0x900); });
+  go("w4 stride", "stride", [](W4Args& a) { a.ldx = 63; });
+  go("w4 out stride", "stride", [](W4Args& a) { a.ldo = 99; });
+  go("w4 null", "null", [](W4Args& a) { a.out = nullptr; });
+  go("w4 no rows", nullptr, [](W4Args& a) { a.rows = 0, a.x = nullptr; });
+  go("w4 alignment", "aligned", [](W4Args& a) { a.out_dtype = kBF16, a.out = at<char>(0x20001); });
+  go("w4 overlap", "overlaps", [](W4Args& a) { a.out = at<char>(0x10040); });
+
+  // the packed layout holds every code and scale once, within its bytes
+  const size_t shapes[][3] = {{1, 1, 32}, {17, 1031, 32}, {33, 129, 64}, {16, 128, 128}, {100, 96, 96}, {5, 300, 0},
+                              {40, 700, 256}, {3, 64, 1024}, {48, 640, 192}};
+  for (auto& s : shapes) {
+    const W4Geom g = w4_geom(s[0], s[1], s[2]);
+    is("w4 step divides the group or the row is one", s[2] == 0 || s[2] >= s[1] || s[2] % g.step == 0, 1);
+    std::set<size_t> seen;
+    for (int k = 0; k < g.nc * 128; ++k) {
+      int found = 0;
+      for (int q = 0; q < 4; ++q)
+        for (int j = 0; j < 4; ++j)
+          for (int e = 0; e < 8; ++e)
+            if (k / 128 * 128 + w4_k(g.step, j, q) + e == k) {
+              ++found;
+              seen.insert(((static_cast<size_t>(k / 128) * 4 + q) * 4 + j) * 8 + w4_nibble(e));
+              // all inputs of a word, and of a matrix instruction's lane groups, share a scale
+              is("w4 word within a scale", (k % 128) / g.step, w4_k(g.step, j, q) / g.step);
+              is("w4 instruction within a scale", w4_k(g.step, j, q) / g.step, w4_k(g.step, j, 0) / g.step);
+            }
+      is("w4 places of an input", found, 1);
+    }
+    is("w4 nibbles", static_cast<long>(seen.size()), g.nc * 128);
+    is("w4 tiles", g.nt * 16 >= g.N && (g.nt - 1) * 16 < g.N, 1);
+    is("w4 scale columns", g.ns * g.step, g.nc * 128);
+  }
+}
+
+static void sequences() {
+  const size_t lens[] = {3, 0, 5, 9, 0};
+  want("lens", check_seqs(lens, 5, 17), nullptr);
+  want("lens short", check_seqs(lens, 5, 18), "sum");
+  want("lens long", check_seqs(lens, 5, 16), "exceed");
+  want("lens one too long", check_seqs(lens, 5, 8), "longer");
+  const size_t wraps[] = {~size_t{0}, 2};
+  want("lens wrap", check_seqs(wraps, 2, 1), "longer");
+  want("equal", check_seqs(nullptr, 4, 12), nullptr);
+  want("unequal", check_seqs(nullptr, 5, 12), "divide");
+  want("none", check_seqs(nullptr, 0, 0), nullptr);
+  want("rows of none", check_seqs(nullptr, 0, 3), "without");
+
+  SeqTab t;
+  int tiles = 0;
+  is("rows of table", fill_seqs(t, lens, 17, 5, 0, 5, 4, &tiles), 17);
+  is("tiles", tiles, 1 + 0 + 2 + 3 + 0);
+  is("ragged", t.len, 0);
+  is("last row", t.row[5], 17);
+  for (int k = 0; k < tiles; ++k) {  // the search of the kernels: sequences whose first tile is at or before k
+    int below = 0;
+    for (int i = 0; i < t.n; ++i) below += t.tile[i] <= k;
+    const int seq = below - 1;
+    is("tile in its sequence", t.tile[seq] <= k && k < t.tile[seq + 1], 1);
+    is("tile has rows", lens[seq] > static_cast<size_t>(k - t.tile[seq]) * 4, 1);
+  }
+  is("part of a table", fill_seqs(t, lens, 17, 5, 2, 2, 4, &tiles), 14);
+  is("its tiles", tiles, 5);
+  is("equal rows", fill_seqs(t, nullptr, 12, 4, 1, 3, 2, &tiles), 9);
+  is("equal tiles", tiles, 6);
+  const size_t none[] = {0, 0, 0};
+  is("no rows", fill_seqs(t, none, 0, 3, 0, 3, 4, &tiles), 0);
+  is("no tiles", tiles, 0);
+}
+
+static void mixers() {
+  const size_t lens[] = {2, 2};
+  auto conv = [&](const char* what, const char* part, auto&& change) {
+    ConvArgs a{kF32, 1, at<float>(0x20000), at<float>(0x10000), at<float>(0x900), nullptr, at<float>(0x30000),
+               lens, 2, 4, 64, 4, 0, 0};
+    change(a);
+    want(what, check(a), part);
+  };
+  conv("conv", nullptr, [](ConvArgs&) {});
+  conv("conv type", "dtype", [](ConvArgs& a) { a.dtype = kI8; });
+  conv("conv width", "width", [](ConvArgs& a) { a.width = 9; });
+  conv("conv no width", "width", [](ConvArgs& a) { a.width = 0; });
+  conv("conv stride", "stride", [](ConvArgs& a) { a.ldo = 63; });
+  conv("conv lens", "sum", [](ConvArgs& a) { a.rows = 5; });
+  conv("conv null", "null", [](ConvArgs& a) { a.w = nullptr; });
+  conv("conv in place", "overlaps", [](ConvArgs& a) { a.out = const_cast<void*>(a.x); });
+  conv("conv state on x", "state", [](ConvArgs& a) { a.state = at<float>(0x10040); });
+  conv("conv state on out", "state", [](ConvArgs& a) { a.state = at<float>(0x20000 - 8); });
+  conv("conv alignment", "aligned", [](ConvArgs& a) { a.state = at<float>(0x30002); });
+  conv("conv no rows", nullptr, [](ConvArgs& a) { a.rows = 0, a.lens = nullptr; });
+  conv("conv halves of one buffer", nullptr,
+       [](ConvArgs& a) { a.ldx = a.ldo = 128, a.out = at<float>(0x10000 + 256); });
+
+  auto scan = [&](const char* what, const char* part, auto&& change) {
+    ScanArgs a{};
+    a.out = at<float>(0x20000), a.u = at<float>(0x10000), a.dt = at<float>(0x30000), a.B = at<float>(0x40000);
+    a.C = at<float>(0x50000), a.A = at<float>(0x900), a.state = at<float>(0x60000);
+    a.lens = lens, a.seqs = 2, a.rows = 4, a.D = 64, a.N = 16;
+    change(a);
+    want(what, check(a), part);
+  };
+  scan("scan", nullptr, [](ScanArgs&) {});
+  scan("scan type", "dtype", [](ScanArgs& a) { a.dtype = 7; });
+  scan("scan states", "states", [](ScanArgs& a) { a.N = 129; });
+  scan("scan no states", "states", [](ScanArgs& a) { a.N = 0; });
+  scan("scan stride", "stride", [](ScanArgs& a) { a.ldb = 15; });
+  scan("scan stride of u", "stride", [](ScanArgs& a) { a.ldu = 63; });
+  scan("scan lens", "exceed", [](ScanArgs& a) { a.rows = 3; });
+  scan("scan null", "null", [](ScanArgs& a) { a.dt = nullptr; });
+  scan("scan in place", "overlaps", [](ScanArgs& a) { a.out = const_cast<void*>(a.u); });
+  scan("scan on z", "overlaps", [](ScanArgs& a) { a.z = at<float>(0x20004); });
+  scan("scan state on B", "state", [](ScanArgs& a) { a.state = at<float>(0x40010); });
+  scan("scan state on out", "state", [](ScanArgs& a) { a.state = at<float>(0x20010); });
+  scan("scan alignment", "aligned", [](ScanArgs& a) { a.skip = at<float>(0x902); });
+  scan("scan B and C in one buffer", nullptr, [](ScanArgs& a) { a.ldb = a.ldc = 32, a.C = at<float>(0x40040); });
+  scan("scan no rows", nullptr, [](ScanArgs& a) { a.rows = 0, a.lens = nullptr, a.u = nullptr; });
+}
+
+int main() {
+  norms();
+  products();
+  sequences();
+  mixers();
+  std::printf("%d unmet\n", bad);
+  return bad ? 1 : 0;
+}
