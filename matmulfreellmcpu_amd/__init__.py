@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 
 import numpy as np
 
@@ -136,10 +137,11 @@ def _np(a, dtype):
 
 
 def _lens(lens, seqs):
-    """(size_t array of sequence lengths or None, their number)."""
+    """(sequence lengths as size_t array or None, its address, the number of sequences)."""
     if lens is None:
-        return None, seqs
-    return C.cast((_sz * len(lens))(*[int(n) for n in lens]), _vp), len(lens)
+        return None, None, seqs
+    a = array("Q", lens)
+    return a, a.buffer_info()[0], len(a)
 
 
 class Engine:
@@ -287,14 +289,14 @@ class Engine:
     def short_conv(self, out, x, w, rows, D, width, bias=None, state=None, lens=None, seqs=1, silu=True, dtype=F32,
                    ldx=0, ldo=0):
         """Short causal convolution of sequences of the lengths lens (None: `seqs` equal ones)."""
-        lp, n = _lens(lens, seqs)
+        _keep, lp, n = _lens(lens, seqs)
         self._chk(self.lib.mmf_short_conv(self.h, dtype, _ptr(out), _ptr(x), _ptr(w), _ptr(bias), _ptr(state), lp, n,
                                           rows, D, width, int(silu), ldx, ldo))
 
     def selective_scan(self, out, u, dt, A, B, C, rows, D, N, skip=None, z=None, dt_bias=None, state=None, lens=None,
                        seqs=1, softplus=True, dtype=F32, ldo=0, ldu=0, lddt=0, ldb=0, ldc=0, ldz=0):
         """Selective state space scan of sequences of the lengths lens (None: `seqs` equal ones)."""
-        lp, n = _lens(lens, seqs)
+        _keep, lp, n = _lens(lens, seqs)
         a = MmfScanArgs(dtype, int(softplus), _ptr(out), _ptr(u), _ptr(dt), _ptr(B), _ptr(C), _ptr(z), _ptr(A),
                         _ptr(skip), _ptr(dt_bias), _ptr(state), lp, n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
         self._chk(self.lib.mmf_selective_scan(self.h, a))

@@ -209,6 +209,7 @@ struct mmf_ctx {
   DBuf raw;  // staging for int8 weights before the repack
   DBuf opy, opq, opct, opsa, opstate;
   DBuf gws;  // split-K workspace of the matrix-core GEMM
+  DBuf layer_ws;          // the scan's chunks: allocated once, at its full size
   DBuf hmacc;             // mmf_ternary_matmul_host: large accumulators on the device
   PinBuf pin_x, pin_acc;  // ... and their pinned host staging
   hipDeviceProp_t prop{};
@@ -1092,7 +1093,7 @@ void mmf_destroy(mmf_ctx* c) {
   for (DBuf* b : {&ss.h, &ss.resid, &ss.g, &ss.recur, &ss.z, &ss.keys}) b->release();
   ss.io.release();
   ss.logits.release();
-  for (DBuf* b : {&c->raw, &c->opy, &c->opq, &c->opct, &c->opsa, &c->opstate, &c->gws, &c->hmacc})
+  for (DBuf* b : {&c->raw, &c->opy, &c->opq, &c->opct, &c->opsa, &c->opstate, &c->gws, &c->hmacc, &c->layer_ws})
     b->release();
   c->pin_x.release();
   c->pin_acc.release();
@@ -1481,7 +1482,7 @@ int mmf_workspace_bytes(mmf_ctx* c, size_t* bytes) {
   return guard(c, [&] {
     if (!bytes) fail(MMF_ERR_ARG, "null output");
     size_t n = 0;
-    for (const DBuf* b : {&c->opy, &c->opq, &c->opct, &c->opsa, &c->opstate, &c->gws}) n += b->n;
+    for (const DBuf* b : {&c->opy, &c->opq, &c->opct, &c->opsa, &c->opstate, &c->gws, &c->layer_ws}) n += b->n;
     *bytes = n;
   });
 }
@@ -1536,6 +1537,17 @@ int mmf_rmsnorm_swishgate(mmf_ctx* c, float* out, const float* g, const float* o
 extern "C++" {
 static void refuse(const char* why) {
   if (why) fail(MMF_ERR_ARG, why);
+}
+// The scan's workspace. It never grows, so that a captured graph's address of it stays good; its first
+// use cannot be inside a capture, which allocates nothing.
+static float* layer_ws(mmf_ctx* c) {
+  if (!c->layer_ws.p) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    MMF_HIP(hipStreamIsCapturing(c->stream, &st));
+    if (st != hipStreamCaptureStatusNone)
+      fail(MMF_ERR_STATE, "the first selective scan of long sequences allocates its workspace: run one before the capture");
+  }
+  return c->layer_ws.as<float>(kScanWsFloats);
 }
 static const W4& w4_of(mmf_ctx* c, int id) {
   if (id < 0 || id >= static_cast<int>(c->w4s.size())) fail(MMF_ERR_ARG, "invalid w4_id " + std::to_string(id));
@@ -1631,7 +1643,7 @@ int mmf_selective_scan(mmf_ctx* c, const mmf_scan_args* s) {
     ScanArgs a{s->dtype, s->softplus, s->out, s->u, s->dt, s->B, s->C, s->z, s->A, s->skip, s->dt_bias, s->state,
                s->lens, s->seqs, s->rows, s->D, s->N, s->ldo, s->ldu, s->lddt, s->ldb, s->ldc, s->ldz};
     refuse(check(a));
-    MMF_HIP(launch_sel_scan(a, c->stream));
+    MMF_HIP(launch_sel_scan(a, scan_splits(a) ? layer_ws(c) : nullptr, c->stream));
   });
 }
 

@@ -283,4 +283,35 @@ inline const char* check(ScanArgs& a) {
   return nullptr;
 }
 
+// How the scan of sequences [first, first + n) is cut: into chunks of `chunk` rows, with two passes
+// (split), or in one piece each.
+struct ScanPlan {
+  bool split;
+  int chunk;
+};
+constexpr size_t kScanWsFloats = size_t{4} << 20;  // the chunks' states and steps: (N + 1) D each
+inline ScanPlan scan_plan(const ScanArgs& a, size_t first, int n) {
+  size_t most = 0, rows = 0;
+  for (int i = 0; i < n; ++i) {
+    const size_t l = a.lens ? a.lens[first + i] : a.rows / a.seqs;
+    most = l > most ? l : most;
+    rows += l;
+  }
+  const ScanPlan whole{false, static_cast<int>(most ? most : 1)};
+  const size_t waves = (a.D + 63) / 64 * ((a.N + 15) / 16);  // of a chunk
+  size_t chunk = (rows * waves / 2048 + 31) / 32 * 32;       // fills the chip's 1024 SIMDs twice
+  if (chunk < 32) chunk = 32;
+  // within the workspace: at most rows / chunk + n chunks
+  const size_t per = (a.N + 1) * a.D;
+  while (chunk < most && (rows / chunk + n) * per > kScanWsFloats) chunk *= 2;
+  if (chunk * 3 > most || (rows / chunk + n) * per > kScanWsFloats) return whole;
+  return {true, static_cast<int>(chunk)};
+}
+// Whether any part of a call needs the workspace.
+inline bool scan_splits(const ScanArgs& a) {
+  for (size_t q = 0; q < a.seqs; q += kSeqs)
+    if (scan_plan(a, q, static_cast<int>(a.seqs - q < kSeqs ? a.seqs - q : kSeqs)).split) return true;
+  return false;
+}
+
 }  // namespace mmf

@@ -10,7 +10,8 @@ namespace mmf {
 // Launchers of arguments that check() has passed.
 hipError_t launch_normq(const NormQArgs& a, hipStream_t s);
 hipError_t launch_conv(const ConvArgs& a, hipStream_t s);
-hipError_t launch_sel_scan(const ScanArgs& a, hipStream_t s);
+// ws: kScanWsFloats floats where scan_splits(a)
+hipError_t launch_sel_scan(const ScanArgs& a, float* ws, hipStream_t s);
 // codes [N, ceil(K / 2)], scales and zeros (or null) [N, ceil(K / group)] on the device -> the packed
 // layout in w4_code_bytes(g) and w4_scale_bytes(g) bytes.
 hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, const W4Geom& g,

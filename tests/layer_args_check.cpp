@@ -202,7 +202,30 @@ static void mixers() {
   scan("scan no rows", nullptr, [](ScanArgs& a) { a.rows = 0, a.lens = nullptr, a.u = nullptr; });
 }
 
+// The scan's chunks: all rows in tiles of at least one row each, and their states within the workspace.
+static void plans() {
+  for (size_t D : {1, 64, 100, 1111, 4096, 100000})
+    for (size_t N : {1, 16, 17, 128})
+      for (size_t rows : {1, 31, 97, 640, 2048, 100000}) {
+        std::vector<size_t> lens = {rows, 0, rows / 2, 1, rows / 3};
+        ScanArgs a{};
+        a.lens = lens.data(), a.seqs = lens.size(), a.D = D, a.N = N;
+        for (size_t l : lens) a.rows += l;
+        const ScanPlan p = scan_plan(a, 0, 5);
+        is("chunk", p.chunk >= 1, 1);
+        SeqTab t;
+        int tiles = 0;
+        fill_seqs(t, a.lens, a.rows, a.seqs, 0, 5, p.chunk, &tiles);
+        if (p.split)
+          is("workspace", static_cast<size_t>(tiles) * (N + 1) * D <= kScanWsFloats, 1);
+        else
+          is("one piece each", tiles, 2 + (rows >= 2) + (rows >= 3));
+        is("split asked for", scan_splits(a), p.split);
+      }
+}
+
 int main() {
+  plans();
   norms();
   products();
   sequences();
