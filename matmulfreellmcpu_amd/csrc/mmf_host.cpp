@@ -209,7 +209,7 @@ struct mmf_ctx {
   DBuf raw;  // staging for int8 weights before the repack
   DBuf opy, opq, opct, opsa, opstate;
   DBuf gws;  // split-K workspace of the matrix-core GEMM
-  DBuf layer_ws;          // the scan's chunks: allocated once, at its full size
+  DBuf layer_ws;          // the scan's chunks, the 4-bit products' laid out rows: allocated once, at its full size
   DBuf hmacc;             // mmf_ternary_matmul_host: large accumulators on the device
   PinBuf pin_x, pin_acc;  // ... and their pinned host staging
   hipDeviceProp_t prop{};
@@ -1538,16 +1538,16 @@ extern "C++" {
 static void refuse(const char* why) {
   if (why) fail(MMF_ERR_ARG, why);
 }
-// The scan's workspace. It never grows, so that a captured graph's address of it stays good; its first
-// use cannot be inside a capture, which allocates nothing.
-static float* layer_ws(mmf_ctx* c) {
+// The layer operators' workspace. It never grows, so that a captured graph's address of it stays good; its
+// first use cannot be inside a capture, which allocates nothing.
+static char* layer_ws(mmf_ctx* c) {
   if (!c->layer_ws.p) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     MMF_HIP(hipStreamIsCapturing(c->stream, &st));
     if (st != hipStreamCaptureStatusNone)
-      fail(MMF_ERR_STATE, "the first selective scan of long sequences allocates its workspace: run one before the capture");
+      fail(MMF_ERR_STATE, "the first call that needs the layer workspace allocates it: make one before the capture");
   }
-  return c->layer_ws.as<float>(kScanWsFloats);
+  return c->layer_ws.as<char>(kLayerWsBytes);
 }
 static const W4& w4_of(mmf_ctx* c, int id) {
   if (id < 0 || id >= static_cast<int>(c->w4s.size())) fail(MMF_ERR_ARG, "invalid w4_id " + std::to_string(id));
@@ -1623,7 +1623,7 @@ int mmf_w4_linear(mmf_ctx* c, int id, int dtype, const void* x, const float* xsc
     const W4& w = w4_of(c, id);
     W4Args a{dtype, out_dtype, x, xscales, out, rows, ldx, ldo};
     refuse(check(a, w.g.N, w.g.K));
-    MMF_HIP(launch_w4(a, w.g, w.codes, w.scales, c->stream));
+    MMF_HIP(launch_w4(a, w.g, w.codes, w.scales, w4_lays(a.dtype, w.g, a.rows) ? layer_ws(c) : nullptr, c->stream));
   });
 }
 
@@ -1643,7 +1643,7 @@ int mmf_selective_scan(mmf_ctx* c, const mmf_scan_args* s) {
     ScanArgs a{s->dtype, s->softplus, s->out, s->u, s->dt, s->B, s->C, s->z, s->A, s->skip, s->dt_bias, s->state,
                s->lens, s->seqs, s->rows, s->D, s->N, s->ldo, s->ldu, s->lddt, s->ldb, s->ldc, s->ldz};
     refuse(check(a));
-    MMF_HIP(launch_sel_scan(a, scan_splits(a) ? layer_ws(c) : nullptr, c->stream));
+    MMF_HIP(launch_sel_scan(a, scan_splits(a) ? reinterpret_cast<float*>(layer_ws(c)) : nullptr, c->stream));
   });
 }
 

@@ -123,6 +123,23 @@ inline const char* check_w4(size_t N, size_t K, size_t group) {
   return nullptr;
 }
 
+// Many rows are laid out as matrix operands first (mmf_w4.hip): bytes of 16 rows' fragments, and with the
+// fp32 or int32 sums of their inputs; rows of a pass, so that these fit the workspace.
+constexpr size_t kLayerWsBytes = size_t{128} << 20;
+inline size_t w4_frag_bytes(int dtype, const W4Geom& g) {
+  return static_cast<size_t>(g.nc) * 128 * 16 * (dtype == kF32 ? 6 : dtype == kI8 ? 1 : 2);
+}
+inline bool w4_lays(int dtype, const W4Geom& g, size_t rows) {
+  (void)g;
+  return rows > (dtype == kF32 ? 20 : 64);
+}
+inline size_t w4_rows_most(int dtype, const W4Geom& g, size_t rows) {
+  if (!w4_lays(dtype, g, rows)) return 65535 * 5;  // the grid's second dimension, in tiles of 5 rows or more
+  size_t tiles = kLayerWsBytes / (w4_frag_bytes(dtype, g) + static_cast<size_t>(g.ns) * 64);
+  if (tiles > 8) tiles = tiles / 8 * 8;
+  return 16 * (tiles < 65535 ? tiles : 65535);
+}
+
 struct W4Args {
   int dtype, out_dtype;
   const void* x;
@@ -289,7 +306,7 @@ struct ScanPlan {
   bool split;
   int chunk;
 };
-constexpr size_t kScanWsFloats = size_t{4} << 20;  // the chunks' states and steps: (N + 1) D each
+constexpr size_t kScanWsFloats = size_t{4} << 20;  // of the workspace: the chunks' states and steps: (N + 1) D each
 inline ScanPlan scan_plan(const ScanArgs& a, size_t first, int n) {
   size_t most = 0, rows = 0;
   for (int i = 0; i < n; ++i) {

@@ -10,13 +10,15 @@ namespace mmf {
 // Launchers of arguments that check() has passed.
 hipError_t launch_normq(const NormQArgs& a, hipStream_t s);
 hipError_t launch_conv(const ConvArgs& a, hipStream_t s);
-// ws: kScanWsFloats floats where scan_splits(a)
+// ws: kLayerWsBytes where scan_splits(a)
 hipError_t launch_sel_scan(const ScanArgs& a, float* ws, hipStream_t s);
 // codes [N, ceil(K / 2)], scales and zeros (or null) [N, ceil(K / group)] on the device -> the packed
 // layout in w4_code_bytes(g) and w4_scale_bytes(g) bytes.
 hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, const W4Geom& g,
                           uint32_t* out, uint32_t* out_scales, hipStream_t s);
-hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s);
+// ws: kLayerWsBytes where w4_lays(a.dtype, g, a.rows)
+hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
+                     hipStream_t s);
 
 // Element type DT of a row tensor: V neighbouring elements in one 16-byte access at any address that
 // the type is aligned at (gfx950 takes vector accesses at element alignment).

@@ -383,6 +383,356 @@ hipError_t rows_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
          : g.step == 64 ? rows_pick<DT, 64>(a, g, codes, scales, s) : rows_pick<DT, 128>(a, g, codes, scales, s);
 }
 
+// ---- many rows ------------------------------------------------------------------------------------
+// The rows are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
+// FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
+// l % 16; zeros behind the last row and input. fp32 rows are three bf16 parts, whose products go into
+// one sum. Beside them stand the sums of a row's inputs over each scale's inputs, [tile][chunk][S][16].
+template <int DT> constexpr int kParts = DT == kF32 ? 3 : 1;
+template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
+
+// One block a tile and chunk; 16 lanes a row, 8 inputs a thread.
+template <int DT, int STEP>
+__global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags, uint32_t* sums) {
+  constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP;
+  const int u = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int c = blockIdx.x, k = c * 128 + 8 * u;
+  const size_t rt = blockIdx.y, row = rt * 16 + r;
+  const bool in = row < a.rows;
+  // the unit's place: word j of lane group q
+  const int j = STEP == 32 ? u >> 2 : (u >> 3) * 2 + (u & 1), q = STEP == 32 ? u & 3 : (u & 7) >> 1;
+  const int h = j >> 1;
+  char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
+  uint32_t total;
+  if constexpr (DT == kF32) {
+    float v[8], sum = 0.0f;
+    uint32_t part[3][8];
+    const float* x = static_cast<const float*>(a.x) + row * a.ldx + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = in && k + i < g.K ? x[i] : 0.0f;
+      sum += v[i];
+      part[0][i] = __builtin_bit_cast(uint32_t, v[i]) & 0xFFFF0000u;
+      const float r1 = v[i] - __builtin_bit_cast(float, part[0][i]);
+      part[1][i] = __builtin_bit_cast(uint32_t, r1) & 0xFFFF0000u;
+      part[2][i] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, part[1][i]));
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      u32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = (part[p][2 * i] >> 16) | (part[p][2 * i + 1] & 0xFFFF0000u);
+      *reinterpret_cast<u32x4*>(to + (p * FR + (j & 1)) * 1024) = o;
+    }
+    total = __builtin_bit_cast(uint32_t, sum);
+  } else if constexpr (DT == kI8) {
+    uint32_t x0 = 0, x1 = 0;
+    int sum = 0;
+    const int8_t* x = static_cast<const int8_t*>(a.x) + row * a.ldx + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = in && k + i < g.K ? x[i] : 0;
+      sum += e;
+      (i < 4 ? x0 : x1) |= static_cast<uint32_t>(e & 255) << (8 * (i & 3));
+    }
+    uint32_t lo, hi;
+    i8_operand(x0, x1, lo, hi);
+    uint32_t* o = reinterpret_cast<uint32_t*>(to + 8 * (j & 1));
+    o[0] = lo;
+    o[1] = hi;
+    total = static_cast<uint32_t>(sum);
+  } else {
+    u32x4 o = {0, 0, 0, 0};
+    float sum = 0.0f;
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t e = in && k + i < g.K ? x[i] : static_cast<uint16_t>(0);
+      sum += Elem<DT>::up(e);
+      o[i / 2] |= static_cast<uint32_t>(e) << (16 * (i & 1));
+    }
+    *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = o;
+    total = __builtin_bit_cast(uint32_t, sum);
+  }
+  constexpr int U = STEP / 8;  // neighbouring threads that share a scale
+#pragma unroll
+  for (int n = 1; n < U; n *= 2) {
+    const uint32_t o = __shfl_xor(static_cast<int>(total), n);
+    if constexpr (DT == kI8)
+      total += o;
+    else
+      total = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, total) + __builtin_bit_cast(float, o));
+  }
+  if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = total;
+}
+
+// A block of kw groups of wn x wr waves, a wave 64 outputs by TT tiles of rows; the groups take chunks in
+// turn, and their sums meet in LDS in a fixed order. The rows' fragments, the scales and the sums go through
+// LDS, shared by a group's waves, a stage (a chunk, or with three parts half a chunk) ahead through
+// registers; codes go straight to their operand's place. The codes' products are summed for a scale's
+// inputs alone, and the scale multiplies that sum, so the weights enter unrounded.
+template <int DT> constexpr int kRowTiles = DT == kF32 ? 2 : 4;  // of a wave: what the registers hold
+template <int DT> constexpr int kHalves = DT == kF32 ? 1 : 2;    // half chunks of a stage
+template <int DT> constexpr int kStageKB = kHalves<DT>* kParts<DT>* kFrags<DT>;  // of a tile of rows
+
+template <int DT, int STEP, int WN>
+__global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint32_t* codes, const uint32_t* scales,
+                                                 const char* frags, const uint32_t* sums, int wr, int row_tiles) {
+  using M = Mat<DT>;
+  using Acc = typename M::Acc;
+  constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP, TT = kRowTiles<DT>, H = kHalves<DT>, KB = kStageKB<DT>;
+  constexpr int kPieces = (TT * KB + WN - 1) / WN;  // KB that a wave moves of a stage
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int gw = WN * wr, kw = (blockDim.x >> 6) / gw, kg = wave / gw, gwave = wave - kg * gw;
+  const int in = gwave % WN, ir = gwave / WN, gthread = threadIdx.x - kg * gw * 64;
+  const int q = lane >> 4;
+  const int btile = blockIdx.x * (WN * 4), tile0 = btile + in * 4, rt0 = blockIdx.y * (wr * TT);
+  // LDS of a group: two buffers of the rows' pieces, the scales [WN 4][S][16] and the sums [wr TT][S][16]
+  const int pieces = wr * TT * KB, words = (WN * 4 + wr * TT) * S * 16, buf_bytes = pieces * 1024 + words * 4;
+  char* mem = lds + kg * 2 * buf_bytes;
+
+  const uint32_t* cw[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) cw[n] = codes + static_cast<size_t>(min(tile0 + n, g.nt - 1)) * g.nc * 256 + lane * 4;
+
+  u32x4 hold[kPieces];
+  constexpr int kWords = ((WN * 4 + 2 * TT) * S * 16 + WN * 128 - 1) / (WN * 128);  // a thread's, of wr = 2
+  constexpr int kWords1 = ((WN * 4 + TT) * S * 16 + WN * 64 - 1) / (WN * 64);       // ... of wr = 1
+  constexpr int kW = kWords > kWords1 ? kWords : kWords1;
+  uint32_t hold_w[kW];
+  auto fetch = [&](int c, int half) {
+    const size_t per = static_cast<size_t>(g.nc) * (2 / H);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int p = i * gw + gwave;
+      if (p < pieces) {
+        const size_t rt = min(rt0 + p / KB, row_tiles - 1);
+        hold[i] = *reinterpret_cast<const u32x4*>(frags + ((rt * per + (H == 2 ? c : 2 * c + half)) * KB + p % KB) * 1024 + lane * 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      const int v = i * gw * 64 + gthread;
+      if (v < words) {
+        const int unit = v / (S * 16), at = v - unit * (S * 16);
+        const size_t from = static_cast<size_t>(c) * S * 16 + at;
+        hold_w[i] = unit < WN * 4 ? scales[static_cast<size_t>(min(btile + unit, g.nt - 1)) * g.ns * 16 + from]
+                                  : sums[static_cast<size_t>(min(rt0 + unit - WN * 4, row_tiles - 1)) * g.ns * 16 + from];
+      }
+    }
+  };
+  auto put = [&](int buf) {
+    char* to = mem + buf * buf_bytes;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int p = i * gw + gwave;
+      if (p < pieces) *reinterpret_cast<u32x4*>(to + p * 1024 + lane * 16) = hold[i];
+    }
+    uint32_t* tw = reinterpret_cast<uint32_t*>(to + pieces * 1024);
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      const int v = i * gw * 64 + gthread;
+      if (v < words) tw[v] = hold_w[i];
+    }
+  };
+
+  f32x4 acc[4][TT];
+  Acc d[4][TT];
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
+  u32x4 w[4], next[4];
+  // all groups make the same number of rounds; a group whose chunks are used up repeats its last one, unused
+  const int rounds = (g.nc + kw - 1) / kw;
+  if (kg < g.nc) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) next[n] = *reinterpret_cast<const u32x4*>(cw[n] + static_cast<size_t>(kg) * 256);
+    fetch(kg, 0);
+    put(0);
+  }
+  __syncthreads();
+  for (int st = 0; st < rounds * (2 / H); ++st) {
+    const int half = H == 2 ? 0 : st & 1, c = (H == 2 ? st : st >> 1) * kw + kg;
+    const int nhalf = H == 2 ? 0 : half ^ 1, nc = nhalf ? c : c + kw;  // of the next stage
+    const bool more = nc < g.nc;
+    if (c < g.nc) {
+    if (half == 0) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        w[n] = next[n];
+        if (c + kw < g.nc) next[n] = *reinterpret_cast<const u32x4*>(cw[n] + static_cast<size_t>(c + kw) * 256);
+      }
+    }
+    if (more) fetch(nc, nhalf);
+    const char* buf = mem + (st & 1) * buf_bytes;
+    const char* mine = buf + ir * TT * KB * 1024 + lane * 16;
+    const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
+    const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + (WN * 4 + ir * TT) * S * 16 + (lane & 15);
+
+    auto clear = [&] {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) d[n][t] = Acc{};
+    };
+    auto flush = [&](int s) {
+      uint32_t x[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) x[t] = x_at[(t * S + s) * 16];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const u32x4 sz = *reinterpret_cast<const u32x4*>(sc_at + (n * S + s) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[i])));
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+            if constexpr (DT == kI8) {
+              acc[n][t][i] = __builtin_fmaf(
+                  sc, static_cast<float>(d[n][t][i] - static_cast<int>(sz[i] >> 16) * static_cast<int>(x[t])), acc[n][t][i]);
+            } else {
+              const float z = static_cast<float>(sz[i] >> 16) + M::base;
+              acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, __builtin_bit_cast(float, x[t]), d[n][t][i]), acc[n][t][i]);
+            }
+          }
+        }
+      }
+    };
+#pragma unroll
+    for (int hh = 0; hh < H; ++hh) {
+      const bool first = H == 2 ? hh == 0 : half == 0;  // half of its chunk
+      if constexpr (DT == kI8) {
+        i32x4 b[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) b[t] = *reinterpret_cast<const i32x4*>(mine + (t * KB + hh) * 1024);
+        if constexpr (STEP == 32) {
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            clear();
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              uint32_t lo, hi;
+              w4_bytes(w[n][2 * hh + jj], lo, hi);
+              const long aw = static_cast<long>(hi) << 32 | lo;
+#pragma unroll
+              for (int t = 0; t < TT; ++t) {
+                const long bx = static_cast<long>(static_cast<uint32_t>(b[t][2 * jj + 1])) << 32 | static_cast<uint32_t>(b[t][2 * jj]);
+                d[n][t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(aw, bx, d[n][t], 0, 0, 0);
+              }
+            }
+            flush(2 * hh + jj);
+          }
+        } else {
+          if (STEP == 64 || hh == 0) clear();
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint32_t lo0, hi0, lo1, hi1;
+            w4_bytes(w[n][2 * hh], lo0, hi0);
+            w4_bytes(w[n][2 * hh + 1], lo1, hi1);
+            const i32x4 aw = __builtin_bit_cast(i32x4, u32x4{lo0, hi0, lo1, hi1});
+#pragma unroll
+            for (int t = 0; t < TT; ++t) d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw, b[t], d[n][t], 0, 0, 0);
+          }
+          if (STEP == 64) flush(hh);
+          if (STEP == 128 && hh == 1) flush(0);
+        }
+      } else {
+        if (STEP == 64 || (STEP == 128 && first)) clear();
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          if (STEP == 32) clear();
+          u32x4 aw[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) aw[n] = w4_operand<DT>(first ? w[n][jj] : w[n][2 + jj]);
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            u32x4 b[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+              b[t] = *reinterpret_cast<const u32x4*>(mine + (t * KB + (hh * P + p) * FR + jj) * 1024);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int t = 0; t < TT; ++t) d[n][t] = M::mul(aw[n], b[t], d[n][t]);
+          }
+          if (STEP == 32) flush((first ? 0 : 2) + jj);
+        }
+        if (STEP == 64) flush(first ? 0 : 1);
+        if (STEP == 128 && !first) flush(0);
+      }
+    }
+    if (more) put((st + 1) & 1);
+    }
+    __syncthreads();
+  }
+
+  if (kw > 1) {  // the groups' sums, in the order of the groups
+    f32x4* red = reinterpret_cast<f32x4*>(lds);
+    if (kg > 0) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) red[(((kg - 1) * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane] = acc[n][t];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+    for (int k = 0; k < kw - 1; ++k)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[n][t] += red[((k * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane];
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const size_t row = static_cast<size_t>(rt0 + ir * TT + t) * 16 + (lane & 15);
+    if (row >= a.rows) continue;
+    const float xsc = DT == kI8 ? a.xscales[row] : 1.0f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int o = (tile0 + n) * 16 + 4 * q;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (o + i < g.N) store_as(a.out, a.out_dtype, row * a.ldo + o + i, DT == kI8 ? acc[n][t][i] * xsc : acc[n][t][i]);
+    }
+  }
+}
+
+template <int DT, int STEP>
+hipError_t gemm_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
+                       hipStream_t s) {
+  const int rt = static_cast<int>((a.rows + 15) / 16);
+  uint32_t* sums = reinterpret_cast<uint32_t*>(ws + rt * w4_frag_bytes(DT, g));
+  k_w4_lay<DT, STEP><<<dim3(g.nc, rt), 256, 0, s>>>(a, g, ws, sums);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  constexpr int TT = kRowTiles<DT>, S = 128 / STEP;
+  auto blocks = [&](int wn, int wr) {
+    return dim3((g.nt + wn * 4 - 1) / (wn * 4), (rt + wr * TT - 1) / (wr * TT));
+  };
+  auto lds = [&](int wn, int wr, int kw) {
+    const size_t buf = static_cast<size_t>(wr) * TT * kStageKB<DT> * 1024 + (wn * 4 + wr * TT) * S * 64;
+    const size_t red = static_cast<size_t>(kw - 1) * wn * wr * TT * 4096;
+    return 2 * kw * buf > red ? 2 * kw * buf : red;
+  };
+  if (static_cast<size_t>(blocks(4, 2).x) * blocks(4, 2).y >= 200) {
+    k_w4_gemm<DT, STEP, 4><<<blocks(4, 2), 512, lds(4, 2, 1), s>>>(a, g, codes, scales, ws, sums, 2, rt);
+  } else if (static_cast<size_t>(blocks(4, 1).x) * blocks(4, 1).y >= 200) {
+    k_w4_gemm<DT, STEP, 4><<<blocks(4, 1), 512, lds(4, 1, 2), s>>>(a, g, codes, scales, ws, sums, 1, rt);
+  } else {
+    k_w4_gemm<DT, STEP, 2><<<blocks(2, 1), 512, lds(2, 1, 4), s>>>(a, g, codes, scales, ws, sums, 1, rt);
+  }
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t gemm_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
+                     hipStream_t s) {
+  return g.step == 32 ? gemm_launch<DT, 32>(a, g, codes, scales, ws, s)
+         : g.step == 64 ? gemm_launch<DT, 64>(a, g, codes, scales, ws, s) : gemm_launch<DT, 128>(a, g, codes, scales, ws, s);
+}
+
 }  // namespace
 
 hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, const W4Geom& g,
@@ -393,18 +743,24 @@ hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const ui
   return hipGetLastError();
 }
 
-hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s) {
-  constexpr size_t kMost = 65535;  // rows of a launch: the grid's second dimension
-  for (size_t r = 0; r < a.rows; r += kMost) {
+template <class F>
+static hipError_t by_type(int dtype, F&& f) {
+  return dtype == kI8 ? f(std::integral_constant<int, kI8>{}) : with_type(dtype, f);
+}
+
+hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
+                     hipStream_t s) {
+  const size_t most = w4_rows_most(a.dtype, g, a.rows);
+  for (size_t r = 0; r < a.rows; r += most) {
     W4Args b = a;
-    b.rows = a.rows - r < kMost ? a.rows - r : kMost;
+    b.rows = a.rows - r < most ? a.rows - r : most;
     b.x = static_cast<const char*>(a.x) + r * a.ldx * dtype_size(a.dtype);
     b.out = static_cast<char*>(a.out) + r * a.ldo * dtype_size(a.out_dtype);
     if (a.xscales) b.xscales = a.xscales + r;
-    const hipError_t e = a.dtype == kF32    ? rows_step<kF32>(b, g, codes, scales, s)
-                         : a.dtype == kBF16 ? rows_step<kBF16>(b, g, codes, scales, s)
-                         : a.dtype == kF16  ? rows_step<kF16>(b, g, codes, scales, s)
-                                            : rows_step<kI8>(b, g, codes, scales, s);
+    const hipError_t e = by_type(a.dtype, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      return w4_lays(a.dtype, g, a.rows) ? gemm_step<DT>(b, g, codes, scales, ws, s) : rows_step<DT>(b, g, codes, scales, s);
+    });
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
