@@ -496,45 +496,41 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
 #pragma unroll
   for (int n = 0; n < 4; ++n) cw[n] = codes + static_cast<size_t>(min(tile0 + n, g.nt - 1)) * g.nc * 256 + lane * 4;
 
+  // Loads and LDS writes have no conditions (an index past the end repeats the last one), so that the
+  // compiler knows which loads are in flight and waits for no younger ones.
   u32x4 hold[kPieces];
   constexpr int kWords = ((WN * 4 + 2 * TT) * S * 16 + WN * 128 - 1) / (WN * 128);  // a thread's, of wr = 2
   constexpr int kWords1 = ((WN * 4 + TT) * S * 16 + WN * 64 - 1) / (WN * 64);       // ... of wr = 1
   constexpr int kW = kWords > kWords1 ? kWords : kWords1;
   uint32_t hold_w[kW];
+  const char* from_p[kPieces];
+  const uint32_t* from_w[kW];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int p = i * gw + gwave;
+    const size_t rt = min(rt0 + p / KB, row_tiles - 1);
+    from_p[i] = frags + rt * g.nc * (2 / H) * (KB * 1024) + (p % KB) * 1024 + lane * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < kW; ++i) {
+    const int v = min(i * gw * 64 + gthread, words - 1), unit = v / (S * 16), at = v - unit * (S * 16);
+    from_w[i] = (unit < WN * 4 ? scales + static_cast<size_t>(min(btile + unit, g.nt - 1)) * g.ns * 16
+                               : sums + static_cast<size_t>(min(rt0 + unit - WN * 4, row_tiles - 1)) * g.ns * 16) + at;
+  }
   auto fetch = [&](int c, int half) {
-    const size_t per = static_cast<size_t>(g.nc) * (2 / H);
+    const size_t st = H == 2 ? c : 2 * c + half;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = i * gw + gwave;
-      if (p < pieces) {
-        const size_t rt = min(rt0 + p / KB, row_tiles - 1);
-        hold[i] = *reinterpret_cast<const u32x4*>(frags + ((rt * per + (H == 2 ? c : 2 * c + half)) * KB + p % KB) * 1024 + lane * 16);
-      }
-    }
+    for (int i = 0; i < kPieces; ++i) hold[i] = *reinterpret_cast<const u32x4*>(from_p[i] + st * (KB * 1024));
 #pragma unroll
-    for (int i = 0; i < kW; ++i) {
-      const int v = i * gw * 64 + gthread;
-      if (v < words) {
-        const int unit = v / (S * 16), at = v - unit * (S * 16);
-        const size_t from = static_cast<size_t>(c) * S * 16 + at;
-        hold_w[i] = unit < WN * 4 ? scales[static_cast<size_t>(min(btile + unit, g.nt - 1)) * g.ns * 16 + from]
-                                  : sums[static_cast<size_t>(min(rt0 + unit - WN * 4, row_tiles - 1)) * g.ns * 16 + from];
-      }
-    }
+    for (int i = 0; i < kW; ++i) hold_w[i] = from_w[i][static_cast<size_t>(c) * S * 16];
   };
   auto put = [&](int buf) {
     char* to = mem + buf * buf_bytes;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = i * gw + gwave;
-      if (p < pieces) *reinterpret_cast<u32x4*>(to + p * 1024 + lane * 16) = hold[i];
-    }
+    for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(to + (i * gw + gwave) * 1024 + lane * 16) = hold[i];
     uint32_t* tw = reinterpret_cast<uint32_t*>(to + pieces * 1024);
 #pragma unroll
-    for (int i = 0; i < kW; ++i) {
-      const int v = i * gw * 64 + gthread;
-      if (v < words) tw[v] = hold_w[i];
-    }
+    for (int i = 0; i < kW; ++i) tw[min(i * gw * 64 + gthread, words - 1)] = hold_w[i];
   };
 
   f32x4 acc[4][TT];
@@ -544,128 +540,129 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
   u32x4 w[4], next[4];
-  // all groups make the same number of rounds; a group whose chunks are used up repeats its last one, unused
-  const int rounds = (g.nc + kw - 1) / kw;
-  if (kg < g.nc) {
+  const int rounds = (g.nc + kw - 1) / kw;  // the same for all groups: a group without a chunk adds nothing
+  auto load_codes = [&](int c) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) next[n] = *reinterpret_cast<const u32x4*>(cw[n] + static_cast<size_t>(kg) * 256);
-    fetch(kg, 0);
-    put(0);
-  }
+    for (int n = 0; n < 4; ++n) next[n] = *reinterpret_cast<const u32x4*>(cw[n] + static_cast<size_t>(c) * 256);
+  };
+  const int last = g.nc - 1;
+  load_codes(min(kg, last));
+  fetch(min(kg, last), 0);
+  put(0);
   __syncthreads();
-  for (int st = 0; st < rounds * (2 / H); ++st) {
-    const int half = H == 2 ? 0 : st & 1, c = (H == 2 ? st : st >> 1) * kw + kg;
-    const int nhalf = H == 2 ? 0 : half ^ 1, nc = nhalf ? c : c + kw;  // of the next stage
-    const bool more = nc < g.nc;
-    if (c < g.nc) {
-    if (half == 0) {
+  for (int r = 0; r < rounds; ++r) {
+    const int c = r * kw + kg;
+    const bool mine_too = c <= last;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        w[n] = next[n];
-        if (c + kw < g.nc) next[n] = *reinterpret_cast<const u32x4*>(cw[n] + static_cast<size_t>(c + kw) * 256);
-      }
-    }
-    if (more) fetch(nc, nhalf);
-    const char* buf = mem + (st & 1) * buf_bytes;
-    const char* mine = buf + ir * TT * KB * 1024 + lane * 16;
-    const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
-    const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + (WN * 4 + ir * TT) * S * 16 + (lane & 15);
+    for (int n = 0; n < 4; ++n) w[n] = next[n];
+    load_codes(min(c + kw, last));
+#pragma unroll
+    for (int hs = 0; hs < 2 / H; ++hs) {
+      const int cur = H == 2 ? r & 1 : hs;
+      if (H == 2 || hs == 1)
+        fetch(min(c + kw, last), 0);
+      else
+        fetch(min(c, last), 1);
+      const char* buf = mem + cur * buf_bytes;
+      const char* mine = buf + ir * TT * KB * 1024 + lane * 16;
+      const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
+      const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + (WN * 4 + ir * TT) * S * 16 + (lane & 15);
 
-    auto clear = [&] {
+      auto clear = [&] {
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) d[n][t] = Acc{};
-    };
-    auto flush = [&](int s) {
-      uint32_t x[TT];
+          for (int t = 0; t < TT; ++t) d[n][t] = Acc{};
+      };
+      auto flush = [&](int s) {
+        if (!mine_too) return;
+        uint32_t x[TT];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) x[t] = x_at[(t * S + s) * 16];
+        for (int t = 0; t < TT; ++t) x[t] = x_at[(t * S + s) * 16];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const u32x4 sz = *reinterpret_cast<const u32x4*>(sc_at + (n * S + s) * 16);
+        for (int n = 0; n < 4; ++n) {
+          const u32x4 sz = *reinterpret_cast<const u32x4*>(sc_at + (n * S + s) * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[i])));
+          for (int i = 0; i < 4; ++i) {
+            const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[i])));
 #pragma unroll
-          for (int t = 0; t < TT; ++t) {
-            if constexpr (DT == kI8) {
-              acc[n][t][i] = __builtin_fmaf(
-                  sc, static_cast<float>(d[n][t][i] - static_cast<int>(sz[i] >> 16) * static_cast<int>(x[t])), acc[n][t][i]);
-            } else {
-              const float z = static_cast<float>(sz[i] >> 16) + M::base;
-              acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, __builtin_bit_cast(float, x[t]), d[n][t][i]), acc[n][t][i]);
-            }
-          }
-        }
-      }
-    };
-#pragma unroll
-    for (int hh = 0; hh < H; ++hh) {
-      const bool first = H == 2 ? hh == 0 : half == 0;  // half of its chunk
-      if constexpr (DT == kI8) {
-        i32x4 b[TT];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) b[t] = *reinterpret_cast<const i32x4*>(mine + (t * KB + hh) * 1024);
-        if constexpr (STEP == 32) {
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            clear();
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              uint32_t lo, hi;
-              w4_bytes(w[n][2 * hh + jj], lo, hi);
-              const long aw = static_cast<long>(hi) << 32 | lo;
-#pragma unroll
-              for (int t = 0; t < TT; ++t) {
-                const long bx = static_cast<long>(static_cast<uint32_t>(b[t][2 * jj + 1])) << 32 | static_cast<uint32_t>(b[t][2 * jj]);
-                d[n][t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(aw, bx, d[n][t], 0, 0, 0);
+            for (int t = 0; t < TT; ++t) {
+              if constexpr (DT == kI8) {
+                acc[n][t][i] = __builtin_fmaf(
+                    sc, static_cast<float>(d[n][t][i] - static_cast<int>(sz[i] >> 16) * static_cast<int>(x[t])), acc[n][t][i]);
+              } else {
+                const float z = static_cast<float>(sz[i] >> 16) + M::base;
+                acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, __builtin_bit_cast(float, x[t]), d[n][t][i]), acc[n][t][i]);
               }
             }
-            flush(2 * hh + jj);
+          }
+        }
+      };
+#pragma unroll
+      for (int hh = 0; hh < H; ++hh) {
+        const int half = H == 2 ? hh : hs;  // of its chunk
+        if constexpr (DT == kI8) {
+          i32x4 b[TT];
+#pragma unroll
+          for (int t = 0; t < TT; ++t) b[t] = *reinterpret_cast<const i32x4*>(mine + (t * KB + hh) * 1024);
+          if constexpr (STEP == 32) {
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+              clear();
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                uint32_t lo, hi;
+                w4_bytes(w[n][2 * half + jj], lo, hi);
+                const long aw = static_cast<long>(hi) << 32 | lo;
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                  const long bx =
+                      static_cast<long>(static_cast<uint32_t>(b[t][2 * jj + 1])) << 32 | static_cast<uint32_t>(b[t][2 * jj]);
+                  d[n][t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(aw, bx, d[n][t], 0, 0, 0);
+                }
+              }
+              flush(2 * half + jj);
+            }
+          } else {
+            if (STEP == 64 || half == 0) clear();
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              uint32_t lo0, hi0, lo1, hi1;
+              w4_bytes(w[n][2 * half], lo0, hi0);
+              w4_bytes(w[n][2 * half + 1], lo1, hi1);
+              const i32x4 aw = __builtin_bit_cast(i32x4, u32x4{lo0, hi0, lo1, hi1});
+#pragma unroll
+              for (int t = 0; t < TT; ++t) d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw, b[t], d[n][t], 0, 0, 0);
+            }
           }
         } else {
-          if (STEP == 64 || hh == 0) clear();
+          if (STEP == 64 || (STEP == 128 && half == 0)) clear();
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t lo0, hi0, lo1, hi1;
-            w4_bytes(w[n][2 * hh], lo0, hi0);
-            w4_bytes(w[n][2 * hh + 1], lo1, hi1);
-            const i32x4 aw = __builtin_bit_cast(i32x4, u32x4{lo0, hi0, lo1, hi1});
+          for (int jj = 0; jj < 2; ++jj) {
+            if (STEP == 32) clear();
+            u32x4 aw[4];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw, b[t], d[n][t], 0, 0, 0);
+            for (int n = 0; n < 4; ++n) aw[n] = w4_operand<DT>(w[n][2 * half + jj]);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+              u32x4 b[TT];
+#pragma unroll
+              for (int t = 0; t < TT; ++t)
+                b[t] = *reinterpret_cast<const u32x4*>(mine + (t * KB + (hh * P + p) * FR + jj) * 1024);
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) d[n][t] = M::mul(aw[n], b[t], d[n][t]);
+            }
+            if (STEP == 32) flush(2 * half + jj);
           }
-          if (STEP == 64) flush(hh);
-          if (STEP == 128 && hh == 1) flush(0);
         }
-      } else {
-        if (STEP == 64 || (STEP == 128 && first)) clear();
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          if (STEP == 32) clear();
-          u32x4 aw[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) aw[n] = w4_operand<DT>(first ? w[n][jj] : w[n][2 + jj]);
-#pragma unroll
-          for (int p = 0; p < P; ++p) {
-            u32x4 b[TT];
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-              b[t] = *reinterpret_cast<const u32x4*>(mine + (t * KB + (hh * P + p) * FR + jj) * 1024);
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-              for (int t = 0; t < TT; ++t) d[n][t] = M::mul(aw[n], b[t], d[n][t]);
-          }
-          if (STEP == 32) flush((first ? 0 : 2) + jj);
-        }
-        if (STEP == 64) flush(first ? 0 : 1);
-        if (STEP == 128 && !first) flush(0);
+        if (STEP == 64) flush(half);
+        if (STEP == 128 && half == 1) flush(0);
       }
+      put(cur ^ 1);
+      __syncthreads();
     }
-    if (more) put((st + 1) & 1);
-    }
-    __syncthreads();
   }
 
   if (kw > 1) {  // the groups' sums, in the order of the groups
@@ -684,19 +681,37 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[n][t] += red[((k * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane];
   }
+  auto store = [&](auto ot) {
+    using O = Elem<decltype(ot)::value>;
+    typedef typename O::T T4 __attribute__((ext_vector_type(4), aligned(sizeof(typename O::T))));
 #pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    const size_t row = static_cast<size_t>(rt0 + ir * TT + t) * 16 + (lane & 15);
-    if (row >= a.rows) continue;
-    const float xsc = DT == kI8 ? a.xscales[row] : 1.0f;
+    for (int t = 0; t < TT; ++t) {
+      const size_t row = static_cast<size_t>(rt0 + ir * TT + t) * 16 + (lane & 15);
+      if (row >= a.rows) continue;
+      const float xsc = DT == kI8 ? a.xscales[row] : 1.0f;
+      typename O::T* out = static_cast<typename O::T*>(a.out) + row * a.ldo;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int o = (tile0 + n) * 16 + 4 * q;
+      for (int n = 0; n < 4; ++n) {
+        const int o = (tile0 + n) * 16 + 4 * q;
+        T4 v;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (o + i < g.N) store_as(a.out, a.out_dtype, row * a.ldo + o + i, DT == kI8 ? acc[n][t][i] * xsc : acc[n][t][i]);
+        for (int i = 0; i < 4; ++i) v[i] = O::down(DT == kI8 ? acc[n][t][i] * xsc : acc[n][t][i]);
+        if (o + 4 <= g.N) {
+          *reinterpret_cast<T4*>(out + o) = v;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (o + i < g.N) out[o + i] = v[i];
+        }
+      }
     }
-  }
+  };
+  if (a.out_dtype == kF32)
+    store(std::integral_constant<int, kF32>{});
+  else if (a.out_dtype == kBF16)
+    store(std::integral_constant<int, kBF16>{});
+  else
+    store(std::integral_constant<int, kF16>{});
 }
 
 template <int DT, int STEP>
