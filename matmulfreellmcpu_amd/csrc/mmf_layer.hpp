@@ -8,6 +8,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 #ifdef __HIPCC__
 #define MMF_HD __host__ __device__
@@ -129,15 +130,45 @@ constexpr size_t kLayerWsBytes = size_t{128} << 20;
 inline size_t w4_frag_bytes(int dtype, const W4Geom& g) {
   return static_cast<size_t>(g.nc) * 128 * 16 * (dtype == kF32 ? 6 : dtype == kI8 ? 1 : 2);
 }
+inline size_t w4_lay_bytes(int dtype, const W4Geom& g, int row_tiles) {  // fragments and sums
+  return row_tiles * (w4_frag_bytes(dtype, g) + static_cast<size_t>(g.ns) * 64);
+}
+inline constexpr int w4_tile_rows(int dtype) { return dtype == kF32 ? 32 : 64; }  // of a wave
+
+// How the many-row kernel's 8 waves stand (wn over 64 outputs each, wr over w4_tile_rows rows each, 8 / (wn wr)
+// over the inputs) and over how many blocks a tile's inputs are split.
+struct W4Plan {
+  int wn, wr, ks;
+};
+inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
+  const int tt = w4_tile_rows(dtype) / 16;
+  auto blocks = [&](int wn, int wr) {
+    return static_cast<size_t>((g.nt + wn * 4 - 1) / (wn * 4)) * ((row_tiles + wr * tt - 1) / (wr * tt));
+  };
+  W4Plan p{2, 1, 1};
+  if (blocks(4, 2) >= 200)
+    p = {4, 2, 1};
+  else if (blocks(4, 1) >= 200)
+    p = {4, 1, 1};
+  return p;
+}
+// The same, with no more splits than the workspace holds the sums of beside the laid out rows.
+inline W4Plan w4_plan(int dtype, const W4Geom& g, int row_tiles) {
+  W4Plan p = w4_pick(dtype, g, row_tiles);
+  const size_t one = static_cast<size_t>(row_tiles) * g.nt * 1024;  // bytes of one split's sums
+  const size_t room = kLayerWsBytes - w4_lay_bytes(dtype, g, row_tiles);
+  while (p.ks > 1 && p.ks * one > room) p.ks /= 2;
+  return p;
+}
 inline bool w4_lays(int dtype, const W4Geom& g, size_t rows) {
   (void)g;
   return rows > (dtype == kF32 ? 20 : 64);
 }
 inline size_t w4_rows_most(int dtype, const W4Geom& g, size_t rows) {
   if (!w4_lays(dtype, g, rows)) return 65535 * 5;  // the grid's second dimension, in tiles of 5 rows or more
-  size_t tiles = kLayerWsBytes / (w4_frag_bytes(dtype, g) + static_cast<size_t>(g.ns) * 64);
+  size_t tiles = kLayerWsBytes / w4_lay_bytes(dtype, g, 1);
   if (tiles > 8) tiles = tiles / 8 * 8;
-  return 16 * (tiles < 65535 ? tiles : 65535);
+  return 16 * (tiles < 4095 ? tiles : 4095);  // k_w4_sum has a block a row in that dimension
 }
 
 struct W4Args {

@@ -477,20 +477,22 @@ template <int DT> constexpr int kStageKB = kHalves<DT>* kParts<DT>* kFrags<DT>; 
 
 template <int DT, int STEP, int WN>
 __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint32_t* codes, const uint32_t* scales,
-                                                 const char* frags, const uint32_t* sums, int wr, int row_tiles) {
+                                                 const char* frags, const uint32_t* sums, float* partials, int wr,
+                                                 int row_tiles) {
   using M = Mat<DT>;
   using Acc = typename M::Acc;
   constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP, TT = kRowTiles<DT>, H = kHalves<DT>, KB = kStageKB<DT>;
   constexpr int kPieces = (TT * KB + WN - 1) / WN;  // KB that a wave moves of a stage
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int gw = WN * wr, kw = (blockDim.x >> 6) / gw, kg = wave / gw, gwave = wave - kg * gw;
-  const int in = gwave % WN, ir = gwave / WN, gthread = threadIdx.x - kg * gw * 64;
+  const int gw = WN * wr, bk = (blockDim.x >> 6) / gw, group = wave / gw, gwave = wave - group * gw;
+  const int kw = bk * gridDim.z, kg = blockIdx.z * bk + group;  // the chunks' groups, of all blocks of a tile
+  const int in = gwave % WN, ir = gwave / WN, gthread = threadIdx.x - group * gw * 64;
   const int q = lane >> 4;
   const int btile = blockIdx.x * (WN * 4), tile0 = btile + in * 4, rt0 = blockIdx.y * (wr * TT);
   // LDS of a group: two buffers of the rows' pieces, the scales [WN 4][S][16] and the sums [wr TT][S][16]
   const int pieces = wr * TT * KB, words = (WN * 4 + wr * TT) * S * 16, buf_bytes = pieces * 1024 + words * 4;
-  char* mem = lds + kg * 2 * buf_bytes;
+  char* mem = lds + group * 2 * buf_bytes;
 
   const uint32_t* cw[4];
 #pragma unroll
@@ -665,21 +667,33 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
     }
   }
 
-  if (kw > 1) {  // the groups' sums, in the order of the groups
+  if (bk > 1) {  // the groups' sums, in the order of the groups
     f32x4* red = reinterpret_cast<f32x4*>(lds);
-    if (kg > 0) {
+    if (group > 0) {
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) red[(((kg - 1) * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane] = acc[n][t];
+        for (int t = 0; t < TT; ++t) red[(((group - 1) * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane] = acc[n][t];
     }
     __syncthreads();
-    if (kg > 0) return;
-    for (int k = 0; k < kw - 1; ++k)
+    if (group > 0) return;
+    for (int k = 0; k < bk - 1; ++k)
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[n][t] += red[((k * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane];
+  }
+  if (partials) {  // one of several blocks of this tile: k_w4_sum adds them
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int rt = rt0 + ir * TT + t;
+      if (rt >= row_tiles) continue;
+      float* to = partials + ((static_cast<size_t>(blockIdx.z) * row_tiles + rt) * 16 + (lane & 15)) * (g.nt * 16) + 4 * q;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (tile0 + n < g.nt) *reinterpret_cast<f32x4*>(to + (tile0 + n) * 16) = acc[n][t];
+    }
+    return;
   }
   auto store = [&](auto ot) {
     using O = Elem<decltype(ot)::value>;
@@ -714,30 +728,45 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
     store(std::integral_constant<int, kF16>{});
 }
 
+// The blocks' partial sums, added in the order of the blocks; four outputs a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void k_w4_sum(W4Args a, W4Geom g, const float* partials, int row_tiles, int ks) {
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const size_t row = blockIdx.y;
+  if (n >= g.N) return;
+  const float* p = partials + row * (g.nt * 16) + n;
+  const size_t step = static_cast<size_t>(row_tiles) * 16 * (g.nt * 16);
+  f32x4 v = *reinterpret_cast<const f32x4*>(p);
+  for (int k = 1; k < ks; ++k) v += *reinterpret_cast<const f32x4*>(p + k * step);
+  if (DT == kI8) v *= a.xscales[row];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < g.N) store_as(a.out, a.out_dtype, row * a.ldo + n + i, v[i]);
+}
+
 template <int DT, int STEP>
 hipError_t gemm_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
                        hipStream_t s) {
   const int rt = static_cast<int>((a.rows + 15) / 16);
   uint32_t* sums = reinterpret_cast<uint32_t*>(ws + rt * w4_frag_bytes(DT, g));
   k_w4_lay<DT, STEP><<<dim3(g.nc, rt), 256, 0, s>>>(a, g, ws, sums);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   constexpr int TT = kRowTiles<DT>, S = 128 / STEP;
-  auto blocks = [&](int wn, int wr) {
-    return dim3((g.nt + wn * 4 - 1) / (wn * 4), (rt + wr * TT - 1) / (wr * TT));
-  };
-  auto lds = [&](int wn, int wr, int kw) {
-    const size_t buf = static_cast<size_t>(wr) * TT * kStageKB<DT> * 1024 + (wn * 4 + wr * TT) * S * 64;
-    const size_t red = static_cast<size_t>(kw - 1) * wn * wr * TT * 4096;
-    return 2 * kw * buf > red ? 2 * kw * buf : red;
-  };
-  if (static_cast<size_t>(blocks(4, 2).x) * blocks(4, 2).y >= 200) {
-    k_w4_gemm<DT, STEP, 4><<<blocks(4, 2), 512, lds(4, 2, 1), s>>>(a, g, codes, scales, ws, sums, 2, rt);
-  } else if (static_cast<size_t>(blocks(4, 1).x) * blocks(4, 1).y >= 200) {
-    k_w4_gemm<DT, STEP, 4><<<blocks(4, 1), 512, lds(4, 1, 2), s>>>(a, g, codes, scales, ws, sums, 1, rt);
-  } else {
-    k_w4_gemm<DT, STEP, 2><<<blocks(2, 1), 512, lds(2, 1, 4), s>>>(a, g, codes, scales, ws, sums, 1, rt);
-  }
+  static_assert(TT == w4_tile_rows(DT) / 16, "the plan's tiles");
+  const W4Plan p = w4_plan(DT, g, rt);
+  const int wn = p.wn, wr = p.wr, kw = 8 / (wn * wr);
+  const size_t buf = static_cast<size_t>(wr) * TT * kStageKB<DT> * 1024 + (wn * 4 + wr * TT) * S * 64;
+  const size_t red = static_cast<size_t>(kw - 1) * wn * wr * TT * 4096, lds = 2 * kw * buf > red ? 2 * kw * buf : red;
+  const dim3 grid((g.nt + wn * 4 - 1) / (wn * 4), (rt + wr * TT - 1) / (wr * TT), p.ks);
+  float* partials = p.ks > 1 ? reinterpret_cast<float*>(ws + w4_lay_bytes(DT, g, rt)) : nullptr;
+  if (wn == 4)
+    k_w4_gemm<DT, STEP, 4><<<grid, 512, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
+  else
+    k_w4_gemm<DT, STEP, 2><<<grid, 512, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
+  e = hipGetLastError();
+  if (e != hipSuccess || !partials) return e;
+  k_w4_sum<DT><<<dim3((g.N + 1023) / 1024, static_cast<unsigned>(a.rows)), 256, 0, s>>>(a, g, partials, rt, p.ks);
   return hipGetLastError();
 }
 
