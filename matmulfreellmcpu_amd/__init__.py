@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from array import array
+from struct import Struct
 
 import numpy as np
 
@@ -39,11 +40,9 @@ class MmfConfig(C.Structure):
                 ("intermediate_size", _sz), ("use_lower_bound", C.c_int), ("rms_norm_eps", C.c_float)]
 
 
-class MmfScanArgs(C.Structure):
-    _fields_ = ([("dtype", C.c_int), ("softplus", C.c_int)]
-                + [(n, _vp) for n in ("out", "u", "dt", "B", "C", "z", "A", "skip", "dt_bias", "state", "lens")]
-                + [(n, _sz) for n in ("seqs", "rows", "D", "N", "ldo", "ldu", "lddt", "ldb", "ldc", "ldz")])
-
+# mmf_scan_args: dtype, softplus; eleven pointers (out ... lens); ten sizes (seqs ... ldz). Packed at once, as a
+# ctypes.Structure of as many fields takes longer than the launch.
+_SCAN_ARGS = Struct("@2i21Q")
 
 TOKEN_CB = C.CFUNCTYPE(None, _vp, C.c_int64)
 
@@ -89,7 +88,7 @@ def load_library(path: str = LIB_PATH):
         "mmf_w4_release": (i, [_vp, i]),
         "mmf_w4_linear": (i, [_vp, i, i, _vp, _vp, i, _vp, _sz, _sz, _sz]),
         "mmf_short_conv": (i, [_vp, i] + [_vp] * 6 + [_sz] * 4 + [i, _sz, _sz]),
-        "mmf_selective_scan": (i, [_vp, C.POINTER(MmfScanArgs)]),
+        "mmf_selective_scan": (i, [_vp, C.c_char_p]),
         "mmf_model_begin": (i, [_vp, C.POINTER(MmfConfig)]),
         "mmf_model_tensor": (i, [_vp, C.c_char_p, i, C.POINTER(_sz), i, _vp]),
         "mmf_model_finalize": (i, [_vp, i, i]),
@@ -297,8 +296,9 @@ class Engine:
                        seqs=1, softplus=True, dtype=F32, ldo=0, ldu=0, lddt=0, ldb=0, ldc=0, ldz=0):
         """Selective state space scan of sequences of the lengths lens (None: `seqs` equal ones)."""
         _keep, lp, n = _lens(lens, seqs)
-        a = MmfScanArgs(dtype, int(softplus), _ptr(out), _ptr(u), _ptr(dt), _ptr(B), _ptr(C), _ptr(z), _ptr(A),
-                        _ptr(skip), _ptr(dt_bias), _ptr(state), lp, n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
+        a = _SCAN_ARGS.pack(dtype, bool(softplus), _ptr(out) or 0, _ptr(u) or 0, _ptr(dt) or 0, _ptr(B) or 0, _ptr(C) or 0,
+                            _ptr(z) or 0, _ptr(A) or 0, _ptr(skip) or 0, _ptr(dt_bias) or 0, _ptr(state) or 0, lp or 0,
+                            n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
         self._chk(self.lib.mmf_selective_scan(self.h, a))
 
     # ---- model ----

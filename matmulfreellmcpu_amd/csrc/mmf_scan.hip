@@ -10,7 +10,7 @@ namespace {
 // log(1 + e) for e in [0, 1] = 2 atanh(s), s = e / (2 + e) <= 1/3, by its series: the terms after
 // s^15 / 15 are below 2^-26 of the sum. 1 + e would lose the digits of a small e.
 __device__ __forceinline__ float log1p_unit(float e) {
-  const float s = e / (2.0f + e), q = s * s;
+  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
   float p = 1.0f / 15;
   p = __builtin_fmaf(p, q, 1.0f / 13);
   p = __builtin_fmaf(p, q, 1.0f / 11);
@@ -24,149 +24,231 @@ __device__ __forceinline__ float softplus(float x) {
   return __builtin_fmaxf(x, 0.0f) + log1p_unit(exp2_fast(-1.44269504f * __builtin_fabsf(x)));
 }
 
-// A lane holds a channel's NS states in registers; a wave is 64 channels, and `nw` waves share a
-// channel with more states. Every lane needs the same B and C of a step: a block keeps kTile steps of them
-// in LDS as fp32 and reads them four at a time, all lanes one address.
+// A lane holds a channel's NS states in registers; a wave is 64 channels, and NW waves share a channel
+// with more states. Every lane needs the same B and C of a step: a block keeps kTile steps of them in LDS as
+// fp32 and reads them four at a time, all lanes one address; the next tile's are in flight meanwhile.
 //
-// What bounds it: the exponentials. A step of 16 states is 16 v_exp_f32 at a quarter of the rate and 64
-// other operations, 512 cycles of a SIMD for 64 channels.
+// What bounds it: the vector ALUs. A step of a state is an exponential (8.6 cycles a wave, measured) and 4
+// other operations (4.3 each), 26 cycles for 64 channels, and a step of a channel some 180 more.
 //
 // Long sequences are cut into chunks so that the chip is full: kSum finds each chunk's end state from
-// zeros and the sum of its steps (the decay over a chunk is exp(A * sum dt)), and kApply starts each
-// chunk from the states before it, folded in order, and writes the outputs. The first chunk of kSum starts
-// from the state itself. A sequence's last chunk needs no sums: its slot of the workspace keeps the
-// state at the start, which kApply's last chunk overwrites in `state`.
-constexpr int kTile = 32, kGroup4 = 4;
+// zeros and the sum of its steps (the decay over a chunk is exp(A * sum dt)), k_carry makes the states
+// before each chunk of these, in order, and kApply starts each chunk there and writes the outputs. The first
+// chunk of kSum starts from the state itself. A sequence's last chunk needs no sums: its slot of the
+// workspace keeps the state at the start, which kApply's last chunk overwrites in `state`. kSum also leaves
+// the steps themselves (softplus and all), where the workspace holds them. (kApply folding the chunks before
+// its own by itself waits a load's time for each: 2048 x 4096 x 16 fp32 113 us, with k_carry 90.)
+constexpr int kTile = 32, kAhead = 4;
 enum ScanPass { kSum = 0, kApply = 1 };
 
 struct ScanWs {
   float* ends;  // [chunk][N][D], or null: sequences in one piece
-  float* steps; // [chunk][D]
+  float* sums;  // [chunk][D]
+  float* dt;    // [row][D], or null
   int chunk;    // rows of a chunk
 };
 
-template <int DT, int NS, int PASS>
-__global__ __launch_bounds__(512) void k_scan(ScanArgs a, SeqTab t, ScanWs ws, size_t seq0, size_t row0, int nw) {
+template <int DT, int NS, int NW, int PASS>
+__global__ __launch_bounds__(NW == 8 ? 512 : 256) void k_scan(ScanArgs a, SeqTab t, ScanWs ws, size_t seq0, size_t row0) {
   using E = Elem<DT>;
   using T = typename E::T;
-  extern __shared__ __align__(16) float lds[];
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int CW = NW >= 4 ? 1 : 4 / NW, NP = NW * NS;        // waves of other channels, padded states
+  constexpr int kUnit = NS < 8 ? NS : 8, kUnits = NS / kUnit;
+  constexpr int kRows = 64 * CW / NS, kIter = (kTile + kRows - 1) / kRows;  // steps that the block stages at a time
+  __shared__ __align__(16) float sB[kTile * NP], sC[PASS == kApply ? kTile * NP : 4];
+  __shared__ float sy[PASS == kApply && NW > 1 ? CW : 1][2][NW][kAhead][64];
   const TileAt at = tile_at(t, blockIdx.x);
   const int chunks = (at.len + ws.chunk - 1) / ws.chunk;
-  const bool split = ws.ends != nullptr;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave % nw, cw = static_cast<int>(blockDim.x >> 6) / nw;
-  const int N = static_cast<int>(a.N), n0 = part * NS, np = nw * NS;
-  const size_t D = a.D, dd = (static_cast<size_t>(blockIdx.y) * cw + wave / nw) * 64 + lane;
+  const int part = wave % NW, cwave = wave / NW;
+  const int N = static_cast<int>(a.N), n0 = part * NS;
+  // A row's address is uniform and a lane adds its channel to it.
+  const size_t D = a.D;
+  const uint32_t dd = (blockIdx.y * CW + cwave) * 64 + lane, d = min(dd, static_cast<uint32_t>(D) - 1);
   const bool live = dd < D;
-  const size_t d = live ? dd : D - 1;
-  float* state = a.state ? a.state + (seq0 + at.seq) * a.N * D + d : nullptr;
-  const size_t slot = static_cast<size_t>(blockIdx.x);
-  auto end_of = [&](size_t item, int n) -> float& { return ws.ends[(item * a.N + n) * D + d]; };
-
-  if (PASS == kSum && at.k == chunks - 1) {  // no sums of the last chunk: its slot keeps the state
-    for (int i = 0; i < NS; ++i)
-      if (live && n0 + i < N) end_of(slot, n0 + i) = state ? state[(n0 + i) * D] : 0.0f;
-    return;
-  }
-
-  float A[NS], h[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) A[i] = n0 + i < N ? a.A[d * a.N + n0 + i] * 1.44269504f : 0.0f;
-  if (!split || PASS == kSum) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i) h[i] = at.k == 0 && state && n0 + i < N ? state[(n0 + i) * D] : 0.0f;
-  } else {
-    const size_t first = slot - at.k;
-    const size_t from = at.k ? first : first + chunks - 1;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) h[i] = n0 + i < N ? end_of(from, n0 + i) : 0.0f;
-    for (int j = 1; j < at.k; ++j) {
-      const float sum = ws.steps[(first + j) * D + d];
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        h[i] = __builtin_fmaf(exp2_fast(sum * A[i]), h[i], n0 + i < N ? end_of(first + j, n0 + i) : 0.0f);
-    }
-  }
-  const float skip = a.skip ? a.skip[d] : 0.0f, bias = a.dt_bias ? a.dt_bias[d] : 0.0f;
+  float* state = a.state ? a.state + (seq0 + at.seq) * a.N * D : nullptr;
+  float* ends = ws.ends + static_cast<size_t>(blockIdx.x) * a.N * D;  // this chunk's slot
 
   const int p0 = at.k * ws.chunk, p1 = min(p0 + ws.chunk, at.len);
   const size_t r0 = row0 + at.row;
-  const T* up = static_cast<const T*>(a.u) + r0 * a.ldu + d;
-  const T* dp = static_cast<const T*>(a.dt) + r0 * a.lddt + d;
-  const T* zp = PASS == kApply && a.z ? static_cast<const T*>(a.z) + r0 * a.ldz + d : nullptr;
-  const T* Bp = static_cast<const T*>(a.B) + r0 * a.ldb;
-  const T* Cp = static_cast<const T*>(a.C) + r0 * a.ldc;
-  T* out = static_cast<T*>(a.out) + r0 * a.ldo + d;
-  float* sB = lds;
-  float* sC = lds + kTile * np;
-  float* sy = lds + 2 * kTile * np + wave / nw * (2 * nw * kGroup4 * 64);  // [2][nw][steps][lane]
-  float total = 0.0f;
-  int flip = 0;
+  const T* up = static_cast<const T*>(a.u) + r0 * a.ldu;
+  const T* dp = static_cast<const T*>(a.dt) + r0 * a.lddt;
+  const T* zp = PASS == kApply && a.z ? static_cast<const T*>(a.z) + r0 * a.ldz : nullptr;
+  T* out = static_cast<T*>(a.out) + r0 * a.ldo;
+  float* wdt = ws.dt ? ws.dt + static_cast<size_t>(at.row) * D : nullptr;
+  const bool ready = PASS == kApply && wdt;  // the steps are
+  const float skip = a.skip ? a.skip[d] : 0.0f, bias = a.dt_bias ? a.dt_bias[d] : 0.0f;
 
-  T un[kGroup4], dn[kGroup4], zn[kGroup4] = {};
-  auto fetch = [&](int p) {
+  // the inputs of two groups of steps, each loaded two groups ahead: a load takes longer than a group
+  struct Inputs {
+    T u[kAhead], dt[kAhead], z[kAhead];
+    float step[kAhead];
+  };
+  Inputs in[2] = {};
+  auto fetch = [&](Inputs& g, int p) {
 #pragma unroll
-    for (int i = 0; i < kGroup4; ++i) {
+    for (int i = 0; i < kAhead; ++i) {
       const size_t r = min(p + i, p1 - 1);
-      un[i] = up[r * a.ldu];
-      dn[i] = dp[r * a.lddt];
-      if (zp) zn[i] = zp[r * a.ldz];
+      g.u[i] = (up + r * a.ldu)[d];
+      if (ready)
+        g.step[i] = (wdt + r * D)[d];
+      else
+        g.dt[i] = (dp + r * a.lddt)[d];
+      if (zp) g.z[i] = (zp + r * a.ldz)[d];
     }
   };
-  fetch(p0);
+  auto step_of = [&](const Inputs& g, int i) {
+    if (ready) return g.step[i];
+    const float v = E::up(g.dt[i]) + bias;
+    return a.softplus ? softplus(v) : v;
+  };
+  fetch(in[0], p0);
+  if (p0 + kAhead < p1) fetch(in[1], p0 + kAhead);
+
+  if (PASS == kSum && at.k == chunks - 1) {  // no sums of the last chunk: its slot keeps the state
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (live && n0 + i < N) (ends + (n0 + i) * D)[d] = state ? (state + (n0 + i) * D)[d] : 0.0f;
+    for (int p = p0; wdt && part == 0 && p < p1; p += kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (live && p + i < p1) (wdt + static_cast<size_t>(p + i) * D)[d] = step_of(in[0], i);
+      in[0] = in[1];
+      fetch(in[1], p + 2 * kAhead);
+    }
+    return;
+  }
+
+  // a tile's B and C: thread i of the block takes state i % NP of every kRows-th step
+  const int sn_ = threadIdx.x % NP, ss = threadIdx.x / NP;
+  const T* Bp = static_cast<const T*>(a.B) + r0 * a.ldb + min(sn_, N - 1);
+  const T* Cp = static_cast<const T*>(a.C) + r0 * a.ldc + min(sn_, N - 1);
+  T bn[kIter], cn[kIter];
+  auto fetch_tile = [&](int pt) {
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const size_t r = min(pt + ss + i * kRows, p1 - 1);
+      bn[i] = Bp[r * a.ldb];
+      if (PASS == kApply) cn[i] = Cp[r * a.ldc];
+    }
+  };
+  fetch_tile(p0);
+
+  // (loads without conditions, so that all are in flight together: what stands past N is not used)
+  float A[NS], h[NS];
+  const float* Ap = a.A + static_cast<size_t>(d) * a.N;
+  if (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < NS; i += 4) {
+      const f4u v = *reinterpret_cast<const f4u*>(Ap + min(n0 + i, N - 4));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) A[i + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) A[i] = Ap[min(n0 + i, N - 1)];
+  }
+  const float* hp = PASS == kApply && ws.ends ? ends : at.k == 0 ? state : nullptr;
+  if (hp) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) h[i] = (hp + min(n0 + i, N - 1) * D)[d];
+  }
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    A[i] = n0 + i < N ? A[i] * 1.44269504f : 0.0f;
+    if (!hp || n0 + i >= N) h[i] = 0.0f;
+  }
+  float total = 0.0f;
+  int flip = 0;
   for (int pt = p0; pt < p1; pt += kTile) {
     const int steps = min(kTile, p1 - pt);
     __syncthreads();
-    for (int i = threadIdx.x; i < steps * np; i += blockDim.x) {
-      const int s = i / np, n = i - s * np;
-      const size_t r = pt + s;
-      sB[i] = n < N ? E::up(Bp[r * a.ldb + n]) : 0.0f;
-      if (PASS == kApply) sC[i] = n < N ? E::up(Cp[r * a.ldc + n]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int s = ss + i * kRows;
+      if (s < kTile) {  // what stands there for no step or state is multiplied by 0 and must be finite
+        const bool in = s < steps && sn_ < N;
+        sB[s * NP + sn_] = in ? E::up(bn[i]) : 0.0f;
+        if (PASS == kApply) sC[s * NP + sn_] = in ? E::up(cn[i]) : 0.0f;
+      }
     }
     __syncthreads();
-    for (int g = 0; g < steps; g += kGroup4) {
-      float u[kGroup4], dt[kGroup4], z[kGroup4];
+    if (pt + kTile < p1) fetch_tile(pt + kTile);
+    float bq[kUnit], cq[kUnit] = {};
+    auto read = [&](int row, int n1) {
+      const int from = row * NP + n0 + n1;
 #pragma unroll
-      for (int i = 0; i < kGroup4; ++i) {
-        u[i] = E::up(un[i]);
-        dt[i] = E::up(dn[i]) + bias;
-        z[i] = E::up(zn[i]);
+      for (int n = 0; n < kUnit; ++n) {
+        bq[n] = sB[from + n];
+        if (PASS == kApply) cq[n] = sC[from + n];
       }
-      if (pt + g + kGroup4 < p1) fetch(pt + g + kGroup4);
+    };
+    read(0, 0);
+    auto group = [&](Inputs& now, int g) {
+      // Steps in a line, with no condition between them; the B and C of a unit of kUnit states are read before
+      // the unit before it is computed. Steps past the end have dt = 0: the decay is 1 and nothing is added.
+      const int left = steps - g;
+      float u[kAhead], step[kAhead], z[kAhead];
 #pragma unroll
-      for (int i = 0; i < kGroup4; ++i) {
-        if (g + i >= steps) break;
-        const float step = a.softplus ? softplus(dt[i]) : dt[i];
-        const float su = step * u[i];
-        const float* b = sB + (g + i) * np + n0;
-        const float* c = sC + (g + i) * np + n0;
-        float y = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          h[n] = __builtin_fmaf(exp2_fast(step * A[n]), h[n], su * b[n]);
-          if (PASS == kApply) y = __builtin_fmaf(c[n], h[n], y);
-        }
-        if (PASS == kSum) {
-          total += step;
-        } else if (nw == 1) {
-          y = __builtin_fmaf(skip, u[i], y);
-          if (zp) y *= silu_fast(z[i]);
-          if (live) out[static_cast<size_t>(pt + g + i) * a.ldo] = E::down(y);
-        } else {
-          sy[((flip * nw + part) * kGroup4 + i) * 64 + lane] = y;
-        }
+      for (int i = 0; i < kAhead; ++i) {
+        u[i] = E::up(now.u[i]);
+        step[i] = step_of(now, i);
+        if (PASS == kSum && wdt && part == 0 && live && i < left) (wdt + static_cast<size_t>(pt + g + i) * D)[d] = step[i];
+        if (i >= left) step[i] = u[i] = 0.0f;
+        if (PASS == kApply) z[i] = E::up(now.z[i]);
       }
-      if (PASS == kApply && nw > 1) {  // the parts' sums in their order; part i % nw writes step i
+      fetch(now, pt + g + 2 * kAhead);
+      float y[kAhead] = {};
+#pragma unroll
+      for (int k = 0; k < kAhead * kUnits; ++k) {
+        const int i = k / kUnits, n1 = k % kUnits * kUnit;
+        float b[kUnit], c[kUnit];
+#pragma unroll
+        for (int n = 0; n < kUnit; ++n) b[n] = bq[n], c[n] = cq[n];
+        // the next unit's B and C (behind the tile's last step: the last one's, unused)
+        if (k + 1 < kAhead * kUnits)
+          read(g + (k + 1) / kUnits, (k + 1) % kUnits * kUnit);
+        else
+          read(min(g + kAhead, kTile - 1), 0);
+        const float su = step[i] * u[i];
+#pragma unroll
+        for (int n = 0; n < kUnit; ++n) {
+          h[n1 + n] = __builtin_fmaf(exp2_fast(step[i] * A[n1 + n]), h[n1 + n], su * b[n]);
+          if (PASS == kApply) y[i] = __builtin_fmaf(c[n], h[n1 + n], y[i]);
+        }
+        if (PASS == kSum && n1 == 0) total += step[i];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (PASS == kSum) return;
+      if constexpr (NW > 1 && PASS == kApply) {  // the parts' sums in their order; part i % NW writes step i
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) sy[cwave][flip][part][i][lane] = y[i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kGroup4; ++i) {
-          if (g + i >= steps || i % nw != part) continue;
-          float y = skip * u[i];
-          for (int w = 0; w < nw; ++w) y += sy[((flip * nw + w) * kGroup4 + i) * 64 + lane];
-          if (zp) y *= silu_fast(z[i]);
-          if (live) out[static_cast<size_t>(pt + g + i) * a.ldo] = E::down(y);
+        for (int i = 0; i < kAhead; ++i) {
+          if (i % NW != part) continue;
+          y[i] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < NW; ++w) y[i] += sy[cwave][flip][w][i][lane];
         }
         flip ^= 1;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (NW > 1 && i % NW != part) continue;
+        float o = __builtin_fmaf(skip, u[i], y[i]);
+        if (zp) o *= silu_fast(z[i]);
+        if (live && i < left) (out + static_cast<size_t>(pt + g + i) * a.ldo)[d] = E::down(o);
+      }
+    };
+    for (int g = 0; g < steps; g += 2 * kAhead) {
+      group(in[0], g);
+      __builtin_amdgcn_sched_barrier(0);
+      if (g + kAhead < steps) {
+        group(in[1], g + kAhead);
+      } else {
+        in[0] = in[1];  // an odd number of groups: only a sequence's end
       }
     }
   }
@@ -174,27 +256,61 @@ __global__ __launch_bounds__(512) void k_scan(ScanArgs a, SeqTab t, ScanWs ws, s
   if (PASS == kSum) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      if (n0 + i < N) end_of(slot, n0 + i) = h[i];
-    if (part == 0) ws.steps[slot * D + d] = total;
+      if (n0 + i < N) (ends + (n0 + i) * D)[d] = h[i];
+    if (part == 0) (ws.sums + static_cast<size_t>(blockIdx.x) * D)[d] = total;
   } else if (state && at.k == chunks - 1) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      if (n0 + i < N) state[(n0 + i) * D] = h[i];
+      if (n0 + i < N) (state + (n0 + i) * D)[d] = h[i];
   }
 }
 
-template <int DT, int NS>
+// The state before each chunk in the place of each chunk's end state: a thread a state of a channel, one
+// sequence a row of blocks, kBatch chunks' loads in flight.
+__global__ __launch_bounds__(256) void k_carry(ScanArgs a, SeqTab t, ScanWs ws) {
+  constexpr int kBatch = 16;
+  const size_t D = a.D, i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int len = t.len > 0 ? t.len : t.row[blockIdx.y + 1] - t.row[blockIdx.y];
+  const int chunks = (len + ws.chunk - 1) / ws.chunk;
+  if (i >= D * a.N || chunks < 2) return;
+  const size_t first = t.len > 0 ? static_cast<size_t>(blockIdx.y) * t.tiles : t.tile[blockIdx.y];
+  const size_t n = i / D, d = i - n * D;
+  const float A = a.A[d * a.N + n] * 1.44269504f;
+  float* ends = ws.ends + first * a.N * D + i;
+  const float* sums = ws.sums + first * D + d;
+  const size_t step = a.N * D;
+  float h = ends[(chunks - 1) * step];  // the state at the start
+  for (int j = 0; j < chunks; j += kBatch) {
+    float e[kBatch], s[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const size_t at = min(j + k, chunks - 1);  // (the last chunk's are not used)
+      e[k] = ends[at * step];
+      s[k] = sums[min(j + k, chunks - 2) * D];
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (j + k >= chunks) break;
+      ends[(j + k) * step] = h;
+      h = j + k ? __builtin_fmaf(exp2_fast(s[k] * A), h, e[k]) : e[k];  // the first one's end has the state in it
+    }
+  }
+}
+
+template <int DT, int NS, int NW>
 hipError_t scan_launch(const ScanArgs& a, const SeqTab& t, const ScanWs& ws, size_t seq0, size_t row0, int tiles,
                        hipStream_t s) {
-  const int nw = static_cast<int>((a.N + NS - 1) / NS), cw = nw >= 4 ? 1 : 4 / nw;
-  const size_t lds = (2 * kTile * static_cast<size_t>(nw) * NS + (nw > 1 ? 2 * nw * kGroup4 * 64 * cw : 0)) * 4;
-  const dim3 grid(tiles, static_cast<unsigned>((a.D + cw * 64 - 1) / (cw * 64)));
+  constexpr int CW = NW >= 4 ? 1 : 4 / NW;
+  const dim3 grid(tiles, static_cast<unsigned>((a.D + CW * 64 - 1) / (CW * 64)));
   if (ws.ends) {
-    k_scan<DT, NS, kSum><<<grid, nw * cw * 64, lds, s>>>(a, t, ws, seq0, row0, nw);
-    const hipError_t e = hipGetLastError();
+    k_scan<DT, NS, NW, kSum><<<grid, NW * CW * 64, 0, s>>>(a, t, ws, seq0, row0);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_carry<<<dim3(static_cast<unsigned>((a.N * a.D + 255) / 256), t.n), 256, 0, s>>>(a, t, ws);
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  k_scan<DT, NS, kApply><<<grid, nw * cw * 64, lds, s>>>(a, t, ws, seq0, row0, nw);
+  k_scan<DT, NS, NW, kApply><<<grid, NW * CW * 64, 0, s>>>(a, t, ws, seq0, row0);
   return hipGetLastError();
 }
 
@@ -216,11 +332,15 @@ hipError_t launch_sel_scan(const ScanArgs& a, float* ws_mem, hipStream_t s) {
         ws.chunk = plan.chunk;
         if (plan.split) {
           ws.ends = ws_mem;
-          ws.steps = ws_mem + static_cast<size_t>(tiles) * a.N * a.D;
+          ws.sums = ws_mem + static_cast<size_t>(tiles) * a.N * a.D;
+          if (rows * a.D <= kLayerWsBytes / 4 - kScanWsFloats) ws.dt = ws_mem + kScanWsFloats;
         }
-        const hipError_t e = a.N <= 4   ? scan_launch<DT, 4>(a, t, ws, q, row0, tiles, s)
-                             : a.N <= 8 ? scan_launch<DT, 8>(a, t, ws, q, row0, tiles, s)
-                                        : scan_launch<DT, 16>(a, t, ws, q, row0, tiles, s);
+        const hipError_t e = a.N <= 4    ? scan_launch<DT, 4, 1>(a, t, ws, q, row0, tiles, s)
+                             : a.N <= 8  ? scan_launch<DT, 8, 1>(a, t, ws, q, row0, tiles, s)
+                             : a.N <= 16 ? scan_launch<DT, 16, 1>(a, t, ws, q, row0, tiles, s)
+                             : a.N <= 32 ? scan_launch<DT, 16, 2>(a, t, ws, q, row0, tiles, s)
+                             : a.N <= 64 ? scan_launch<DT, 16, 4>(a, t, ws, q, row0, tiles, s)
+                                         : scan_launch<DT, 16, 8>(a, t, ws, q, row0, tiles, s);
         if (e != hipSuccess) return e;
       }
       row0 += rows;
