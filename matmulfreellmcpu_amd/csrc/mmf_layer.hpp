@@ -124,24 +124,25 @@ inline const char* check_w4(size_t N, size_t K, size_t group) {
   return nullptr;
 }
 
-// Many rows are laid out as matrix operands first (mmf_w4.hip): bytes of 16 rows' fragments, and with the
-// fp32 or int32 sums of their inputs; rows of a pass, so that these fit the workspace.
+// Many rows are laid out as matrix operands first (mmf_w4.hip): bytes of 16 rows' fragments (fp32: two fp16
+// parts), and with a number for each row and scale; rows of a pass, so that these fit the workspace.
 constexpr size_t kLayerWsBytes = size_t{128} << 20;
 inline size_t w4_frag_bytes(int dtype, const W4Geom& g) {
-  return static_cast<size_t>(g.nc) * 128 * 16 * (dtype == kF32 ? 6 : dtype == kI8 ? 1 : 2);
+  return static_cast<size_t>(g.nc) * 128 * 16 * (dtype == kF32 ? 4 : dtype == kI8 ? 1 : 2);
 }
 inline size_t w4_lay_bytes(int dtype, const W4Geom& g, int row_tiles) {  // fragments and sums
   return row_tiles * (w4_frag_bytes(dtype, g) + static_cast<size_t>(g.ns) * 64);
 }
-inline constexpr int w4_tile_rows(int dtype) { return dtype == kF32 ? 32 : 64; }  // of a wave
+constexpr int kW4TileRows = 64;  // of a wave
 
-// How the many-row kernel's 8 waves stand (wn over 64 outputs each, wr over w4_tile_rows rows each, 8 / (wn wr)
+// How the many-row kernel's 8 waves stand (wn over 64 outputs each, wr over kW4TileRows rows each, 8 / (wn wr)
 // over the inputs) and over how many blocks a tile's inputs are split.
 struct W4Plan {
   int wn, wr, ks;
 };
 inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
-  const int tt = w4_tile_rows(dtype) / 16;
+  constexpr int tt = kW4TileRows / 16;
+  (void)dtype;
   auto blocks = [&](int wn, int wr) {
     return static_cast<size_t>((g.nt + wn * 4 - 1) / (wn * 4)) * ((row_tiles + wr * tt - 1) / (wr * tt));
   };

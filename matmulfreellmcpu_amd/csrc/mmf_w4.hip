@@ -101,6 +101,18 @@ __device__ __forceinline__ void i8_operand(uint32_t x0, uint32_t x1, uint32_t& l
   hi = __builtin_amdgcn_perm(x1, x0, 0x07030602);
 }
 
+// Pairs of fp16: a - b, exact for 128 + q and 128 + z.
+__device__ __forceinline__ u32x4 less(u32x4 a, uint32_t b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = a[i];  // (a bit_cast of the element itself takes element 0)
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - __builtin_bit_cast(f16x2, b));
+  }
+  return r;
+}
+
 // 16 bytes of a row of 16-bit elements (8) or bytes (16) from element k, zeros behind K.
 template <int DT>
 __device__ __forceinline__ u32x4 row_16B(const char* row, int k, int K, bool whole) {
@@ -386,10 +398,16 @@ hipError_t rows_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
 // ---- many rows ------------------------------------------------------------------------------------
 // The rows are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
 // FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
-// l % 16; zeros behind the last row and input. fp32 rows are three bf16 parts, whose products go into
-// one sum. Beside them stand the sums of a row's inputs over each scale's inputs, [tile][chunk][S][16].
-template <int DT> constexpr int kParts = DT == kF32 ? 3 : 1;
+// l % 16; zeros behind the last row and input. Beside them stands a number for each row and scale's inputs,
+// [tile][chunk][S][16]:
+//   fp32 rows are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of fp32, with 2^k
+//     bringing the largest of a scale's inputs below 2^15; the number is 2^-k (NaN where an input is none);
+//   fp16 rows are as they are, and it is 1;
+//   bf16 and int8 rows are as they are, and it is the sum of the inputs.
+// fp16 operands take the codes with the zero point off: 128 + q and 128 + z are exact, and so is q - z.
+template <int DT> constexpr int kParts = DT == kF32 ? 2 : 1;
 template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
+template <int DT> constexpr int kOperand = DT == kF32 ? kF16 : DT;
 
 // One block a tile and chunk; 16 lanes a row, 8 inputs a thread.
 template <int DT, int STEP>
@@ -404,27 +422,38 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
   const int h = j >> 1;
   char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
   uint32_t total;
+  constexpr int U = STEP / 8;  // neighbouring threads that share a scale
   if constexpr (DT == kF32) {
-    float v[8], sum = 0.0f;
-    uint32_t part[3][8];
+    float v[8];
+    uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN are the largest
     const float* x = static_cast<const float*>(a.x) + row * a.ldx + k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = in && k + i < g.K ? x[i] : 0.0f;
-      sum += v[i];
-      part[0][i] = __builtin_bit_cast(uint32_t, v[i]) & 0xFFFF0000u;
-      const float r1 = v[i] - __builtin_bit_cast(float, part[0][i]);
-      part[1][i] = __builtin_bit_cast(uint32_t, r1) & 0xFFFF0000u;
-      part[2][i] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, part[1][i]));
+      top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
     }
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      u32x4 o;
+    for (int n = 1; n < U; n *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), n)));
+    const uint32_t e = top >> 23, up = min(268u - e, 253u);  // 2^k with k = 14 - exponent, at most 2^126
+    const float f = __builtin_bit_cast(float, up << 23);
+    u32x4 hi, lo;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = (part[p][2 * i] >> 16) | (part[p][2 * i + 1] & 0xFFFF0000u);
-      *reinterpret_cast<u32x4*>(to + (p * FR + (j & 1)) * 1024) = o;
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h[2], l[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float y = v[2 * i + m] * f;
+        const _Float16 p = static_cast<_Float16>(y);
+        h[m] = __builtin_bit_cast(uint16_t, p);
+        l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
+      }
+      hi[i] = h[0] | h[1] << 16;
+      lo[i] = l[0] | l[1] << 16;
     }
-    total = __builtin_bit_cast(uint32_t, sum);
+    *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = hi;
+    *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
+    if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = e == 255 ? 0x7FC00000u : (254 - up) << 23;
+    return;
   } else if constexpr (DT == kI8) {
     uint32_t x0 = 0, x1 = 0;
     int sum = 0;
@@ -453,8 +482,11 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
     }
     *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = o;
     total = __builtin_bit_cast(uint32_t, sum);
+    if (DT == kF16) {
+      if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = 0x3F800000u;
+      return;
+    }
   }
-  constexpr int U = STEP / 8;  // neighbouring threads that share a scale
 #pragma unroll
   for (int n = 1; n < U; n *= 2) {
     const uint32_t o = __shfl_xor(static_cast<int>(total), n);
@@ -471,7 +503,7 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
 // LDS, shared by a group's waves, a stage (a chunk, or with three parts half a chunk) ahead through
 // registers; codes go straight to their operand's place. The codes' products are summed for a scale's
 // inputs alone, and the scale multiplies that sum, so the weights enter unrounded.
-template <int DT> constexpr int kRowTiles = DT == kF32 ? 2 : 4;  // of a wave: what the registers hold
+constexpr int kRowTiles = 4;                                 // of a wave: what the registers hold
 template <int DT> constexpr int kHalves = DT == kF32 ? 1 : 2;    // half chunks of a stage
 template <int DT> constexpr int kStageKB = kHalves<DT>* kParts<DT>* kFrags<DT>;  // of a tile of rows
 
@@ -479,9 +511,10 @@ template <int DT, int STEP, int WN>
 __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint32_t* codes, const uint32_t* scales,
                                                  const char* frags, const uint32_t* sums, float* partials, int wr,
                                                  int row_tiles) {
-  using M = Mat<DT>;
+  constexpr int OT = kOperand<DT>;
+  using M = Mat<OT>;
   using Acc = typename M::Acc;
-  constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP, TT = kRowTiles<DT>, H = kHalves<DT>, KB = kStageKB<DT>;
+  constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP, TT = kRowTiles, H = kHalves<DT>, KB = kStageKB<DT>;
   constexpr int kPieces = (TT * KB + WN - 1) / WN;  // KB that a wave moves of a stage
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -570,6 +603,18 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
       const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
       const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + (WN * 4 + ir * TT) * S * 16 + (lane & 15);
 
+      // the zero points of this lane's outputs of the operand (lane % 16 of each tile), as pairs of 128 + z
+      uint32_t zero[4];
+      auto zeros = [&](int s) {
+        if constexpr (OT == kF16) {
+          const uint32_t* z_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + (lane & 15);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t z = z_at[(n * S + s) * 16] >> 16;
+            zero[n] = M::bits + (z << 3 | z << 19);
+          }
+        }
+      };
       auto clear = [&] {
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -589,7 +634,9 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
             const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[i])));
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-              if constexpr (DT == kI8) {
+              if constexpr (OT == kF16) {
+                acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(float, x[t]), acc[n][t][i]);
+              } else if constexpr (DT == kI8) {
                 acc[n][t][i] = __builtin_fmaf(
                     sc, static_cast<float>(d[n][t][i] - static_cast<int>(sz[i] >> 16) * static_cast<int>(x[t])), acc[n][t][i]);
               } else {
@@ -639,12 +686,16 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
           }
         } else {
           if (STEP == 64 || (STEP == 128 && half == 0)) clear();
+          if (STEP >= 64) zeros(STEP == 64 ? half : 0);
 #pragma unroll
           for (int jj = 0; jj < 2; ++jj) {
-            if (STEP == 32) clear();
+            if (STEP == 32) clear(), zeros(2 * half + jj);
             u32x4 aw[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) aw[n] = w4_operand<DT>(w[n][2 * half + jj]);
+            for (int n = 0; n < 4; ++n) {
+              aw[n] = w4_operand<OT>(w[n][2 * half + jj]);
+              if constexpr (OT == kF16) aw[n] = less(aw[n], zero[n]);
+            }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
               u32x4 b[TT];
@@ -752,8 +803,8 @@ hipError_t gemm_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
   k_w4_lay<DT, STEP><<<dim3(g.nc, rt), 256, 0, s>>>(a, g, ws, sums);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  constexpr int TT = kRowTiles<DT>, S = 128 / STEP;
-  static_assert(TT == w4_tile_rows(DT) / 16, "the plan's tiles");
+  constexpr int TT = kRowTiles, S = 128 / STEP;
+  static_assert(TT == kW4TileRows / 16, "the plan's tiles");
   const W4Plan p = w4_plan(DT, g, rt);
   const int wn = p.wn, wr = p.wr, kw = 8 / (wn * wr);
   const size_t buf = static_cast<size_t>(wr) * TT * kStageKB<DT> * 1024 + (wn * 4 + wr * TT) * S * 64;
