@@ -135,10 +135,10 @@ inline size_t w4_lay_bytes(int dtype, const W4Geom& g, int row_tiles) {  // frag
 }
 constexpr int kW4TileRows = 64;  // of a wave
 
-// How the many-row kernel's 8 waves stand (wn over 64 outputs each, wr over kW4TileRows rows each, 8 / (wn wr)
-// over the inputs) and over how many blocks a tile's inputs are split.
+// How the many-row kernel's waves stand (wn over 64 outputs each, wr over kW4TileRows rows each, bk over the
+// inputs; 4 or 8 in all) and over how many blocks a tile's inputs are split.
 struct W4Plan {
-  int wn, wr, ks;
+  int wn, wr, bk, ks;
 };
 inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
   constexpr int tt = kW4TileRows / 16;
@@ -146,11 +146,11 @@ inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
   auto blocks = [&](int wn, int wr) {
     return static_cast<size_t>((g.nt + wn * 4 - 1) / (wn * 4)) * ((row_tiles + wr * tt - 1) / (wr * tt));
   };
-  W4Plan p{2, 1, 1};
-  if (blocks(4, 2) >= 200)
-    p = {4, 2, 1};
+  W4Plan p{2, 1, 4, 1};
+  if (blocks(4, 1) >= 400)
+    p = {4, 1, 1, 1};
   else if (blocks(4, 1) >= 200)
-    p = {4, 1, 1};
+    p = {4, 1, 2, 1};
   return p;
 }
 // The same, with no more splits than the workspace holds the sums of beside the laid out rows.

@@ -324,7 +324,7 @@ __global__ __launch_bounds__(CT == 1 ? 1024 : 512) void k_w4_rows(W4Args a, W4Ge
 #pragma unroll
           for (int t = 0; t < CT; ++t) {
             if constexpr (DT == kI8) {
-              acc[n][t][i] = __builtin_fmaf(sc, static_cast<float>(d[n][t][i] - static_cast<int>(v >> 16) * sum[t][i]),
+              acc[n][t][i] = __builtin_fmaf(sc, static_cast<float>(d[n][t][i] - __mul24(static_cast<int>(v >> 16), sum[t][i])),
                                             acc[n][t][i]);
             } else {
               const float z = static_cast<float>(v >> 16) + M::base;
@@ -638,7 +638,7 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
                 acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(float, x[t]), acc[n][t][i]);
               } else if constexpr (DT == kI8) {
                 acc[n][t][i] = __builtin_fmaf(
-                    sc, static_cast<float>(d[n][t][i] - static_cast<int>(sz[i] >> 16) * static_cast<int>(x[t])), acc[n][t][i]);
+                    sc, static_cast<float>(d[n][t][i] - __mul24(static_cast<int>(sz[i] >> 16), static_cast<int>(x[t]))), acc[n][t][i]);
               } else {
                 const float z = static_cast<float>(sz[i] >> 16) + M::base;
                 acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, __builtin_bit_cast(float, x[t]), d[n][t][i]), acc[n][t][i]);
@@ -806,15 +806,15 @@ hipError_t gemm_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
   constexpr int TT = kRowTiles, S = 128 / STEP;
   static_assert(TT == kW4TileRows / 16, "the plan's tiles");
   const W4Plan p = w4_plan(DT, g, rt);
-  const int wn = p.wn, wr = p.wr, kw = 8 / (wn * wr);
+  const int wn = p.wn, wr = p.wr, kw = p.bk;
   const size_t buf = static_cast<size_t>(wr) * TT * kStageKB<DT> * 1024 + (wn * 4 + wr * TT) * S * 64;
   const size_t red = static_cast<size_t>(kw - 1) * wn * wr * TT * 4096, lds = 2 * kw * buf > red ? 2 * kw * buf : red;
   const dim3 grid((g.nt + wn * 4 - 1) / (wn * 4), (rt + wr * TT - 1) / (wr * TT), p.ks);
   float* partials = p.ks > 1 ? reinterpret_cast<float*>(ws + w4_lay_bytes(DT, g, rt)) : nullptr;
   if (wn == 4)
-    k_w4_gemm<DT, STEP, 4><<<grid, 512, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
+    k_w4_gemm<DT, STEP, 4><<<grid, wn * wr * kw * 64, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
   else
-    k_w4_gemm<DT, STEP, 2><<<grid, 512, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
+    k_w4_gemm<DT, STEP, 2><<<grid, wn * wr * kw * 64, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
   e = hipGetLastError();
   if (e != hipSuccess || !partials) return e;
   k_w4_sum<DT><<<dim3((g.N + 1023) / 1024, static_cast<unsigned>(a.rows)), 256, 0, s>>>(a, g, partials, rt, p.ks);
