@@ -135,35 +135,39 @@ inline size_t w4_lay_bytes(int dtype, const W4Geom& g, int row_tiles) {  // frag
 }
 constexpr int kW4TileRows = 64;  // of a wave
 
-// How the many-row kernel's waves stand (wn over 64 outputs each, wr over kW4TileRows rows each, bk over the
-// inputs; 4 or 8 in all) and over how many blocks a tile's inputs are split.
+// How the many-row kernel's waves stand (wn over 64 outputs each, bk over the inputs; 4 or 8 in all, of
+// kW4TileRows rows) and over how many blocks a tile's inputs are split.
 struct W4Plan {
-  int wn, wr, bk, ks;
+  int wn, bk, ks;
 };
-inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
-  constexpr int tt = kW4TileRows / 16;
-  (void)dtype;
-  auto blocks = [&](int wn, int wr) {
-    return static_cast<size_t>((g.nt + wn * 4 - 1) / (wn * 4)) * ((row_tiles + wr * tt - 1) / (wr * tt));
+// A block multiplies 64 wn outputs by 64 rows. Blocks of 256 outputs and four waves, two on a compute unit,
+// where there are more than 256 of them (2048 x 2048 x 11264 fp32, us: 200, and as half as many blocks of eight
+// waves 215; 224 with the inputs split over two groups of waves). Down to 130, two groups over the inputs (256
+// x 2048 x 11264 43, by smaller tiles 55). Below, tiles of 128 outputs and four groups, and the inputs over as
+// many blocks as the chip takes at once: 64 x 6912 x 2560 78 -> 27 by 8, 128 x 6912 x 2560 81 -> 36 by 4.
+inline W4Plan w4_pick(const W4Geom& g, int row_tiles) {
+  auto blocks = [&](int wn) {
+    return static_cast<size_t>((g.nt + wn * 4 - 1) / (wn * 4)) * ((row_tiles + kW4TileRows / 16 - 1) / (kW4TileRows / 16));
   };
-  W4Plan p{2, 1, 4, 1};
-  if (blocks(4, 1) >= 400)
-    p = {4, 1, 1, 1};
-  else if (blocks(4, 1) >= 200)
-    p = {4, 1, 2, 1};
+  if (blocks(4) > 256) return {4, 1, 1};
+  if (blocks(4) >= 130) return {4, 2, 1};
+  W4Plan p{2, 4, 1};
+  while (blocks(2) * p.ks * 2 <= 256 && p.ks * 8 <= g.nc) p.ks *= 2;
   return p;
 }
 // The same, with no more splits than the workspace holds the sums of beside the laid out rows.
 inline W4Plan w4_plan(int dtype, const W4Geom& g, int row_tiles) {
-  W4Plan p = w4_pick(dtype, g, row_tiles);
+  W4Plan p = w4_pick(g, row_tiles);
   const size_t one = static_cast<size_t>(row_tiles) * g.nt * 1024;  // bytes of one split's sums
   const size_t room = kLayerWsBytes - w4_lay_bytes(dtype, g, row_tiles);
   while (p.ks > 1 && p.ks * one > room) p.ks /= 2;
   return p;
 }
+// Whether a call's rows are laid out: from 0.6 G products of fp32 rows on, 2.5 G of others (us, by the kernel
+// of few rows -> laid out: fp32 64 x 2048 x 2048 10 -> 17, 64 x 6912 x 2560 40 -> 27; bf16 128 x 6912 x 2560
+// 21 -> 25, 128 x 2048 x 11264 23 -> 19). Laying out and its launches cost 10 to 15 us.
 inline bool w4_lays(int dtype, const W4Geom& g, size_t rows) {
-  (void)g;
-  return rows > (dtype == kF32 ? 20 : 64);
+  return rows > 16 && static_cast<double>(rows) * g.K * g.N > (dtype == kF32 ? 0.6e9 : 2.5e9);
 }
 inline size_t w4_rows_most(int dtype, const W4Geom& g, size_t rows) {
   if (!w4_lays(dtype, g, rows)) return 65535 * 5;  // the grid's second dimension, in tiles of 5 rows or more

@@ -138,7 +138,7 @@ constexpr int kPartStride = 272;  // bytes of a column's 128 parts in LDS, 16 ap
 template <int DT, int CT> constexpr int kPartBytes = DT == kF32 ? CT * 15 * kPartStride : 0;
 
 template <int DT, int STEP, int NT, int CT>
-__global__ __launch_bounds__(CT == 1 ? 1024 : 512) void k_w4_rows(W4Args a, W4Geom g, const uint32_t* codes,
+__global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4Args a, W4Geom g, const uint32_t* codes,
                                                                       const uint32_t* scales) {
   using M = Mat<DT>;
   using Acc = typename M::Acc;
@@ -374,19 +374,35 @@ hipError_t rows_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
   return hipGetLastError();
 }
 
+// Tiles of outputs a wave (nt) and waves a block. `units` is the tiles of outputs times the groups of rows.
+// One column tile: a wave a tile; 16 waves where the inputs are long (us: 1 x 6912 x 2560 fp32 6.6 by 8 waves,
+// 5.4 by 16; 1 x 2048 x 11264 5.2 and 6.8). Many rows of one tile share the rows' operands over four tiles of
+// outputs instead where there are enough of these (bf16 16 x 2048 x 11264 8.8 -> 6.9).
+// Two column tiles: the rows' operands are most of what is read, so a wave takes as many tiles of outputs as leave
+// the chip full, and fewer waves share a block when there are more of them (bf16, one tile -> chosen: 64 x 6912 x
+// 2560 28.1 -> 17.7, 128 x 6912 x 2560 41 -> 21, 128 x 2048 x 11264 45 -> 23). fp32 rows, whose parts are
+// made anew for each column tile, gain less (64 x 2048 x 11264 64 -> 44) and take two at most.
 template <int DT, int STEP>
 hipError_t rows_pick(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s) {
-  const int R = kTileRows<DT>;
-  const int ct = a.rows <= static_cast<size_t>(R) ? 1 : 2;
-  const size_t groups = (a.rows + ct * R - 1) / (ct * R);
-  const int nt = g.nt * groups >= 512 ? 2 : 1;
+  constexpr size_t R = kTileRows<DT>;
+  constexpr bool F = DT == kF32;
+  if (a.rows <= R) {
+    if constexpr (!F) {
+      if (a.rows > 8 && g.nt >= 512) return rows_launch<DT, STEP, 4, 1>(a, g, codes, scales, g.nc < 8 ? g.nc : 8, s);
+    }
+    const int most = g.nc > 32 ? 16 : 8;
+    return rows_launch<DT, STEP, 1, 1>(a, g, codes, scales, g.nc < most ? g.nc : most, s);
+  }
+  const size_t groups = (a.rows + 2 * R - 1) / (2 * R), units = g.nt * groups;
+  const int nt = units <= (F ? 512 : 256) ? 1 : F || units <= 512 ? 2 : 4;
   const size_t blocks = (g.nt + nt - 1) / nt * groups;
-  int waves = ct == 1 ? 16 : 8;
-  while (waves > 1 && (blocks * waves > 8192 || waves > g.nc)) waves /= 2;
-  if (ct == 1) return nt == 1 ? rows_launch<DT, STEP, 1, 1>(a, g, codes, scales, waves, s)
-                              : rows_launch<DT, STEP, 2, 1>(a, g, codes, scales, waves, s);
-  return nt == 1 ? rows_launch<DT, STEP, 1, 2>(a, g, codes, scales, waves, s)
-                 : rows_launch<DT, STEP, 2, 2>(a, g, codes, scales, waves, s);
+  const int most = blocks <= (F ? 1536 : nt == 4 ? 256 : 512) ? 8 : F || blocks <= 512 ? 4 : 2;
+  const int waves = g.nc < most ? g.nc : most;
+  if (nt == 1) return rows_launch<DT, STEP, 1, 2>(a, g, codes, scales, waves, s);
+  if constexpr (!F) {
+    if (nt == 4) return rows_launch<DT, STEP, 4, 2>(a, g, codes, scales, waves, s);
+  }
+  return rows_launch<DT, STEP, 2, 2>(a, g, codes, scales, waves, s);
 }
 
 template <int DT>
@@ -498,8 +514,8 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
   if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = total;
 }
 
-// A block of kw groups of wn x wr waves, a wave 64 outputs by TT tiles of rows; the groups take chunks in
-// turn, and their sums meet in LDS in a fixed order. The rows' fragments, the scales and the sums go through
+// A block of up to four groups of WN waves, a wave 64 outputs by TT tiles of rows; the groups, of all blocks of a
+// tile, take chunks in turn, and a block's sums meet in LDS in a fixed order. The rows' fragments, the scales and the sums go through
 // LDS, shared by a group's waves, a stage (a chunk, or with three parts half a chunk) ahead through
 // registers; codes go straight to their operand's place. The codes' products are summed for a scale's
 // inputs alone, and the scale multiplies that sum, so the weights enter unrounded.
@@ -509,22 +525,22 @@ template <int DT> constexpr int kStageKB = kHalves<DT>* kParts<DT>* kFrags<DT>; 
 
 template <int DT, int STEP, int WN>
 __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint32_t* codes, const uint32_t* scales,
-                                                 const char* frags, const uint32_t* sums, float* partials, int wr,
+                                                 const char* frags, const uint32_t* sums, float* partials,
                                                  int row_tiles) {
   constexpr int OT = kOperand<DT>;
   using M = Mat<OT>;
   using Acc = typename M::Acc;
   constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP, TT = kRowTiles, H = kHalves<DT>, KB = kStageKB<DT>;
-  constexpr int kPieces = (TT * KB + WN - 1) / WN;  // KB that a wave moves of a stage
+  constexpr int kPieces = TT * KB / WN;  // KB that a wave moves of a stage
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int gw = WN * wr, bk = (blockDim.x >> 6) / gw, group = wave / gw, gwave = wave - group * gw;
+  const int bk = (blockDim.x >> 6) / WN, group = wave / WN, in = wave % WN;
   const int kw = bk * gridDim.z, kg = blockIdx.z * bk + group;  // the chunks' groups, of all blocks of a tile
-  const int in = gwave % WN, ir = gwave / WN, gthread = threadIdx.x - group * gw * 64;
+  const int gthread = threadIdx.x - group * WN * 64;
   const int q = lane >> 4;
-  const int btile = blockIdx.x * (WN * 4), tile0 = btile + in * 4, rt0 = blockIdx.y * (wr * TT);
-  // LDS of a group: two buffers of the rows' pieces, the scales [WN 4][S][16] and the sums [wr TT][S][16]
-  const int pieces = wr * TT * KB, words = (WN * 4 + wr * TT) * S * 16, buf_bytes = pieces * 1024 + words * 4;
+  const int btile = blockIdx.x * (WN * 4), tile0 = btile + in * 4, rt0 = blockIdx.y * TT;
+  // LDS of a group: two buffers of the rows' pieces, the scales [WN 4][S][16] and the rows' numbers [TT][S][16]
+  constexpr int pieces = TT * KB, words = (WN * 4 + TT) * S * 16, buf_bytes = pieces * 1024 + words * 4;
   char* mem = lds + group * 2 * buf_bytes;
 
   const uint32_t* cw[4];
@@ -534,21 +550,19 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
   // Loads and LDS writes have no conditions (an index past the end repeats the last one), so that the
   // compiler knows which loads are in flight and waits for no younger ones.
   u32x4 hold[kPieces];
-  constexpr int kWords = ((WN * 4 + 2 * TT) * S * 16 + WN * 128 - 1) / (WN * 128);  // a thread's, of wr = 2
-  constexpr int kWords1 = ((WN * 4 + TT) * S * 16 + WN * 64 - 1) / (WN * 64);       // ... of wr = 1
-  constexpr int kW = kWords > kWords1 ? kWords : kWords1;
+  constexpr int kW = (words + WN * 64 - 1) / (WN * 64);  // words that a thread moves
   uint32_t hold_w[kW];
   const char* from_p[kPieces];
   const uint32_t* from_w[kW];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const int p = i * gw + gwave;
+    const int p = i * WN + in;
     const size_t rt = min(rt0 + p / KB, row_tiles - 1);
     from_p[i] = frags + rt * g.nc * (2 / H) * (KB * 1024) + (p % KB) * 1024 + lane * 16;
   }
 #pragma unroll
   for (int i = 0; i < kW; ++i) {
-    const int v = min(i * gw * 64 + gthread, words - 1), unit = v / (S * 16), at = v - unit * (S * 16);
+    const int v = min(i * WN * 64 + gthread, words - 1), unit = v / (S * 16), at = v - unit * (S * 16);
     from_w[i] = (unit < WN * 4 ? scales + static_cast<size_t>(min(btile + unit, g.nt - 1)) * g.ns * 16
                                : sums + static_cast<size_t>(min(rt0 + unit - WN * 4, row_tiles - 1)) * g.ns * 16) + at;
   }
@@ -562,10 +576,10 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
   auto put = [&](int buf) {
     char* to = mem + buf * buf_bytes;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(to + (i * gw + gwave) * 1024 + lane * 16) = hold[i];
+    for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(to + (i * WN + in) * 1024 + lane * 16) = hold[i];
     uint32_t* tw = reinterpret_cast<uint32_t*>(to + pieces * 1024);
 #pragma unroll
-    for (int i = 0; i < kW; ++i) tw[min(i * gw * 64 + gthread, words - 1)] = hold_w[i];
+    for (int i = 0; i < kW; ++i) tw[min(i * WN * 64 + gthread, words - 1)] = hold_w[i];
   };
 
   f32x4 acc[4][TT];
@@ -599,9 +613,9 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
       else
         fetch(min(c, last), 1);
       const char* buf = mem + cur * buf_bytes;
-      const char* mine = buf + ir * TT * KB * 1024 + lane * 16;
+      const char* mine = buf + lane * 16;
       const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
-      const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + (WN * 4 + ir * TT) * S * 16 + (lane & 15);
+      const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + WN * 4 * S * 16 + (lane & 15);
 
       // the zero points of this lane's outputs of the operand (lane % 16 of each tile), as pairs of 128 + z
       uint32_t zero[4];
@@ -724,7 +738,7 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) red[(((group - 1) * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane] = acc[n][t];
+        for (int t = 0; t < TT; ++t) red[(((group - 1) * WN + in) * (4 * TT) + n * TT + t) * 64 + lane] = acc[n][t];
     }
     __syncthreads();
     if (group > 0) return;
@@ -732,12 +746,12 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) acc[n][t] += red[((k * gw + gwave) * (4 * TT) + n * TT + t) * 64 + lane];
+        for (int t = 0; t < TT; ++t) acc[n][t] += red[((k * WN + in) * (4 * TT) + n * TT + t) * 64 + lane];
   }
   if (partials) {  // one of several blocks of this tile: k_w4_sum adds them
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      const int rt = rt0 + ir * TT + t;
+      const int rt = rt0 + t;
       if (rt >= row_tiles) continue;
       float* to = partials + ((static_cast<size_t>(blockIdx.z) * row_tiles + rt) * 16 + (lane & 15)) * (g.nt * 16) + 4 * q;
 #pragma unroll
@@ -751,7 +765,7 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
     typedef typename O::T T4 __attribute__((ext_vector_type(4), aligned(sizeof(typename O::T))));
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      const size_t row = static_cast<size_t>(rt0 + ir * TT + t) * 16 + (lane & 15);
+      const size_t row = static_cast<size_t>(rt0 + t) * 16 + (lane & 15);
       if (row >= a.rows) continue;
       const float xsc = DT == kI8 ? a.xscales[row] : 1.0f;
       typename O::T* out = static_cast<typename O::T*>(a.out) + row * a.ldo;
@@ -806,15 +820,15 @@ hipError_t gemm_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
   constexpr int TT = kRowTiles, S = 128 / STEP;
   static_assert(TT == kW4TileRows / 16, "the plan's tiles");
   const W4Plan p = w4_plan(DT, g, rt);
-  const int wn = p.wn, wr = p.wr, kw = p.bk;
-  const size_t buf = static_cast<size_t>(wr) * TT * kStageKB<DT> * 1024 + (wn * 4 + wr * TT) * S * 64;
-  const size_t red = static_cast<size_t>(kw - 1) * wn * wr * TT * 4096, lds = 2 * kw * buf > red ? 2 * kw * buf : red;
-  const dim3 grid((g.nt + wn * 4 - 1) / (wn * 4), (rt + wr * TT - 1) / (wr * TT), p.ks);
+  const size_t buf = TT * kStageKB<DT> * 1024 + (p.wn * 4 + TT) * S * 64, stages = 2 * p.bk * buf;
+  const size_t red = (p.bk - 1) * p.wn * TT * 4096, lds = stages > red ? stages : red;  // up to 152 KB
+  const dim3 grid((g.nt + p.wn * 4 - 1) / (p.wn * 4), (rt + TT - 1) / TT, p.ks);
   float* partials = p.ks > 1 ? reinterpret_cast<float*>(ws + w4_lay_bytes(DT, g, rt)) : nullptr;
-  if (wn == 4)
-    k_w4_gemm<DT, STEP, 4><<<grid, wn * wr * kw * 64, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
+  const int threads = p.wn * p.bk * 64;
+  if (p.wn == 4)
+    k_w4_gemm<DT, STEP, 4><<<grid, threads, lds, s>>>(a, g, codes, scales, ws, sums, partials, rt);
   else
-    k_w4_gemm<DT, STEP, 2><<<grid, wn * wr * kw * 64, lds, s>>>(a, g, codes, scales, ws, sums, partials, wr, rt);
+    k_w4_gemm<DT, STEP, 2><<<grid, threads, lds, s>>>(a, g, codes, scales, ws, sums, partials, rt);
   e = hipGetLastError();
   if (e != hipSuccess || !partials) return e;
   k_w4_sum<DT><<<dim3((g.N + 1023) / 1024, static_cast<unsigned>(a.rows)), 256, 0, s>>>(a, g, partials, rt, p.ks);

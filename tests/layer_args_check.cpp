@@ -224,7 +224,31 @@ static void plans() {
       }
 }
 
+// The many-row product's plan: the laid out rows and the blocks' sums within the workspace, whatever the shape.
+static void products_plan() {
+  for (size_t N : {1, 16, 1333, 11264, 50000, 1000000})
+    for (size_t K : {1, 130, 1031, 6912, 100000, 1000000})
+      for (size_t rows : {1, 16, 100, 2048, 70000})
+        for (int t : {kF32, kBF16, kF16, kI8})
+          for (size_t group : {size_t{32}, size_t{64}, size_t{128}, size_t{0}}) {
+            const W4Geom g = w4_geom(N, K, group);
+            const size_t most = w4_rows_most(t, g, rows);
+            is("rows of a pass", most >= 1, 1);
+            if (!w4_lays(t, g, rows)) continue;
+            for (size_t r : {most < rows ? most : rows, rows % most ? rows % most : size_t{1}}) {
+              const int rt = static_cast<int>((r + 15) / 16);
+              const W4Plan p = w4_plan(t, g, rt);
+              const size_t sums = p.ks > 1 ? static_cast<size_t>(p.ks) * rt * 16 * g.nt * 16 * 4 : 0;
+              is("workspace of a product", w4_lay_bytes(t, g, rt) + sums <= kLayerWsBytes, 1);
+              is("waves", p.wn * p.bk == 4 || p.wn * p.bk == 8, 1);
+              is("grid", rt <= 65535 && r <= 65535 * 16, 1);
+              if (p.ks > 1) is("grid of sums", r <= 65535, 1);
+            }
+          }
+}
+
 int main() {
+  products_plan();
   plans();
   norms();
   products();
