@@ -149,8 +149,10 @@ int mmf_rmsnorm_swishgate(mmf_ctx* ctx, float* out, const float* g, const float*
  * and ld elements apart (0: as long as a row; never less). Sums, states and scales are fp32 or
  * wider, and each output is rounded to its type once, to nearest even. Outputs may not overlap
  * other tensors of the call unless said otherwise (MMF_ERR_ARG where the addresses show it).
- * Nothing is allocated by these calls but what mmf_workspace_bytes counts, so that they can be
- * captured into a graph of the context's stream. Calls with no rows do nothing.
+ * Long scans and products of many rows use a workspace of the context (mmf_workspace_bytes counts it):
+ * the first such call allocates it, and fails with MMF_ERR_STATE under stream capture; nothing else
+ * is allocated, and it never moves or grows, so calls can be captured into graphs of the context's
+ * stream. Like calls, replays on one context must not overlap. Calls with no rows do nothing.
  *
  * Several sequences stand one after the other in the rows. lens (host, may be NULL) holds their
  * `seqs` lengths, which sum to rows and may be 0; with NULL all have rows / seqs rows, so that
@@ -184,8 +186,8 @@ int mmf_w4_release(mmf_ctx* ctx, int w4_id);
  * dtype MMF_F32, MMF_BF16, MMF_F16, or MMF_I8 with xscales [rows] (else NULL): the codes and scales
  * of mmf_add_rmsnorm_q8. out is of out_dtype (a float type). The weights enter every sum as the
  * integers they are, with no rounding, and the scale multiplies a group's fp32 sum (int8 x: its
- * exact integer sum). A row that holds an infinity or NaN has no finite output; finite inputs
- * should stay below 1e36. */
+ * exact integer sum). fp32 rows keep their digits for inputs between 1e-30 and 1e36. A row that holds
+ * an infinity or NaN has no finite output. */
 int mmf_w4_linear(mmf_ctx* ctx, int w4_id, int dtype, const void* x, const float* xscales, int out_dtype, void* out,
                   size_t rows, size_t ldx, size_t ldo);
 

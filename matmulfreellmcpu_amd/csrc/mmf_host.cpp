@@ -228,6 +228,7 @@ int guard(mmf_ctx* ctx, F&& f) {
     f();
     return MMF_OK;
   } catch (const Err& e) {
+    (void)hipGetLastError();  // reported here, and not by the next call's launch as well
     ctx->err = e.msg;
     return e.code;
   } catch (const std::bad_alloc&) {

@@ -24,6 +24,12 @@ __device__ __forceinline__ float softplus(float x) {
   return __builtin_fmaxf(x, 0.0f) + log1p_unit(exp2_fast(-1.44269504f * __builtin_fabsf(x)));
 }
 
+// A in powers of two; -infinity as the lowest finite value, so that a step of 0 has the decay 1 with it too.
+__device__ __forceinline__ float log2_decay(float A) {
+  A *= 1.44269504f;
+  return A < -3.4e38f ? -3.4e38f : A;
+}
+
 // A lane holds a channel's NS states in registers; a wave is 64 channels, and NW waves share a channel
 // with more states. Every lane needs the same B and C of a step: a block keeps kTile steps of them in LDS as
 // fp32 and reads them four at a time, all lanes one address; the next tile's are in flight meanwhile.
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(NW == 8 ? 512 : 256) void k_scan(ScanArgs a, SeqTab
   }
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    A[i] = n0 + i < N ? A[i] * 1.44269504f : 0.0f;
+    A[i] = n0 + i < N ? log2_decay(A[i]) : 0.0f;
     if (!hp || n0 + i >= N) h[i] = 0.0f;
   }
   float total = 0.0f;
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(256) void k_carry(ScanArgs a, SeqTab t, ScanWs ws) 
   if (i >= D * a.N || chunks < 2) return;
   const size_t first = t.len > 0 ? static_cast<size_t>(blockIdx.y) * t.tiles : t.tile[blockIdx.y];
   const size_t n = i / D, d = i - n * D;
-  const float A = a.A[d * a.N + n] * 1.44269504f;
+  const float A = log2_decay(a.A[d * a.N + n]);
   float* ends = ws.ends + first * a.N * D + i;
   const float* sums = ws.sums + first * D + d;
   const size_t step = a.N * D;

@@ -299,6 +299,72 @@ def test_w4_wide_range(eng):  # noqa: F811
     assert (again[keep] == got[keep]).all()
 
 
+@pytest.mark.parametrize("t", [F32, BF16, F16, I8])
+def test_w4_long_rows_and_many(eng, t):  # noqa: F811
+    """One row of many inputs; more rows than one launch or pass takes."""
+    rng = np.random.default_rng(40 + t)
+    run_w4(eng, rng, t, 1, 12000, 40, 128, zeros=True)
+    run_w4(eng, rng, t, 3, 9999, 17, 32, zeros=False, padx=5)
+    run_w4(eng, rng, t, 66000, 640 if t != F32 else 160, 64, 64, zeros=True, padx=1)
+
+
+def test_w4_small_values(eng):  # noqa: F811
+    """fp16 rows below fp16's normal range, and fp32 rows whose largest input is 1e6 times the others, by both kernels."""
+    rng = np.random.default_rng(41)
+    for rows, K, N in ((3, 256, 48), (40, 2048, 8192)):
+        w = W4(eng, rng, N, K, 64, True)
+        x = (rng.integers(-8, 9, (rows, K)) * 2.0 ** -24).astype(np.float16)
+        X, O = Rows(eng, x, F16), out_rows(eng, (rows, N), F32)
+        eng.w4_linear(w.id, X.ptr, O.ptr, rows, dtype=F16)
+        eng.sync()
+        want = x.astype(np.float64) @ w.w.T
+        assert np.linalg.norm(O.get() - want) <= 4e-6 * np.linalg.norm(want)
+        x = rng.standard_normal((rows, K)).astype(np.float32)
+        x[:, 5] *= 1e6
+        X = Rows(eng, x, F32)
+        eng.w4_linear(w.id, X.ptr, O.ptr, rows)
+        eng.sync()
+        # less the large input's own share, which is exact in fp32 to half a step of it: what is left of the
+        # others is off by a few steps of the sum's size at most
+        want = x.astype(np.float64) @ w.w.T
+        assert (np.abs(O.get() - want) <= 16 * U * (np.abs(x[:, 5:6] * w.w[:, 5]) + np.linalg.norm(want) / np.sqrt(want.size))).all()
+
+
+def test_offsets_beyond_32_bits(eng):  # noqa: F811
+    """Rows 2.4 GB apart: the same outputs as of neighbouring rows."""
+    rng = np.random.default_rng(42)
+    cols, ld = 100, 1_200_000_000
+    x = coded(rng.standard_normal((3, cols)), BF16)
+    near = Rows(eng, x, BF16)
+    p = C.c_void_p()
+    eng._chk(eng.lib.mmf_malloc(eng.h, C.byref(p), (2 * ld + cols) * 2))
+    try:
+        for r in range(3):
+            row = np.ascontiguousarray(x[r])
+            eng._chk(eng.lib.mmf_upload(eng.h, p.value + 2 * r * ld, row.ctypes.data_as(C.c_void_p), row.nbytes))
+        w, f = W4(eng, rng, 30, cols, 32, True), np.float32
+        nw, cw = Dev(eng, np.ones(cols, f)), Dev(eng, rng.standard_normal((cols, 4)).astype(f))
+        A = Dev(eng, -np.ones((cols, 16), f))
+        B = Rows(eng, coded(rng.standard_normal((3, 16)), BF16), BF16)
+        for what in ("norm", "w4", "conv", "scan"):
+            got = []
+            for ptr, step in ((near.ptr, cols), (p.value, ld)):
+                O, S = out_rows(eng, (3, cols if what != "w4" else 30), I8 if what == "norm" else BF16), out_rows(eng, (3, 1), F32)
+                if what == "norm":
+                    eng.add_rmsnorm_q8(O.ptr, S.ptr, ptr, nw.ptr, 3, cols, dtype=BF16, ldx=step)
+                elif what == "w4":
+                    eng.w4_linear(w.id, ptr, O.ptr, 3, dtype=BF16, out_dtype=BF16, ldx=step)
+                elif what == "conv":
+                    eng.short_conv(O.ptr, ptr, cw.ptr, 3, cols, 4, dtype=BF16, ldx=step)
+                else:
+                    eng.selective_scan(O.ptr, ptr, ptr, A.ptr, B.ptr, B.ptr, 3, cols, 16, dtype=BF16, ldu=step, lddt=step)
+                eng.sync()
+                got.append(O.get())
+            assert (got[0].view(np.uint8) == got[1].view(np.uint8)).all(), what
+    finally:
+        eng.lib.mmf_free(eng.h, p)
+
+
 def test_w4_refusals(eng):  # noqa: F811
     from matmulfreellmcpu_amd import MmfError
     rng = np.random.default_rng(1)
@@ -515,6 +581,7 @@ def test_scan_many_sequences(eng):  # noqa: F811
     run_scan(eng, rng, F32, [int(n) for n in rng.integers(0, 5, 600)], 40, 16)  # several tables of sequences
     run_scan(eng, rng, F32, [1] * 500, 70, 16)
     run_scan(eng, rng, F32, [12] * 300, 24, 4, seqs=300)
+    run_scan(eng, rng, F32, [700] + [1, 0, 2] * 90 + [900, 400], 64, 16)  # chunks in two of the tables
 
 
 def test_scan_strong_decay_and_large_steps(eng):  # noqa: F811
@@ -537,6 +604,28 @@ def test_scan_strong_decay_and_large_steps(eng):  # noqa: F811
     eng.sync()
     want = 100.0 * u[-1].astype(np.float64) * B[-1].astype(np.float64)[:, None]
     assert (np.abs(S.get()[0] - want) <= 2 * U * np.abs(want)).all()
+
+
+def test_scan_infinite_decay_and_nan(eng):  # noqa: F811
+    """A decay rate of -infinity keeps nothing of the state, at a sequence's ragged end too; a NaN stays in its channel."""
+    rng = np.random.default_rng(16)
+    T, D, N = 69, 70, 16  # a ragged group of steps
+    u, dt = rng.standard_normal((T, D)).astype(np.float32), np.full((T, D), 0.5, np.float32)
+    B, Cm = (rng.standard_normal((T, N)).astype(np.float32) for _ in range(2))
+    A = -np.ones((D, N), np.float32)
+    A[3], u[5, 40] = -np.inf, np.nan
+    d = {k: Dev(eng, v) for k, v in dict(u=u, dt=dt, B=B, C=Cm, A=A).items()}
+    S, O = Dev(eng, np.ones((1, N, D), np.float32)), Dev(eng, shape=(T, D))
+    eng.selective_scan(O.ptr, d["u"].ptr, d["dt"].ptr, d["A"].ptr, d["B"].ptr, d["C"].ptr, T, D, N, state=S.ptr,
+                       softplus=False)
+    eng.sync()
+    o, s = O.get(), S.get()[0]
+    want = 0.5 * u[:, 3].astype(np.float64)[:, None] * B
+    assert (np.abs(s[:, 3] - want[-1]) <= 2 * U * np.abs(want[-1])).all()
+    assert (np.abs(o[:, 3] - (want * Cm).sum(1)) <= 20 * U * np.abs(want * Cm).sum(1)).all()
+    others = np.arange(D) != 40
+    assert np.isfinite(o[:, others]).all() and np.isfinite(s[:, others]).all()
+    assert np.isfinite(o[:5, 40]).all() and np.isnan(o[5:, 40]).all() and np.isnan(s[:, 40]).all()
 
 
 def test_scan_carries_its_state(eng):  # noqa: F811
@@ -659,22 +748,83 @@ def test_layer_prompt_then_tokens(eng):  # noqa: F811
         near(L.d_conv.get(), L.conv_state, 5e-5, "carried inputs")
 
 
-def test_layer_in_a_graph(eng):  # noqa: F811
-    """The layer's step captured once and replayed between eager work: every replay equals the eager
-    calls on the same buffers bit for bit."""
+def hip_graphs():
     hip = C.CDLL("libamdhip64.so.7")
     for n in ("hipStreamBeginCapture", "hipStreamEndCapture", "hipGraphInstantiate", "hipGraphLaunch",
               "hipGraphExecDestroy", "hipGraphDestroy"):
         getattr(hip, n).restype = C.c_int
+    return hip
+
+
+def captured(hip, stream, work):
+    """(graph, executable graph) of work() on the stream."""
+    graph, ge = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    work()
+    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(ge), graph, None, None, C.c_size_t(0)) == 0
+    return graph, ge
+
+
+def test_workspace_in_graphs():
+    """The workspace's first use is refused under capture, and leaves the capture alone; two graphs that share
+    it, a long scan and a product of many rows, replay in turn with eager calls between them."""
+    from matmulfreellmcpu_amd import Engine, MmfError
+    e, hip = Engine(0), hip_graphs()
+    try:
+        rng, f = np.random.default_rng(50), np.float32
+        T, D, N, R, K, M = 700, 128, 16, 80, 1024, 8192
+        u, B, A = rng.standard_normal((T, D)).astype(f), rng.standard_normal((T, N)).astype(f), -np.ones((D, N), f)
+        d = {k: Dev(e, v) for k, v in dict(u=u, B=B, A=A, x=rng.standard_normal((R, K)).astype(f)).items()}
+        w = W4(e, rng, M, K, 128, True)
+        y, o = Dev(e, np.zeros((T, D), f)), Dev(e, np.zeros((R, M), f))
+        scan = lambda: e.selective_scan(y.ptr, d["u"].ptr, d["u"].ptr, d["A"].ptr, d["B"].ptr, d["B"].ptr, T, D, N)  # noqa: E731
+        product = lambda: e.w4_linear(w.id, d["x"].ptr, o.ptr, R)  # noqa: E731
+        assert e.workspace_bytes() == 0
+        stream = C.c_void_p(e.stream)
+
+        def refused():
+            for call in (scan, product):
+                with pytest.raises(MmfError, match="before the capture"):
+                    call()
+            e.w4_linear(w.id, d["x"].ptr, o.ptr, 2)  # needs none
+
+        graph, ge = captured(hip, stream, refused)
+        assert hip.hipGraphLaunch(ge, stream) == 0
+        e.sync()
+        assert hip.hipGraphExecDestroy(ge) == 0 and hip.hipGraphDestroy(graph) == 0
+        scan(), product()
+        e.sync()
+        want_y, want_o, size = y.get(), o.get(), e.workspace_bytes()
+        assert size > 0
+        graphs = [captured(hip, stream, scan), captured(hip, stream, product)]
+        for step in range(4):
+            for b in (y, o):
+                z = np.zeros(b.shape, f)
+                e._chk(e.lib.mmf_upload(e.h, b.ptr, z.ctypes.data_as(C.c_void_p), z.nbytes))
+            for _, ge in graphs[::1 if step % 2 else -1]:
+                assert hip.hipGraphLaunch(ge, stream) == 0
+            e.sync()
+            assert (y.get() == want_y).all() and (o.get() == want_o).all(), step
+            product(), scan()
+            e.sync()
+        assert e.workspace_bytes() == size
+        for g, ge in graphs:
+            assert hip.hipGraphExecDestroy(ge) == 0 and hip.hipGraphDestroy(g) == 0
+    finally:
+        e.close()
+
+
+def test_layer_in_a_graph(eng):  # noqa: F811
+    """The layer's step captured once and replayed between eager work: every replay equals the eager
+    calls on the same buffers bit for bit."""
+    hip = hip_graphs()
     rng = np.random.default_rng(22)
     L, E = (Layer(eng, np.random.default_rng(23), 128, 256, 16, 4, 8, 8) for _ in range(2))
     L.run(8), E.run(8)  # workspaces
     eng.sync()
-    stream, graph, ge = C.c_void_p(eng.stream), C.c_void_p(), C.c_void_p()
-    assert hip.hipStreamBeginCapture(stream, 0) == 0
-    L.run(8)
-    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
-    assert hip.hipGraphInstantiate(C.byref(ge), graph, None, None, C.c_size_t(0)) == 0
+    stream = C.c_void_p(eng.stream)
+    graph, ge = captured(hip, stream, lambda: L.run(8))
     for step in range(4):
         x = rng.standard_normal((8, 128)).astype(np.float32)
         for layer in (L, E):
