@@ -225,6 +225,14 @@ inline const char* check_seqs(const size_t* lens, size_t seqs, size_t rows) {
   return sum == rows ? nullptr : "the sequences' lengths do not sum to the rows";
 }
 
+// Whether sequences [first, first + n) have one row each: a token of each.
+inline bool one_row_each(const size_t* lens, size_t rows, size_t seqs, size_t first, int n) {
+  if (!lens) return rows == seqs;
+  for (int i = 0; i < n; ++i)
+    if (lens[first + i] != 1) return false;
+  return true;
+}
+
 // The table of sequences [first, first + n) with tiles of `step` rows; returns its rows, and tiles
 // in *ntiles.
 inline size_t fill_seqs(SeqTab& t, const size_t* lens, size_t rows, size_t seqs, size_t first, int n, int step,

@@ -320,6 +320,118 @@ hipError_t scan_launch(const ScanArgs& a, const SeqTab& t, const ScanWs& ws, siz
   return hipGetLastError();
 }
 
+// One row of each sequence: bound by reading and writing the states. A block is 64 channels, a wave NQ of their
+// states; it goes through `per` sequences with the decay rates in registers (their rows of N floats are
+// the dearest to read: 64 cache lines a load), the next sequence's state in flight. B and C are one
+// load a wave, handed out by v_readlane. The waves' sums meet in LDS.
+constexpr int kStepSeqs = 8;  // most sequences of a block
+template <int DT, int NQ>
+__global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, size_t seq0, size_t row0, int seqs, int per) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  __shared__ float sy[kStepSeqs][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int N = static_cast<int>(a.N), n0 = wave * NQ;
+  const size_t D = a.D;
+  const uint32_t dd = blockIdx.y * 64 + lane, d = min(dd, static_cast<uint32_t>(D) - 1);
+  const bool live = dd < D;
+  const int q0 = blockIdx.x * per, q1 = min(q0 + per, seqs);
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f;
+
+  struct Inputs {
+    T u, dt, bc;
+    float h[NQ];
+  };
+  auto fetch = [&](Inputs& in, int q) {
+    const size_t r = row0 + q;
+    in.u = (static_cast<const T*>(a.u) + r * a.ldu)[d];
+    in.dt = (static_cast<const T*>(a.dt) + r * a.lddt)[d];
+    const int n = min(n0 + (lane & (NQ - 1)), N - 1);
+    in.bc = lane & NQ ? (static_cast<const T*>(a.C) + r * a.ldc)[n] : (static_cast<const T*>(a.B) + r * a.ldb)[n];
+    if (a.state) {
+      const float* h = a.state + (seq0 + q) * N * D;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) in.h[i] = (h + min(n0 + i, N - 1) * D)[d];
+    }
+  };
+  Inputs now, next = {};
+  fetch(next, q0);
+  float A[NQ];
+  const float* Ap = a.A + static_cast<size_t>(d) * N;
+  if (NQ >= 4 && N % 4 == 0) {
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (int i = 0; i < NQ; i += 4) {
+      const f4u v = *reinterpret_cast<const f4u*>(Ap + min(n0 + i, N - 4));
+#pragma unroll
+      for (int k = 0; k < 4 && i + k < NQ; ++k) A[i + k] = log2_decay(v[k]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) A[i] = log2_decay(Ap[min(n0 + i, N - 1)]);
+  }
+  T uo[kStepSeqs / 4], zo[kStepSeqs / 4] = {};  // of the outputs that this wave writes
+#pragma unroll
+  for (int k = 0; k < kStepSeqs / 4; ++k) {
+    const size_t r = row0 + min(q0 + wave + 4 * k, q1 - 1);
+    uo[k] = (static_cast<const T*>(a.u) + r * a.ldu)[d];
+    if (a.z) zo[k] = (static_cast<const T*>(a.z) + r * a.ldz)[d];
+  }
+  for (int q = q0; q < q1; ++q) {
+    now = next;
+    if (q + 1 < q1) fetch(next, q + 1);
+    const float u = E::up(now.u), v = E::up(now.dt) + bias, step = a.softplus ? softplus(v) : v, su = step * u;
+    const float bc = E::up(now.bc);
+    float y = 0.0f;
+    float* h = a.state + (seq0 + q) * N * D;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      if (n0 + i >= N) break;
+      const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bc), i));
+      const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bc), NQ + i));
+      const float old = a.state ? now.h[i] : 0.0f;
+      const float x = __builtin_fmaf(exp2_fast(step * A[i]), old, su * b);
+      y = __builtin_fmaf(c, x, y);
+      if (a.state && live) (h + (n0 + i) * D)[d] = x;
+    }
+    sy[q - q0][wave][lane] = y;
+  }
+  __syncthreads();
+  if (!live) return;
+  const float skip = a.skip ? a.skip[d] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < kStepSeqs / 4; ++k) {
+    const int q = q0 + wave + 4 * k;
+    if (q >= q1) break;
+    float y = (sy[q - q0][0][lane] + sy[q - q0][1][lane]) + (sy[q - q0][2][lane] + sy[q - q0][3][lane]);
+    y = __builtin_fmaf(skip, E::up(uo[k]), y);
+    if (a.z) y *= silu_fast(E::up(zo[k]));
+    (static_cast<T*>(a.out) + (row0 + q) * a.ldo)[d] = E::down(y);
+  }
+}
+
+template <int DT>
+hipError_t step_launch(const ScanArgs& a, size_t seq0, size_t row0, int seqs, hipStream_t s) {
+  const unsigned cols = static_cast<unsigned>((a.D + 63) / 64);
+  // as many sequences a block as leave two blocks for each compute unit
+  int per = kStepSeqs;
+  while (per > 1 && static_cast<size_t>(cols) * ((seqs + per - 1) / per) < 512) per /= 2;
+  const dim3 grid((seqs + per - 1) / per, cols);
+  if (a.N <= 4)
+    k_scan_step<DT, 1><<<grid, 256, 0, s>>>(a, seq0, row0, seqs, per);
+  else if (a.N <= 8)
+    k_scan_step<DT, 2><<<grid, 256, 0, s>>>(a, seq0, row0, seqs, per);
+  else if (a.N <= 16)
+    k_scan_step<DT, 4><<<grid, 256, 0, s>>>(a, seq0, row0, seqs, per);
+  else if (a.N <= 32)
+    k_scan_step<DT, 8><<<grid, 256, 0, s>>>(a, seq0, row0, seqs, per);
+  else if (a.N <= 64)
+    k_scan_step<DT, 16><<<grid, 256, 0, s>>>(a, seq0, row0, seqs, per);
+  else
+    k_scan_step<DT, 32><<<grid, 256, 0, s>>>(a, seq0, row0, seqs, per);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_sel_scan(const ScanArgs& a, float* ws_mem, hipStream_t s) {
@@ -331,6 +443,12 @@ hipError_t launch_sel_scan(const ScanArgs& a, float* ws_mem, hipStream_t s) {
       SeqTab t;
       int tiles = 0;
       const int n = static_cast<int>(a.seqs - q < kSeqs ? a.seqs - q : kSeqs);
+      if (one_row_each(a.lens, a.rows, a.seqs, q, n)) {
+        const hipError_t e = step_launch<DT>(a, q, row0, n, s);
+        if (e != hipSuccess) return e;
+        row0 += n;
+        continue;
+      }
       const ScanPlan plan = scan_plan(a, q, n);
       const size_t rows = fill_seqs(t, a.lens, a.rows, a.seqs, q, n, plan.chunk, &tiles);
       if (tiles) {
