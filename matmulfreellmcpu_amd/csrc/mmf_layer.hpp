@@ -163,12 +163,18 @@ inline W4Plan w4_plan(int dtype, const W4Geom& g, int row_tiles) {
   while (p.ks > 1 && p.ks * one > room) p.ks /= 2;
   return p;
 }
-// Whether a call's rows are laid out: from 0.6 G products of fp32 rows on, 2.5 G of others (us, by the kernel
-// of few rows -> laid out: fp32 64 x 2048 x 2048 10 -> 17, 64 x 6912 x 2560 40 -> 27; bf16 128 x 6912 x 2560
-// 21 -> 25, 128 x 2048 x 11264 23 -> 19). Laying out and its launches cost 10 to 15 us.
-inline bool w4_lays(int dtype, const W4Geom& g, size_t rows) {
-  return rows > 16 && static_cast<double>(rows) * g.K * g.N > (dtype == kF32 ? 0.6e9 : 2.5e9);
+// The kernel of a call: of few rows, as they are or (fp32) laid out, or by tiles of many, which are laid out.
+// Lines by the products of a call, measured (us): fp32 rows laid out from 0.15 G on (16 x 2048 x 2048 6.6 as they
+// are, 6.8 laid out; 10 x 6912 x 2560 23 and 11; 128 x 2048 x 2048 20 and 11.5), by tiles from 1.6 G on (64 x 6912
+// x 2560 20 laid out, 25 by tiles; 128 x 2048 x 11264 38 and 26). Others by tiles from 2.5 G on (bf16 128 x 6912 x
+// 2560 21 by few rows' kernel, 25 by tiles; 128 x 2048 x 11264 23 and 18).
+enum W4Way { kRowsAsIs, kLaidRows, kTiles };
+inline W4Way w4_way(int dtype, const W4Geom& g, size_t rows) {
+  const double work = static_cast<double>(rows) * g.K * g.N;
+  if (rows > 16 && work > (dtype == kF32 ? 1.6e9 : 2.5e9)) return kTiles;
+  return dtype == kF32 && rows > 5 && work > 0.15e9 ? kLaidRows : kRowsAsIs;
 }
+inline bool w4_lays(int dtype, const W4Geom& g, size_t rows) { return w4_way(dtype, g, rows) != kRowsAsIs; }
 inline size_t w4_rows_most(int dtype, const W4Geom& g, size_t rows) {
   if (!w4_lays(dtype, g, rows)) return 65535 * 5;  // the grid's second dimension, in tiles of 5 rows or more
   size_t tiles = kLayerWsBytes / w4_lay_bytes(dtype, g, 1);

@@ -128,21 +128,127 @@ __device__ __forceinline__ u32x4 row_16B(const char* row, int k, int K, bool who
   return v;
 }
 
+// ---- rows laid out --------------------------------------------------------------------------------
+// Many rows, and fp32 rows from a line on, are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
+// FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
+// l % 16; zeros behind the last row and input. Beside them stands a number for each row and scale's inputs,
+// [tile][chunk][S][16]:
+//   fp32 rows are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of fp32, with 2^k
+//     bringing the largest of a scale's inputs below 2^15; the number is 2^-k (NaN where an input is none);
+//   fp16 rows are as they are, and it is 1;
+//   bf16 and int8 rows are as they are, and it is the sum of the inputs.
+// fp16 operands take the codes with the zero point off: 128 + q and 128 + z are exact, and so is q - z.
+template <int DT> constexpr int kParts = DT == kF32 ? 2 : 1;
+template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
+template <int DT> constexpr int kOperand = DT == kF32 ? kF16 : DT;
+
+// One block a tile and chunk; 16 lanes a row, 8 inputs a thread.
+template <int DT, int STEP>
+__global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags, uint32_t* sums) {
+  constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP;
+  const int u = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int c = blockIdx.x, k = c * 128 + 8 * u;
+  const size_t rt = blockIdx.y, row = rt * 16 + r;
+  const bool in = row < a.rows;
+  // the unit's place: word j of lane group q
+  const int j = STEP == 32 ? u >> 2 : (u >> 3) * 2 + (u & 1), q = STEP == 32 ? u & 3 : (u & 7) >> 1;
+  const int h = j >> 1;
+  char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
+  uint32_t total;
+  constexpr int U = STEP / 8;  // neighbouring threads that share a scale
+  if constexpr (DT == kF32) {
+    float v[8];
+    uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN are the largest
+    const float* x = static_cast<const float*>(a.x) + row * a.ldx + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = in && k + i < g.K ? x[i] : 0.0f;
+      top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+    }
+#pragma unroll
+    for (int n = 1; n < U; n *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), n)));
+    const uint32_t e = top >> 23, up = min(268u - e, 253u);  // 2^k with k = 14 - exponent, at most 2^126
+    const float f = __builtin_bit_cast(float, up << 23);
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h[2], l[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float y = v[2 * i + m] * f;
+        const _Float16 p = static_cast<_Float16>(y);
+        h[m] = __builtin_bit_cast(uint16_t, p);
+        l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
+      }
+      hi[i] = h[0] | h[1] << 16;
+      lo[i] = l[0] | l[1] << 16;
+    }
+    *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = hi;
+    *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
+    if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = e == 255 ? 0x7FC00000u : (254 - up) << 23;
+    return;
+  } else if constexpr (DT == kI8) {
+    uint32_t x0 = 0, x1 = 0;
+    int sum = 0;
+    const int8_t* x = static_cast<const int8_t*>(a.x) + row * a.ldx + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = in && k + i < g.K ? x[i] : 0;
+      sum += e;
+      (i < 4 ? x0 : x1) |= static_cast<uint32_t>(e & 255) << (8 * (i & 3));
+    }
+    uint32_t lo, hi;
+    i8_operand(x0, x1, lo, hi);
+    uint32_t* o = reinterpret_cast<uint32_t*>(to + 8 * (j & 1));
+    o[0] = lo;
+    o[1] = hi;
+    total = static_cast<uint32_t>(sum);
+  } else {
+    u32x4 o = {0, 0, 0, 0};
+    float sum = 0.0f;
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx + k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t e = in && k + i < g.K ? x[i] : static_cast<uint16_t>(0);
+      sum += Elem<DT>::up(e);
+      o[i / 2] |= static_cast<uint32_t>(e) << (16 * (i & 1));
+    }
+    *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = o;
+    total = __builtin_bit_cast(uint32_t, sum);
+    if (DT == kF16) {
+      if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = 0x3F800000u;
+      return;
+    }
+  }
+#pragma unroll
+  for (int n = 1; n < U; n *= 2) {
+    const uint32_t o = __shfl_xor(static_cast<int>(total), n);
+    if constexpr (DT == kI8)
+      total += o;
+    else
+      total = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, total) + __builtin_bit_cast(float, o));
+  }
+  if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = total;
+}
+
+// ---- few rows -------------------------------------------------------------------------------------
 // Few rows: one pass over the weights, bound by reading them. A block's waves split the chunks of NT
 // tiles of 16 outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix
 // operand's place and multiplies it with CT column tiles. A column is a row, or for fp32 rows one of a row's
 // three bf16 parts (hi + mid + lo = x exactly), 5 rows a tile: a wave cuts its chunk's rows into parts
-// once, in LDS of its own. The waves' sums meet in LDS in one fixed order.
-template <int DT> constexpr int kTileRows = DT == kF32 ? 5 : 16;
+// once, in LDS of its own; or (LAID) a column is a row, of laid out parts. The waves' sums meet in LDS in one
+// fixed order.
+template <int DT, bool LAID> constexpr int kTileRows = DT == kF32 && !LAID ? 5 : 16;
 constexpr int kPartStride = 272;  // bytes of a column's 128 parts in LDS, 16 apart in banks
-template <int DT, int CT> constexpr int kPartBytes = DT == kF32 ? CT * 15 * kPartStride : 0;
+template <int DT, int CT, bool LAID> constexpr int kPartBytes = DT == kF32 && !LAID ? CT * 15 * kPartStride : 0;
 
-template <int DT, int STEP, int NT, int CT>
-__global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4Args a, W4Geom g, const uint32_t* codes,
-                                                                      const uint32_t* scales) {
-  using M = Mat<DT>;
+template <int DT, int STEP, int NT, int CT, bool LAID>
+__global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4_rows(
+    W4Args a, W4Geom g, const uint32_t* codes, const uint32_t* scales, const char* frags, const uint32_t* sums, int row_tiles) {
+  static_assert(!LAID || DT == kF32, "other rows are read as they are");
+  using M = Mat<LAID ? kF16 : DT>;
   using Acc = typename M::Acc;
-  constexpr int S = 128 / STEP, R = kTileRows<DT>;
+  constexpr int S = 128 / STEP, R = kTileRows<DT, LAID>;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int col = lane & 15, q = lane >> 4;
@@ -150,7 +256,7 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
   const int tile0 = blockIdx.x * NT;
   const size_t es = DT == kF32 ? 4 : DT == kI8 ? 1 : 2;
   const char* x0 = static_cast<const char*>(a.x) + static_cast<size_t>(row0) * a.ldx * es;
-  char* part = lds + wave * kPartBytes<DT, CT>;
+  char* part = lds + wave * kPartBytes<DT, CT, LAID>;
 
   const char* xr[CT];  // this lane's row of each column tile (a row past the end repeats the last one)
 #pragma unroll
@@ -162,6 +268,20 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
     const size_t tile = min(tile0 + n, g.nt - 1);
     cw[n] = codes + tile * g.nc * 256 + lane * 4;
     sw[n] = scales + tile * g.ns * 16 + q * 4;
+  }
+
+  // LAID: this lane's place in each tile's fragments and numbers, and its operand's outputs' scales
+  const char* fr[CT];
+  const uint32_t *num[CT], *zw[NT];
+  if constexpr (LAID) {
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const size_t rt = min(static_cast<int>(blockIdx.y) * CT + t, row_tiles - 1);
+      fr[t] = frags + rt * g.nc * 8192 + lane * 16;
+      num[t] = sums + rt * g.ns * 16 + col;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) zw[n] = sw[n] - q * 4 + col;
   }
 
   f32x4 acc[NT][CT];
@@ -191,8 +311,25 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
       for (int s = 0; s < S; ++s) csz[n][s] = sz[n][s];
     }
     // the rows' operands of this chunk
-    u32x4 b[CT][4];
-    if constexpr (DT == kF32) {
+    constexpr int P = LAID ? 2 : 1;
+    u32x4 b[CT][4 * P];
+    uint32_t x[CT][S], z[NT][S];
+    if constexpr (LAID) {  // [half][part][word of the half]
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[t][j] = *reinterpret_cast<const u32x4*>(fr[t] + (static_cast<size_t>(c) * 8 + j) * 1024);
+#pragma unroll
+        for (int s = 0; s < S; ++s) x[t][s] = num[t][(static_cast<size_t>(c) * S + s) * 16];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const uint32_t v = zw[n][(static_cast<size_t>(c) * S + s) * 16] >> 16;
+          z[n][s] = M::bits + (v << 3 | v << 19);
+        }
+    } else if constexpr (DT == kF32) {
       for (int r = 0; r < rows; ++r) {  // two neighbours a lane, three parts each
         const float* p = reinterpret_cast<const float*>(x0) + r * a.ldx + c * 128 + 2 * lane;
         const int k = c * 128 + 2 * lane;
@@ -306,9 +443,19 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
           const int j = s * (4 / S) + jj;
           u32x4 aw[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) aw[n] = w4_operand<DT>(cur[n][j]);
+          for (int n = 0; n < NT; ++n) {
+            aw[n] = w4_operand<LAID ? kF16 : DT>(cur[n][j]);
+            if constexpr (LAID) aw[n] = less(aw[n], z[n][s]);
+          }
 #pragma unroll
           for (int t = 0; t < CT; ++t) {
+            if constexpr (LAID) {
+#pragma unroll
+              for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) d[n][t] = M::mul(aw[n], b[t][(j >> 1) * 4 + p * 2 + (j & 1)], d[n][t]);
+              continue;
+            }
             sum[t] = M::mul(u32x4{one, one, one, one}, b[t][j], sum[t]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) d[n][t] = M::mul(aw[n], b[t][j], d[n][t]);
@@ -326,9 +473,11 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
             if constexpr (DT == kI8) {
               acc[n][t][i] = __builtin_fmaf(sc, static_cast<float>(d[n][t][i] - __mul24(static_cast<int>(v >> 16), sum[t][i])),
                                             acc[n][t][i]);
+            } else if constexpr (LAID) {
+              acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(float, x[t][s]), acc[n][t][i]);
             } else {
-              const float z = static_cast<float>(v >> 16) + M::base;
-              acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, sum[t][i], d[n][t][i]), acc[n][t][i]);
+              const float off = static_cast<float>(v >> 16) + M::base;
+              acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-off, sum[t][i], d[n][t][i]), acc[n][t][i]);
             }
           }
         }
@@ -343,15 +492,15 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
 #pragma unroll
     for (int t = 0; t < CT; ++t) red[((wave * NT + n) * CT + t) * 64 + lane] = acc[n][t];
   __syncthreads();
-  const float* sums = reinterpret_cast<const float*>(lds);
+  const float* held = reinterpret_cast<const float*>(lds);
   for (int i = threadIdx.x; i < NT * 16 * rows; i += blockDim.x) {
     const int n = i % (NT * 16), r = i / (NT * 16), t = r / R;
     if (tile0 * 16 + n >= g.N) continue;
     const int at = (((n / 16) * CT + t) * 64 + (n % 16 / 4) * 16) * 4 + n % 4;
     float v = 0.0f;
     for (int wv = 0; wv < waves; ++wv) {
-      const float* p = sums + wv * (NT * CT * 256) + at;
-      if constexpr (DT == kF32) {
+      const float* p = held + wv * (NT * CT * 256) + at;
+      if constexpr (DT == kF32 && !LAID) {
         const int c0 = r % 5 * 3;  // the small parts first
         v += (p[(c0 + 2) * 4] + p[(c0 + 1) * 4]) + p[c0 * 4];
       } else {
@@ -363,14 +512,15 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 ? 1024 : 512) void k_w4_rows(W4A
   }
 }
 
-template <int DT, int STEP, int NT, int CT>
+template <int DT, int STEP, int NT, int CT, bool LAID = false>
 hipError_t rows_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, int waves,
-                       hipStream_t s) {
-  const size_t part = static_cast<size_t>(waves) * kPartBytes<DT, CT>, red = static_cast<size_t>(waves) * NT * CT * 1024;
+                       hipStream_t s, const char* frags = nullptr, const uint32_t* sums = nullptr) {
+  const size_t part = static_cast<size_t>(waves) * kPartBytes<DT, CT, LAID>, red = static_cast<size_t>(waves) * NT * CT * 1024;
   const size_t lds = part > red ? part : red;  // at most 64 KB: 16 waves of one column tile, 8 of two
-  auto* k = k_w4_rows<DT, STEP, NT, CT>;
-  const unsigned per = CT * kTileRows<DT>;
-  k<<<dim3((g.nt + NT - 1) / NT, static_cast<unsigned>((a.rows + per - 1) / per)), waves * 64, lds, s>>>(a, g, codes, scales);
+  const unsigned per = CT * kTileRows<DT, LAID>;
+  k_w4_rows<DT, STEP, NT, CT, LAID>
+      <<<dim3((g.nt + NT - 1) / NT, static_cast<unsigned>((a.rows + per - 1) / per)), waves * 64, lds, s>>>(
+          a, g, codes, scales, frags, sums, static_cast<int>((a.rows + 15) / 16));
   return hipGetLastError();
 }
 
@@ -380,11 +530,11 @@ hipError_t rows_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
 // outputs instead where there are enough of these (bf16 16 x 2048 x 11264 8.8 -> 6.9).
 // Two column tiles: the rows' operands are most of what is read, so a wave takes as many tiles of outputs as leave
 // the chip full, and fewer waves share a block when there are more of them (bf16, one tile -> chosen: 64 x 6912 x
-// 2560 28.1 -> 17.7, 128 x 6912 x 2560 41 -> 21, 128 x 2048 x 11264 45 -> 23). fp32 rows, whose parts are
-// made anew for each column tile, gain less (64 x 2048 x 11264 64 -> 44) and take two at most.
+// 2560 28.1 -> 17.7, 128 x 6912 x 2560 41 -> 21, 128 x 2048 x 11264 45 -> 23). fp32 rows, whose parts are made
+// anew for each column tile, take two at most.
 template <int DT, int STEP>
 hipError_t rows_pick(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s) {
-  constexpr size_t R = kTileRows<DT>;
+  constexpr size_t R = kTileRows<DT, false>;
   constexpr bool F = DT == kF32;
   if (a.rows <= R) {
     if constexpr (!F) {
@@ -405,6 +555,22 @@ hipError_t rows_pick(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
   return rows_launch<DT, STEP, 2, 2>(a, g, codes, scales, waves, s);
 }
 
+// fp32 rows laid out, by the kernel of few rows.
+template <int STEP>
+hipError_t laid_rows(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws, hipStream_t s) {
+  const int rt = static_cast<int>((a.rows + 15) / 16);
+  uint32_t* sums = reinterpret_cast<uint32_t*>(ws + rt * w4_frag_bytes(kF32, g));
+  k_w4_lay<kF32, STEP><<<dim3(g.nc, rt), 256, 0, s>>>(a, g, ws, sums);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const size_t units = static_cast<size_t>(g.nt) * ((rt + 1) / 2);
+  const int waves = g.nc < 8 ? g.nc : 8;
+  if (rt == 1) return units <= 256 ? rows_launch<kF32, STEP, 1, 1, true>(a, g, codes, scales, waves, s, ws, sums)
+                                   : rows_launch<kF32, STEP, 2, 1, true>(a, g, codes, scales, waves, s, ws, sums);
+  return units <= 256 ? rows_launch<kF32, STEP, 1, 2, true>(a, g, codes, scales, waves, s, ws, sums)
+                      : rows_launch<kF32, STEP, 2, 2, true>(a, g, codes, scales, waves, s, ws, sums);
+}
+
 template <int DT>
 hipError_t rows_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s) {
   return g.step == 32 ? rows_pick<DT, 32>(a, g, codes, scales, s)
@@ -412,108 +578,6 @@ hipError_t rows_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
 }
 
 // ---- many rows ------------------------------------------------------------------------------------
-// The rows are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
-// FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
-// l % 16; zeros behind the last row and input. Beside them stands a number for each row and scale's inputs,
-// [tile][chunk][S][16]:
-//   fp32 rows are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of fp32, with 2^k
-//     bringing the largest of a scale's inputs below 2^15; the number is 2^-k (NaN where an input is none);
-//   fp16 rows are as they are, and it is 1;
-//   bf16 and int8 rows are as they are, and it is the sum of the inputs.
-// fp16 operands take the codes with the zero point off: 128 + q and 128 + z are exact, and so is q - z.
-template <int DT> constexpr int kParts = DT == kF32 ? 2 : 1;
-template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
-template <int DT> constexpr int kOperand = DT == kF32 ? kF16 : DT;
-
-// One block a tile and chunk; 16 lanes a row, 8 inputs a thread.
-template <int DT, int STEP>
-__global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags, uint32_t* sums) {
-  constexpr int P = kParts<DT>, FR = kFrags<DT>, S = 128 / STEP;
-  const int u = threadIdx.x & 15, r = threadIdx.x >> 4;
-  const int c = blockIdx.x, k = c * 128 + 8 * u;
-  const size_t rt = blockIdx.y, row = rt * 16 + r;
-  const bool in = row < a.rows;
-  // the unit's place: word j of lane group q
-  const int j = STEP == 32 ? u >> 2 : (u >> 3) * 2 + (u & 1), q = STEP == 32 ? u & 3 : (u & 7) >> 1;
-  const int h = j >> 1;
-  char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
-  uint32_t total;
-  constexpr int U = STEP / 8;  // neighbouring threads that share a scale
-  if constexpr (DT == kF32) {
-    float v[8];
-    uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN are the largest
-    const float* x = static_cast<const float*>(a.x) + row * a.ldx + k;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = in && k + i < g.K ? x[i] : 0.0f;
-      top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
-    }
-#pragma unroll
-    for (int n = 1; n < U; n *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), n)));
-    const uint32_t e = top >> 23, up = min(268u - e, 253u);  // 2^k with k = 14 - exponent, at most 2^126
-    const float f = __builtin_bit_cast(float, up << 23);
-    u32x4 hi, lo;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t h[2], l[2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const float y = v[2 * i + m] * f;
-        const _Float16 p = static_cast<_Float16>(y);
-        h[m] = __builtin_bit_cast(uint16_t, p);
-        l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
-      }
-      hi[i] = h[0] | h[1] << 16;
-      lo[i] = l[0] | l[1] << 16;
-    }
-    *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = hi;
-    *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
-    if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = e == 255 ? 0x7FC00000u : (254 - up) << 23;
-    return;
-  } else if constexpr (DT == kI8) {
-    uint32_t x0 = 0, x1 = 0;
-    int sum = 0;
-    const int8_t* x = static_cast<const int8_t*>(a.x) + row * a.ldx + k;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = in && k + i < g.K ? x[i] : 0;
-      sum += e;
-      (i < 4 ? x0 : x1) |= static_cast<uint32_t>(e & 255) << (8 * (i & 3));
-    }
-    uint32_t lo, hi;
-    i8_operand(x0, x1, lo, hi);
-    uint32_t* o = reinterpret_cast<uint32_t*>(to + 8 * (j & 1));
-    o[0] = lo;
-    o[1] = hi;
-    total = static_cast<uint32_t>(sum);
-  } else {
-    u32x4 o = {0, 0, 0, 0};
-    float sum = 0.0f;
-    const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx + k;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t e = in && k + i < g.K ? x[i] : static_cast<uint16_t>(0);
-      sum += Elem<DT>::up(e);
-      o[i / 2] |= static_cast<uint32_t>(e) << (16 * (i & 1));
-    }
-    *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = o;
-    total = __builtin_bit_cast(uint32_t, sum);
-    if (DT == kF16) {
-      if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = 0x3F800000u;
-      return;
-    }
-  }
-#pragma unroll
-  for (int n = 1; n < U; n *= 2) {
-    const uint32_t o = __shfl_xor(static_cast<int>(total), n);
-    if constexpr (DT == kI8)
-      total += o;
-    else
-      total = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, total) + __builtin_bit_cast(float, o));
-  }
-  if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = total;
-}
-
 // A block of up to four groups of WN waves, a wave 64 outputs by TT tiles of rows; the groups, of all blocks of a
 // tile, take chunks in turn, and a block's sums meet in LDS in a fixed order. The rows' fragments, the scales and the sums go through
 // LDS, shared by a group's waves, a stage (a chunk, or with three parts half a chunk) ahead through
@@ -868,7 +932,14 @@ hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
     if (a.xscales) b.xscales = a.xscales + r;
     const hipError_t e = by_type(a.dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      return w4_lays(a.dtype, g, a.rows) ? gemm_step<DT>(b, g, codes, scales, ws, s) : rows_step<DT>(b, g, codes, scales, s);
+      const W4Way way = w4_way(a.dtype, g, a.rows);
+      if (way == kTiles) return gemm_step<DT>(b, g, codes, scales, ws, s);
+      if constexpr (DT == kF32) {
+        if (way == kLaidRows)
+          return g.step == 32   ? laid_rows<32>(b, g, codes, scales, ws, s)
+                 : g.step == 64 ? laid_rows<64>(b, g, codes, scales, ws, s) : laid_rows<128>(b, g, codes, scales, ws, s);
+      }
+      return rows_step<DT>(b, g, codes, scales, s);
     });
     if (e != hipSuccess) return e;
   }

@@ -26,7 +26,8 @@ def coded(a, t):
     """float array -> the type's storage (to nearest, ties to even)."""
     a = np.asarray(a)
     if t != BF16:
-        return a.astype(STORE[t])
+        with np.errstate(over="ignore"):  # fp16 beyond 65504: infinity
+            return a.astype(STORE[t])
     b = np.ascontiguousarray(a, np.float32).view(np.uint32)
     up = ((b + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint16)
     return np.where(np.isnan(a), np.uint16(0x7FC0), up)
@@ -236,6 +237,8 @@ def run_w4(eng, rng, t, rows, K, N, group, zeros, out_t=F32, exact=True, padx=0,
         else:  # exact integers per group, then an fp32 sum over the groups: G + 2 roundings
             G = -(-K // group) if group else 1
             mag = np.abs(xv) @ np.abs(w.w.T) * xs
+            rounded = value(coded(want.astype(np.float32), out_t), out_t)
+            want = np.where(np.isinf(rounded), rounded, want)  # beyond fp16's largest value, 65504
             close(got, want, U * (-(-K // 32) + 3) * mag, out_t, "w4 int8")
     else:
         # each of the sums' roundings is half a step of a partial sum, and these stay below the sums of
@@ -269,12 +272,32 @@ def test_w4_many_rows(eng, t):  # noqa: F811
         run_w4(eng, rng, t, rows, K, N, group, zeros=True, padx=3, pado=1)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128, 0])
+def test_w4_laid_rows(eng, group):  # noqa: F811
+    """fp32 rows that are laid out for the kernel of few rows: one and two column tiles, one and two output tiles."""
+    rng = np.random.default_rng(60 + group)
+    for i, (rows, K, N) in enumerate(((7, 5000, 4400), (16, 9001, 1200), (17, 2049, 4500), (50, 1031, 3000))):
+        run_w4(eng, rng, F32, rows, K, N, group, zeros=i % 2 == 0, padx=i, offx=1, pado=3, out_t=FLOATS[i % 3])
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16, I8])
+@pytest.mark.parametrize("i", [0, 1, 2])
+def test_w4_tiles(eng, t, i):  # noqa: F811
+    """Products of many rows: inputs split over blocks, over a block's waves, and not at all."""
+    rng = np.random.default_rng(70 + t)
+    rows, K, N = ((80, 4100, 8001), (131, 1301, 16300), (701, 600, 6500))[i]
+    for k in (0, 1):
+        group = (32, 64, 128, 0)[(t + i + 2 * k) % 4]
+        run_w4(eng, rng, t, rows, K, N, group, zeros=k == 0, padx=k, pado=1 - k, out_t=F32 if k else FLOATS[(t + i) % 3])
+
+
 @pytest.mark.parametrize("t", [F32, BF16, F16, I8])
 @pytest.mark.parametrize("out_t", FLOATS)
 def test_w4_rounding(eng, t, out_t):  # noqa: F811
     """Real inputs: the fp32 rows keep all their digits."""
     rng = np.random.default_rng(17 + t + out_t)
-    for rows, K, N in ((1, 2048, 130), (4, 6912, 48), (24, 1031, 70), (70, 512, 100), (300, 640, 160)):
+    for rows, K, N in ((1, 2048, 130), (4, 6912, 48), (24, 1031, 70), (70, 512, 100), (300, 640, 160), (90, 2048, 1100),
+                       (130, 1600, 13000)):
         run_w4(eng, rng, t, rows, K, N, group=[32, 64, 128][rows % 3], zeros=rows != 4, out_t=out_t, exact=False)
 
 
