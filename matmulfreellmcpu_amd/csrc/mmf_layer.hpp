@@ -140,27 +140,41 @@ constexpr int kW4TileRows = 64;  // of a wave
 struct W4Plan {
   int wn, bk, ks;
 };
-// A block multiplies 64 wn outputs by 64 rows. Blocks of 256 outputs and four waves, two on a compute unit,
-// where there are more than 256 of them (2048 x 2048 x 11264 fp32, us: 200, and as half as many blocks of eight
-// waves 215; 224 with the inputs split over two groups of waves). Down to 130, two groups over the inputs (256
-// x 2048 x 11264 43, by smaller tiles 55). Below, tiles of 128 outputs and four groups, and the inputs over as
-// many blocks as the chip takes at once: 64 x 6912 x 2560 78 -> 27 by 8, 128 x 6912 x 2560 81 -> 36 by 4.
-inline W4Plan w4_pick(const W4Geom& g, int row_tiles) {
-  auto blocks = [&](int wn) {
-    return static_cast<size_t>((g.nt + wn * 4 - 1) / (wn * 4)) * ((row_tiles + kW4TileRows / 16 - 1) / (kW4TileRows / 16));
-  };
-  if (blocks(4) > 256) return {4, 1, 1};
-  if (blocks(4) >= 130) return {4, 2, 1};
-  W4Plan p{2, 4, 1};
-  while (blocks(2) * p.ks * 2 <= 256 && p.ks * 8 <= g.nc) p.ks *= 2;
-  return p;
+// The plan of the least time by this count: a chunk of inputs of 64 x 64 outputs takes a SIMD `unit` us (fp32 2.2,
+// 16-bit 1.25, int8 1.05 with a scale for 128 inputs; more scalings with more scales), 1.3 times that where a compute unit
+// has fewer than 8 waves to overlap, and up to 1.3 times where fewer outputs share the rows' operands; the
+// fullest compute unit counts. Split inputs cost a launch and the partial sums, written and read at 4 TB/s.
+// Measured (us): fp32 2048 x 6912 x 2560 277 as {4, 1, 1} and 220 as {4, 1, 3}; 512 x 6912 x 2560 147 and 75 as
+// {2, 4, 1}; bf16 2048 x 2048 x 2048 39 and 33 as {4, 2, 1}; fp32 2048 x 2048 x 11264 191, as {4, 2, 1} 215.
+inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
+  const double unit = (dtype == kF32 ? 2.2 : dtype == kI8 ? 1.05 : 1.25) * (g.step == 32 ? 1.8 : g.step == 64 ? 1.2 : 1.0);
+  const int rows = (row_tiles + kW4TileRows / 16 - 1) / (kW4TileRows / 16);
+  const double sums = row_tiles * 16.0 * g.nt * 16.0 * 4 * 2 / 4e6;  // us of one split's
+  const struct {
+    int wn, bk;
+    double share;
+  } forms[] = {{4, 1, 1.0}, {4, 2, 1.0}, {2, 2, 1.15}, {2, 4, 1.3}};
+  W4Plan best{4, 1, 1};
+  double least = 0;
+  for (const auto& f : forms)
+    for (int ks = 1; ks <= 8 && (ks == 1 || ks * f.bk <= g.nc); ++ks) {
+      const double blocks = static_cast<double>((g.nt + f.wn * 4 - 1) / (f.wn * 4)) * rows * ks;
+      const double most = static_cast<double>(static_cast<size_t>((blocks + 255) / 256));  // blocks of a compute unit
+      const int chunks = (g.nc + f.bk * ks - 1) / (f.bk * ks), waves = f.wn * f.bk;
+      const double t = most * chunks * (waves / 4.0) * unit * f.share * (most * waves < 8 ? 1.3 : 1.0) + (ks > 1 ? 4 + ks * sums : 0);
+      if (least == 0 || t < least) {
+        least = t;
+        best = {f.wn, f.bk, ks};
+      }
+    }
+  return best;
 }
 // The same, with no more splits than the workspace holds the sums of beside the laid out rows.
 inline W4Plan w4_plan(int dtype, const W4Geom& g, int row_tiles) {
-  W4Plan p = w4_pick(g, row_tiles);
+  W4Plan p = w4_pick(dtype, g, row_tiles);
   const size_t one = static_cast<size_t>(row_tiles) * g.nt * 1024;  // bytes of one split's sums
   const size_t room = kLayerWsBytes - w4_lay_bytes(dtype, g, row_tiles);
-  while (p.ks > 1 && p.ks * one > room) p.ks /= 2;
+  while (p.ks > 1 && p.ks * one > room) --p.ks;
   return p;
 }
 // The kernel of a call: of few rows, as they are or (fp32) laid out, or by tiles of many, which are laid out.
