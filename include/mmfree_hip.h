@@ -186,8 +186,10 @@ int mmf_w4_release(mmf_ctx* ctx, int w4_id);
  * dtype MMF_F32, MMF_BF16, MMF_F16, or MMF_I8 with xscales [rows] (else NULL): the codes and scales
  * of mmf_add_rmsnorm_q8. out is of out_dtype (a float type). The weights enter every sum as the
  * integers they are, with no rounding, and the scale multiplies a group's fp32 sum (int8 x: its
- * exact integer sum). fp32 rows keep their digits for inputs between 1e-30 and 1e36. A row that holds
- * an infinity or NaN has no finite output. */
+ * exact integer sum). An output's error is the rounding of fp32 sums of 31 |scale x| over all inputs of the
+ * row, also of those that weights of 0 meet: an input 1e7 times the others leaves few of their digits. fp32
+ * rows keep their digits for inputs between 1e-30 and 1e36. A row that holds an infinity or NaN has no
+ * finite output. */
 int mmf_w4_linear(mmf_ctx* ctx, int w4_id, int dtype, const void* x, const float* xscales, int out_dtype, void* out,
                   size_t rows, size_t ldx, size_t ldo);
 
