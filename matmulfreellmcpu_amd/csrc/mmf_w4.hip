@@ -113,6 +113,9 @@ __device__ __forceinline__ u32x4 less(u32x4 a, uint32_t b) {
   return r;
 }
 
+// Four bytes: a code less its zero point, with b = 0x80 - z in each: their sum is at most 0x8F, so nothing carries.
+__device__ __forceinline__ uint32_t less_bytes(uint32_t a, uint32_t b) { return (a + b) ^ 0x80808080u; }
+
 // 16 bytes of a row of 16-bit elements (8) or bytes (16) from element k, zeros behind K.
 template <int DT>
 __device__ __forceinline__ u32x4 row_16B(const char* row, int k, int K, bool whole) {
@@ -131,13 +134,13 @@ __device__ __forceinline__ u32x4 row_16B(const char* row, int k, int K, bool who
 // ---- rows laid out --------------------------------------------------------------------------------
 // Many rows, and fp32 rows from a line on, are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
 // FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
-// l % 16; zeros behind the last row and input. Beside them stands a number for each row and scale's inputs,
-// [tile][chunk][S][16]:
+// l % 16; zeros behind the last row and input. Beside them stands, for fp32 and bf16, a number for each row and
+// scale's inputs, [tile][chunk][S][16]:
 //   fp32 rows are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of fp32, with 2^k
 //     bringing the largest of a scale's inputs below 2^15; the number is 2^-k (NaN where an input is none);
-//   fp16 rows are as they are, and it is 1;
-//   bf16 and int8 rows are as they are, and it is the sum of the inputs.
-// fp16 operands take the codes with the zero point off: 128 + q and 128 + z are exact, and so is q - z.
+//   bf16 rows are as they are, and it is the sum of the inputs;
+//   fp16 and int8 rows are as they are.
+// fp16 and int8 operands take the codes with the zero point off: 128 + q and 128 + z are exact, and so is q - z.
 template <int DT> constexpr int kParts = DT == kF32 ? 2 : 1;
 template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
 template <int DT> constexpr int kOperand = DT == kF32 ? kF16 : DT;
@@ -154,7 +157,6 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
   const int j = STEP == 32 ? u >> 2 : (u >> 3) * 2 + (u & 1), q = STEP == 32 ? u & 3 : (u & 7) >> 1;
   const int h = j >> 1;
   char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
-  uint32_t total;
   constexpr int U = STEP / 8;  // neighbouring threads that share a scale
   if constexpr (DT == kF32) {
     float v[8];
@@ -186,15 +188,12 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
     *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = hi;
     *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
     if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = e == 255 ? 0x7FC00000u : (254 - up) << 23;
-    return;
   } else if constexpr (DT == kI8) {
     uint32_t x0 = 0, x1 = 0;
-    int sum = 0;
     const int8_t* x = static_cast<const int8_t*>(a.x) + row * a.ldx + k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = in && k + i < g.K ? x[i] : 0;
-      sum += e;
       (i < 4 ? x0 : x1) |= static_cast<uint32_t>(e & 255) << (8 * (i & 3));
     }
     uint32_t lo, hi;
@@ -202,7 +201,6 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
     uint32_t* o = reinterpret_cast<uint32_t*>(to + 8 * (j & 1));
     o[0] = lo;
     o[1] = hi;
-    total = static_cast<uint32_t>(sum);
   } else {
     u32x4 o = {0, 0, 0, 0};
     float sum = 0.0f;
@@ -210,25 +208,16 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint16_t e = in && k + i < g.K ? x[i] : static_cast<uint16_t>(0);
-      sum += Elem<DT>::up(e);
+      if constexpr (DT == kBF16) sum += Elem<DT>::up(e);
       o[i / 2] |= static_cast<uint32_t>(e) << (16 * (i & 1));
     }
     *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = o;
-    total = __builtin_bit_cast(uint32_t, sum);
-    if (DT == kF16) {
-      if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = 0x3F800000u;
-      return;
+    if constexpr (DT == kBF16) {
+#pragma unroll
+      for (int n = 1; n < U; n *= 2) sum += __shfl_xor(sum, n);
+      if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = __builtin_bit_cast(uint32_t, sum);
     }
   }
-#pragma unroll
-  for (int n = 1; n < U; n *= 2) {
-    const uint32_t o = __shfl_xor(static_cast<int>(total), n);
-    if constexpr (DT == kI8)
-      total += o;
-    else
-      total = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, total) + __builtin_bit_cast(float, o));
-  }
-  if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = total;
 }
 
 // ---- few rows -------------------------------------------------------------------------------------
@@ -610,8 +599,9 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
   const int gthread = threadIdx.x - group * WN * 64;
   const int q = lane >> 4;
   const int btile = blockIdx.x * (WN * 4), tile0 = btile + in * 4, rt0 = blockIdx.y * TT;
-  // LDS of a group: two buffers of the rows' pieces, the scales [WN 4][S][16] and the rows' numbers [TT][S][16]
-  constexpr int pieces = TT * KB, words = (WN * 4 + TT) * S * 16, buf_bytes = pieces * 1024 + words * 4;
+  // LDS of a group: two buffers of the rows' pieces, the scales [WN 4][S][16] and the rows' numbers, if any, [TT][S][16]
+  constexpr bool kNumbers = w4_numbers(DT);
+  constexpr int pieces = TT * KB, words = (WN * 4 + (kNumbers ? TT : 0)) * S * 16, buf_bytes = pieces * 1024 + words * 4;
   char* mem = lds + group * 2 * buf_bytes;
 
   const uint32_t* cw[4];
@@ -688,15 +678,18 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
       const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
       const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + WN * 4 * S * 16 + (lane & 15);
 
-      // the zero points of this lane's outputs of the operand (lane % 16 of each tile), as pairs of 128 + z
+      // the zero points of this lane's outputs of the operand (lane % 16 of each tile), for less() or less_bytes()
       uint32_t zero[4];
       auto zeros = [&](int s) {
-        if constexpr (OT == kF16) {
+        if constexpr (OT != kBF16) {
           const uint32_t* z_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + (lane & 15);
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             const uint32_t z = z_at[(n * S + s) * 16] >> 16;
-            zero[n] = M::bits + (z << 3 | z << 19);
+            if constexpr (OT == kI8)
+              zero[n] = 0x80808080u - z * 0x01010101u;
+            else
+              zero[n] = M::bits + (z << 3 | z << 19);
           }
         }
       };
@@ -710,7 +703,7 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
         if (!mine_too) return;
         uint32_t x[TT];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) x[t] = x_at[(t * S + s) * 16];
+        for (int t = 0; t < TT; ++t) x[t] = kNumbers ? x_at[(t * S + s) * 16] : 0;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const u32x4 sz = *reinterpret_cast<const u32x4*>(sc_at + (n * S + s) * 16);
@@ -719,11 +712,10 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
             const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[i])));
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-              if constexpr (OT == kF16) {
+              if constexpr (DT == kF32) {
                 acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(float, x[t]), acc[n][t][i]);
-              } else if constexpr (DT == kI8) {
-                acc[n][t][i] = __builtin_fmaf(
-                    sc, static_cast<float>(d[n][t][i] - __mul24(static_cast<int>(sz[i] >> 16), static_cast<int>(x[t]))), acc[n][t][i]);
+              } else if constexpr (!kNumbers) {
+                acc[n][t][i] = __builtin_fmaf(sc, static_cast<float>(d[n][t][i]), acc[n][t][i]);
               } else {
                 const float z = static_cast<float>(sz[i] >> 16) + M::base;
                 acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, __builtin_bit_cast(float, x[t]), d[n][t][i]), acc[n][t][i]);
@@ -743,11 +735,12 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) {
               clear();
+              zeros(2 * half + jj);
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
                 uint32_t lo, hi;
                 w4_bytes(w[n][2 * half + jj], lo, hi);
-                const long aw = static_cast<long>(hi) << 32 | lo;
+                const long aw = static_cast<long>(less_bytes(hi, zero[n])) << 32 | less_bytes(lo, zero[n]);
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
                   const long bx =
@@ -759,12 +752,15 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
             }
           } else {
             if (STEP == 64 || half == 0) clear();
+            zeros(STEP == 64 ? half : 0);
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
               uint32_t lo0, hi0, lo1, hi1;
               w4_bytes(w[n][2 * half], lo0, hi0);
               w4_bytes(w[n][2 * half + 1], lo1, hi1);
-              const i32x4 aw = __builtin_bit_cast(i32x4, u32x4{lo0, hi0, lo1, hi1});
+              const uint32_t z = zero[n];
+              const i32x4 aw = __builtin_bit_cast(
+                  i32x4, u32x4{less_bytes(lo0, z), less_bytes(hi0, z), less_bytes(lo1, z), less_bytes(hi1, z)});
 #pragma unroll
               for (int t = 0; t < TT; ++t) d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw, b[t], d[n][t], 0, 0, 0);
             }
@@ -891,7 +887,7 @@ hipError_t gemm_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
   constexpr int TT = kRowTiles, S = 128 / STEP;
   static_assert(TT == kW4TileRows / 16, "the plan's tiles");
   const W4Plan p = w4_plan(DT, g, rt);
-  const size_t buf = TT * kStageKB<DT> * 1024 + (p.wn * 4 + TT) * S * 64, stages = 2 * p.bk * buf;
+  const size_t buf = TT * kStageKB<DT> * 1024 + (p.wn * 4 + (w4_numbers(DT) ? TT : 0)) * S * 64, stages = 2 * p.bk * buf;
   const size_t red = (p.bk - 1) * p.wn * TT * 4096, lds = stages > red ? stages : red;  // up to 152 KB
   const dim3 grid((g.nt + p.wn * 4 - 1) / (p.wn * 4), (rt + TT - 1) / TT, p.ks);
   float* partials = p.ks > 1 ? reinterpret_cast<float*>(ws + w4_lay_bytes(DT, g, rt)) : nullptr;
