@@ -292,6 +292,16 @@ def test_w4_tiles(eng, t, i):  # noqa: F811
 
 
 @pytest.mark.parametrize("t", [F32, BF16, F16, I8])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_tiles_of_every_step(eng, t, group):  # noqa: F811
+    """Many rows with scales for 32, 64 and 128 inputs: few outputs and many, inputs in one run and in several."""
+    rng = np.random.default_rng(90 + group + t)
+    for i, (rows, K, N) in enumerate(((3100, 6900, 120), (90, 4100, 8001), (701, 600, 6500), (700, 2000, 2100),
+                                      (1515, 737, 2809))):
+        run_w4(eng, rng, t, rows, K, N, group, zeros=i % 2 == 0, padx=i, pado=i % 3)
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16, I8])
 @pytest.mark.parametrize("out_t", FLOATS)
 def test_w4_rounding(eng, t, out_t):  # noqa: F811
     """Real inputs: the fp32 rows keep all their digits."""
