@@ -85,6 +85,24 @@ inline const char* check(NormQArgs& a) {
   return nullptr;
 }
 
+// The kernel of a call: `threads` a row, each with `vecs` vectors of 16 bytes in registers, so that the row is read
+// once (threads * vecs vectors hold it), or threads 0: rows too long for that, read twice. A wave a row where
+// that fills the chip or a wave's one vector a lane is all it needs; else a block.
+struct NormPlan {
+  int threads, vecs;
+};
+constexpr int kNormVecs = 8, kNormVecsBlock = 4;  // the most of a wave or 256 threads, and what 1024 threads have
+inline NormPlan norm_plan(int dtype, size_t rows, size_t cols) {
+  const size_t v = 16 / dtype_size(dtype), all = (cols + v - 1) / v;
+  auto of = [&](size_t threads) {
+    return NormPlan{static_cast<int>(threads), static_cast<int>((all + threads - 1) / threads)};
+  };
+  if (all <= 64 || (all <= 64 * kNormVecs && rows >= 2048)) return of(64);
+  if (all <= 256 * kNormVecs) return of(256);
+  if (all <= 1024 * kNormVecsBlock) return {1024, kNormVecsBlock};
+  return {0, 0};
+}
+
 // ---- products with 4-bit weights ----------------------------------------------------------------
 // Weights laid out for the kernels. Outputs go in tiles of 16 and inputs in chunks of 128, padded:
 //   codes [ntile][chunk][lane 0..63][word 0..3]: lane l holds output 16 ntile + l % 16, and word j

@@ -191,11 +191,12 @@ __global__ __launch_bounds__(256) void k_normq_long(NormQArgs a) {
 
 }  // namespace
 
-template <int DT, int T, int NV = 8>
-static hipError_t normq_rows(const NormQArgs& a, int nv, hipStream_t s) {
+template <int DT, int T, int NV = kNormVecs>
+static hipError_t normq_rows(const NormQArgs& a, int vecs, hipStream_t s) {
   if constexpr (NV > 1) {  // the instance of the smallest NV that holds the row
-    if (nv < NV) return normq_rows<DT, T, NV == 8 ? 6 : NV - 1>(a, nv, s);
+    if (vecs < NV) return normq_rows<DT, T, NV - 1>(a, vecs, s);
   }
+  if (vecs != NV) return hipErrorInvalidValue;
   constexpr int B = T < 256 ? 256 : T;
   k_normq<DT, T, NV><<<static_cast<unsigned>((a.rows + B / T - 1) / (B / T)), B, 0, s>>>(a);
   return hipGetLastError();
@@ -204,17 +205,14 @@ static hipError_t normq_rows(const NormQArgs& a, int nv, hipStream_t s) {
 hipError_t launch_normq(const NormQArgs& a, hipStream_t s) {
   if (!a.rows || !a.cols) return hipSuccess;
   return with_type(a.dtype, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value, V = Elem<DT>::V;
-    const size_t vecs = (a.cols + V - 1) / V;
-    auto nv = [&](size_t t) { return static_cast<int>((vecs + t - 1) / t); };
-    // a wave a row where that fills the chip or a wave is all it needs; else a block
-    if (vecs <= 64 || (vecs <= 64 * 8 && a.rows >= 2048)) return normq_rows<DT, 64>(a, nv(64), s);
-    if (vecs <= 256 * 8) return normq_rows<DT, 256>(a, nv(256), s);
-    if (vecs <= 1024 * 4) {
-      k_normq<DT, 1024, 4><<<static_cast<unsigned>(a.rows), 1024, 0, s>>>(a);
-      return hipGetLastError();
-    }
-    k_normq_long<DT><<<static_cast<unsigned>(a.rows), 256, 0, s>>>(a);
+    constexpr int DT = decltype(dt)::value;
+    const NormPlan p = norm_plan(DT, a.rows, a.cols);
+    if (p.threads == 64) return normq_rows<DT, 64>(a, p.vecs, s);
+    if (p.threads == 256) return normq_rows<DT, 256>(a, p.vecs, s);
+    if (p.threads == 1024)
+      k_normq<DT, 1024, kNormVecsBlock><<<static_cast<unsigned>(a.rows), 1024, 0, s>>>(a);
+    else
+      k_normq_long<DT><<<static_cast<unsigned>(a.rows), 256, 0, s>>>(a);
     return hipGetLastError();
   });
 }

@@ -247,7 +247,26 @@ static void products_plan() {
           }
 }
 
+// The norm's plan: its threads' vectors hold the row, one fewer each would not, and the form has a kernel.
+static void norm_plans() {
+  for (int t : {kF32, kBF16, kF16})
+    for (size_t rows : {1, 2047, 2048, 100000})
+      for (size_t cols = 1; cols <= 40000; ++cols) {
+        const NormPlan p = norm_plan(t, rows, cols);
+        const size_t vec = 16 / dtype_size(t), held = static_cast<size_t>(p.threads) * p.vecs * vec;
+        if (!p.threads) {
+          is("norm of rows read twice", cols > 1024 * kNormVecsBlock * vec, 1);
+          continue;
+        }
+        is("norm's threads", p.threads == 64 || p.threads == 256 || (p.threads == 1024 && p.vecs == kNormVecsBlock), 1);
+        is("norm's vectors", p.vecs >= 1 && p.vecs <= kNormVecs, 1);
+        is("norm holds the row", held >= cols, 1);
+        if (p.threads < 1024) is("norm's smallest", held - static_cast<size_t>(p.threads) * vec < cols, 1);
+      }
+}
+
 int main() {
+  norm_plans();
   products_plan();
   plans();
   norms();
