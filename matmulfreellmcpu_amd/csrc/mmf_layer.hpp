@@ -130,6 +130,10 @@ inline W4Geom w4_geom(size_t N, size_t K, size_t group) {
 MMF_HD inline constexpr int w4_k(int step, int j, int q) {
   return step == 32 ? 32 * j + 8 * q : 64 * (j >> 1) + 16 * q + 8 * (j & 1);
 }
+// Neighbouring inputs that a lane of the few-row kernel loads of a row at once, from w4_k on: a word's 8, or of
+// int8 rows the 16 of two words where these are neighbours. (No load goes past its chunk: a whole last chunk ends
+// with the row, and the last row's with the caller's memory.)
+MMF_HD inline constexpr int w4_load(int dtype, int step) { return dtype == kI8 && step != 32 ? 16 : 8; }
 // Nibble of element e (0..7) of a word: neighbours 2p and 2p + 1 are nibbles p and p + 4, the same bits
 // of the word's two halves, so that one mask makes a pair of 16-bit floats of them.
 MMF_HD inline constexpr int w4_nibble(int e) { return 4 * (e & 1) + (e >> 1); }

@@ -52,7 +52,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(1)));
 typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 
 __device__ __forceinline__ uint32_t rotr(uint32_t w, int n) { return __builtin_amdgcn_alignbit(w, w, n); }
@@ -116,12 +115,14 @@ __device__ __forceinline__ u32x4 less(u32x4 a, uint32_t b) {
 // Four bytes: a code less its zero point, with b = 0x80 - z in each: their sum is at most 0x8F, so nothing carries.
 __device__ __forceinline__ uint32_t less_bytes(uint32_t a, uint32_t b) { return (a + b) ^ 0x80808080u; }
 
-// 16 bytes of a row of 16-bit elements (8) or bytes (16) from element k, zeros behind K.
-template <int DT>
-__device__ __forceinline__ u32x4 row_16B(const char* row, int k, int K, bool whole) {
-  constexpr int ES = DT == kI8 ? 1 : 2, V = 16 / ES;
-  if (whole || k + V <= K) return *reinterpret_cast<const u32x4u*>(row + static_cast<size_t>(k) * ES);
-  u32x4 v = {0, 0, 0, 0};
+// A lane's load of a row of 16-bit elements or bytes: the V elements from k on (16 bytes, or 8), zeros behind K.
+template <int DT, int STEP>
+__device__ __forceinline__ auto row_load(const char* row, int k, int K, bool whole) {
+  constexpr int ES = DT == kI8 ? 1 : 2, V = w4_load(DT, STEP);
+  typedef uint32_t Vec __attribute__((ext_vector_type(V * ES / 4)));
+  typedef uint32_t VecU __attribute__((ext_vector_type(V * ES / 4), aligned(1)));
+  if (whole || k + V <= K) return static_cast<Vec>(*reinterpret_cast<const VecU*>(row + static_cast<size_t>(k) * ES));
+  Vec v = {};
   for (int i = 0; i < V; ++i)
     if (k + i < K) {
       const uint32_t e = ES == 1 ? *reinterpret_cast<const uint8_t*>(row + k + i)
@@ -359,11 +360,11 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
         for (int j = 0; j < 4; j += 2) {  // two words' 16 inputs: neighbours, or with steps of 32 two runs of 8
           u32x4 v;
           if constexpr (STEP == 32) {
-            const u32x4 v0 = row_16B<DT>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole),
-                        v1 = row_16B<DT>(xr[t], c * 128 + w4_k(STEP, j + 1, q), g.K, whole);
+            const auto v0 = row_load<DT, STEP>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole);
+            const auto v1 = row_load<DT, STEP>(xr[t], c * 128 + w4_k(STEP, j + 1, q), g.K, whole);
             v = u32x4{v0.x, v0.y, v1.x, v1.y};
           } else {
-            v = row_16B<DT>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole);
+            v = row_load<DT, STEP>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole);
           }
           uint32_t lo0, hi0, lo1, hi1;
           i8_operand(v.x, v.y, lo0, hi0);
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
 #pragma unroll
       for (int t = 0; t < CT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[t][j] = row_16B<DT>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole);
+        for (int j = 0; j < 4; ++j) b[t][j] = row_load<DT, STEP>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole);
     }
     if (c + waves < g.nc) fetch(c + waves);
 

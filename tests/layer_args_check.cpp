@@ -119,6 +119,23 @@ static void products() {
   }
 }
 
+// The few-row kernel's loads of a row stay in its chunk and bring each of its inputs once.
+static void product_loads() {
+  for (int t : {kBF16, kF16, kI8})
+    for (int step : {32, 64, 128}) {
+      const int n = w4_load(t, step);
+      int got[128] = {};
+      for (int q = 0; q < 4; ++q)
+        for (int j = 0; j < 4; j += n / 8)
+          for (int e = 0; e < n; ++e) {
+            const int k = w4_k(step, j, q) + e;
+            is("w4 load within its chunk", k < 128, 1);
+            if (k < 128) ++got[k];
+          }
+      for (int k = 0; k < 128; ++k) is("w4 loads of an input", got[k], 1);
+    }
+}
+
 static void sequences() {
   const size_t lens[] = {3, 0, 5, 9, 0};
   want("lens", check_seqs(lens, 5, 17), nullptr);
@@ -271,6 +288,7 @@ int main() {
   plans();
   norms();
   products();
+  product_loads();
   sequences();
   mixers();
   std::printf("%d unmet\n", bad);
