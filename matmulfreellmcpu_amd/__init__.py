@@ -261,6 +261,8 @@ class Engine:
         codes, cp = _np(codes, np.uint8)
         scales, sp = _np(scales, np.float16)
         N, K = codes.shape[0], 2 * codes.shape[1] if K is None else K
+        if group < 0:
+            raise ValueError(f"group {group} is negative")
         groups = -(-K // group) if group else 1
         if codes.shape != (N, (K + 1) // 2) or scales.shape != (N, groups):
             raise ValueError(f"codes {codes.shape} and scales {scales.shape} are not those of {N} x {K} in groups of {group}")

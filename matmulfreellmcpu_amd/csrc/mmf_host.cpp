@@ -100,6 +100,7 @@ struct Proj {
 // 4-bit weights (mmf_w4_register): codes and scales in one allocation.
 struct W4 {
   W4Geom g{};
+  size_t group = 0;  // as registered: any size, where a row is one group
   void* mem = nullptr;
   const uint32_t *codes = nullptr, *scales = nullptr;
 };
@@ -1574,6 +1575,7 @@ int mmf_w4_register(mmf_ctx* c, const uint8_t* codes, const uint16_t* scales, co
     refuse(check_w4(N, K, group));
     W4 w;
     w.g = w4_geom(N, K, group);
+    w.group = group ? group : K;
     const size_t groups = (K + w.g.group - 1) / w.g.group, nc = N * ((K + 1) / 2), ns = N * groups * 2,
                  nz = zeros ? N * groups : 0;
     for (size_t i = 0; i < nz; ++i)
@@ -1605,7 +1607,7 @@ int mmf_w4_shape(mmf_ctx* c, int id, size_t* N, size_t* K, size_t* group) {
     const W4& w = w4_of(c, id);
     if (N) *N = w.g.N;
     if (K) *K = w.g.K;
-    if (group) *group = w.g.group;
+    if (group) *group = w.group;
   });
 }
 

@@ -112,13 +112,13 @@ inline NormPlan norm_plan(int dtype, size_t rows, size_t cols) {
 // step is the kernel's scale granularity, 32, 64 or 128 inputs: the largest that divides the group
 // (of rows that are one group: 128).
 struct W4Geom {
-  int N, K, group, step, nt, nc, ns;  // tiles of 16 outputs, chunks of 128 inputs, scales a tile row
+  int N, K, group, step, nt, nc, ns;  // inputs of a scale (at most K), tiles of 16 outputs, chunks of 128 inputs, scales a tile row
 };
 inline W4Geom w4_geom(size_t N, size_t K, size_t group) {
   W4Geom g;
   g.N = static_cast<int>(N);
   g.K = static_cast<int>(K);
-  g.group = static_cast<int>(group ? group : K);
+  g.group = static_cast<int>(group && group < K ? group : K);
   g.step = !group || group >= K || group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32;
   g.nt = static_cast<int>((N + 15) / 16);
   g.nc = static_cast<int>((K + 127) / 128);

@@ -92,6 +92,16 @@ static void products() {
   go("w4 alignment", "aligned", [](W4Args& a) { a.out_dtype = kBF16, a.out = at<char>(0x20001); });
   go("w4 overlap", "overlaps", [](W4Args& a) { a.out = at<char>(0x10040); });
 
+  // a group of any size at or beyond the row is the row, also past what an int holds
+  for (size_t group : {size_t{64}, size_t{1} << 20, (size_t{1} << 31) - 32, size_t{1} << 31, size_t{1} << 32,
+                       (size_t{1} << 32) + 32, ~size_t{31}}) {
+    want("w4 large group", check_w4(16, 64, group), nullptr);
+    const W4Geom g = w4_geom(16, 64, group);
+    is("w4 large group's inputs", g.group, 64);
+    is("w4 large group's step", g.step, 128);
+  }
+  is("w4 group", w4_geom(16, 64, 32).group, 32);
+
   // the packed layout holds every code and scale once, within its bytes
   const size_t shapes[][3] = {{1, 1, 32}, {17, 1031, 32}, {33, 129, 64}, {16, 128, 128}, {100, 96, 96}, {5, 300, 0},
                               {40, 700, 256}, {3, 64, 1024}, {48, 640, 192}};

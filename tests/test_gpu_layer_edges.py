@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_layer import F32, FLOATS, run_norm
+from test_gpu_layer import F32, FLOATS, I8, run_norm, run_w4
 from test_gpu_parity import eng  # noqa: F401  (module fixture)
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +33,16 @@ def test_norm_widths(eng, cols, t):  # noqa: F811
     run_norm(eng, rng, t, 2, cols, pads=(1, 0, 2, 0, 3), offs=(1, 0, 1, 0, 1))
     if cols < 7000:
         run_norm(eng, rng, t, 2050, cols, h=False, y=False)
+
+
+# ---- 4-bit products ---------------------------------------------------------------------------
+
+
+def test_w4_groups_beyond_the_row(eng):  # noqa: F811
+    """A group of any size that holds the row is one group a row, and is the shape that is given back."""
+    rng = np.random.default_rng(30)
+    for group in (96, 2 ** 20, 2 ** 31 - 32, 2 ** 31, 2 ** 32, 2 ** 32 + 32, 2 ** 62):
+        for t in (F32, I8):
+            run_w4(eng, rng, t, 3, 77, 21, group, zeros=True)
+    with pytest.raises(ValueError, match="negative"):
+        eng.register_w4(np.zeros((4, 10), np.uint8), np.zeros((4, 0), np.float16), K=20, group=-32)
