@@ -35,17 +35,35 @@ struct RowsOf {
 
 inline bool rows_aligned(const RowsOf& a) { return reinterpret_cast<uintptr_t>(a.p) % a.esize == 0; }
 
-// Whether two row tensors of `rows` rows share an element. Tensors that are column ranges of one
-// buffer (the same ld) overlap only if their columns do; others are compared by their whole ranges.
+// Whether the bytes from p on share one with a row tensor of `rows` rows: p may stand between two of its rows.
+inline bool bytes_overlap(const void* p, size_t bytes, const RowsOf& t, size_t rows) {
+  if (!rows || !p || !t.p || !bytes || !t.cols) return false;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(t.p);
+  const size_t step = t.ld * t.esize, row = t.cols * t.esize;
+  if (a + bytes <= b || a >= b + (rows - 1) * step + row) return false;
+  if (a <= b) return true;
+  const size_t in = (a - b) % step;  // of the row that starts at or before p; a later one follows if p is past its end
+  return in < row || in + bytes > step;
+}
+inline bool array_overlaps(const void* p, size_t n, const RowsOf& t, size_t rows) { return bytes_overlap(p, n * 4, t, rows); }
+// Whether two row tensors of `rows` rows share a byte. Tensors with the same distance from row to row do if their
+// columns do; others are compared row by row, where their whole ranges meet.
 inline bool rows_overlap(const RowsOf& a, const RowsOf& b, size_t rows) {
   if (!rows || !a.p || !b.p || !a.cols || !b.cols) return false;
   const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
-  const uintptr_t ea = pa + ((rows - 1) * a.ld + a.cols) * a.esize, eb = pb + ((rows - 1) * b.ld + b.cols) * b.esize;
+  const size_t step = a.ld * a.esize, row = a.cols * a.esize;
+  const uintptr_t ea = pa + (rows - 1) * step + row, eb = pb + ((rows - 1) * b.ld + b.cols) * b.esize;
   if (ea <= pb || eb <= pa) return false;
-  const size_t step = a.ld * a.esize;
-  if (step != b.ld * b.esize) return true;
-  const size_t d = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;
-  return d < a.cols * a.esize || d + b.cols * b.esize > step;
+  if (step == b.ld * b.esize) {
+    const size_t d = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;
+    return d < row || d + b.cols * b.esize > step;
+  }
+  for (size_t r = 0; r < rows; ++r)
+    if (bytes_overlap(static_cast<const char*>(a.p) + r * step, row, b, rows)) return true;
+  return false;
+}
+inline bool arrays_overlap(const void* p, size_t n, const void* q, size_t m) {
+  return array_overlaps(p, n, RowsOf{q, m, m, 4}, 1);
 }
 inline bool same_rows(const RowsOf& a, const RowsOf& b) { return a.p == b.p && a.ld == b.ld && a.esize == b.esize; }
 
@@ -82,6 +100,11 @@ inline const char* check(NormQArgs& a) {
   for (const RowsOf& in : {x, r, h})
     if (rows_overlap(y, in, a.rows) || rows_overlap(c, in, a.rows)) return "an output overlaps another tensor of the call";
   if (rows_overlap(y, c, a.rows)) return "an output overlaps another tensor of the call";
+  for (const RowsOf& t : {x, r, h, y, c})
+    if (array_overlaps(a.scales, a.rows, t, a.rows)) return "the scales overlap another tensor of the call";
+  for (const RowsOf& out : {h, y, c})
+    if (array_overlaps(a.w, a.cols, out, a.rows)) return "an output overlaps the weights";
+  if (arrays_overlap(a.scales, a.rows, a.w, a.cols)) return "the scales overlap another tensor of the call";
   return nullptr;
 }
 
@@ -242,7 +265,7 @@ inline const char* check(W4Args& a, size_t N, size_t K) {
   const RowsOf x{a.x, a.ldx, K, dtype_size(a.dtype)}, o{a.out, a.ldo, N, dtype_size(a.out_dtype)},
       s{a.xscales, 1, 1, 4};
   if (!rows_aligned(x) || !rows_aligned(o) || !rows_aligned(s)) return "a pointer is not aligned to its type";
-  if (rows_overlap(x, o, a.rows) || rows_overlap(s, o, a.rows)) return "the output overlaps an input";
+  if (rows_overlap(x, o, a.rows) || array_overlaps(a.xscales, a.rows, o, a.rows)) return "the output overlaps an input";
   return nullptr;
 }
 
@@ -334,10 +357,16 @@ inline const char* check(ConvArgs& a) {
   for (const RowsOf& t : {x, o, w, b, s})
     if (!rows_aligned(t)) return "a pointer is not aligned to its type";
   if (rows_overlap(x, o, a.rows)) return "the output overlaps the input";
-  const RowsOf whole{a.state, a.seqs * held, a.seqs * held, 4};
-  for (const RowsOf& t : {x, o}) {
-    const size_t all = (a.rows - 1) * t.ld + t.cols;
-    if (rows_overlap(whole, RowsOf{t.p, all, all, es}, 1)) return "the state overlaps another tensor of the call";
+  const size_t all = a.seqs * held;
+  for (const RowsOf& t : {x, o})
+    if (array_overlaps(a.state, all, t, a.rows)) return "the state overlaps another tensor of the call";
+  const struct {
+    const float* p;
+    size_t n;
+  } params[] = {{a.w, a.D * a.width}, {a.bias, a.D}};
+  for (const auto& p : params) {
+    if (array_overlaps(p.p, p.n, o, a.rows)) return "the output overlaps the weights or the bias";
+    if (arrays_overlap(a.state, all, p.p, p.n)) return "the state overlaps another tensor of the call";
   }
   return nullptr;
 }
@@ -374,18 +403,23 @@ inline const char* check(ScanArgs& a) {
   const RowsOf ins[] = {{a.u, a.ldu, a.D, es}, {a.dt, a.lddt, a.D, es}, {a.B, a.ldb, a.N, es}, {a.C, a.ldc, a.N, es},
                         {a.z, a.ldz, a.D, es}};
   const size_t held = a.seqs * a.N * a.D;
-  const RowsOf whole{a.state, held, held, 4};
   if (!rows_aligned(o)) return "a pointer is not aligned to its type";
   for (const RowsOf& t : ins) {
     if (!rows_aligned(t)) return "a pointer is not aligned to its type";
     if (rows_overlap(o, t, a.rows)) return "the output overlaps an input";
-    const size_t all = (a.rows - 1) * t.ld + t.cols;
-    if (rows_overlap(whole, RowsOf{t.p, all, all, es}, 1)) return "the state overlaps another tensor of the call";
+    if (array_overlaps(a.state, held, t, a.rows)) return "the state overlaps another tensor of the call";
   }
   for (const float* p : {a.A, a.skip, a.dt_bias, static_cast<const float*>(a.state)})
     if (reinterpret_cast<uintptr_t>(p) % 4) return "a pointer is not aligned to its type";
-  const size_t all = (a.rows - 1) * a.ldo + a.D;
-  if (rows_overlap(whole, RowsOf{a.out, all, all, es}, 1)) return "the state overlaps another tensor of the call";
+  if (array_overlaps(a.state, held, o, a.rows)) return "the state overlaps another tensor of the call";
+  const struct {
+    const float* p;
+    size_t n;
+  } params[] = {{a.A, a.D * a.N}, {a.skip, a.D}, {a.dt_bias, a.D}};
+  for (const auto& p : params) {
+    if (array_overlaps(p.p, p.n, o, a.rows)) return "the output overlaps an input";
+    if (arrays_overlap(a.state, held, p.p, p.n)) return "the state overlaps another tensor of the call";
+  }
   return nullptr;
 }
 

@@ -65,6 +65,22 @@ static void norms() {
      [](NormQArgs& a) { a.ldx = a.ldh = 200, a.h = at<float>(0x10000 + 400); });
   go("norm touching neighbours", "overlaps",
      [](NormQArgs& a) { a.ldx = a.ldh = 200, a.h = at<float>(0x10000 + 396); });
+  // scales [4] and weights [100] beside rows of 400 bytes (codes: 100)
+  go("norm scales on x", "overlap", [](NormQArgs& a) { a.scales = at<float>(0x10000 + 1596); });
+  go("norm scales behind x", nullptr, [](NormQArgs& a) { a.scales = at<float>(0x10000 + 1600); });
+  go("norm scales up to x", nullptr, [](NormQArgs& a) { a.scales = at<float>(0x10000 - 16); });
+  go("norm scales into x", "overlap", [](NormQArgs& a) { a.scales = at<float>(0x10000 - 12); });
+  go("norm scales on res", "overlap", [](NormQArgs& a) { a.scales = at<float>(0x20000); });
+  go("norm scales on h", "overlap", [](NormQArgs& a) { a.scales = at<float>(0x30000 + 4); });
+  go("norm scales on y", "overlap", [](NormQArgs& a) { a.y = at<float>(0x60000), a.scales = at<float>(0x60000 + 400); });
+  go("norm scales on codes", "overlap", [](NormQArgs& a) { a.scales = at<float>(0x40000 + 396); });
+  go("norm scales on w", "overlap", [](NormQArgs& a) { a.scales = at<float>(0x900 + 396); });
+  go("norm scales in a gap", nullptr, [](NormQArgs& a) { a.ldx = 200, a.scales = at<float>(0x10000 + 800 - 16); });
+  go("norm scales out of a gap", "overlap", [](NormQArgs& a) { a.ldx = 200, a.scales = at<float>(0x10000 + 800 - 12); });
+  go("norm h on w", "overlaps", [](NormQArgs& a) { a.w = at<float>(0x30000 - 396); });
+  go("norm y on w", "overlaps", [](NormQArgs& a) { a.y = at<float>(0x900); });
+  go("norm codes on w", "overlaps", [](NormQArgs& a) { a.codes = at<int8_t>(0x900 + 399); });
+  go("norm codes behind w", nullptr, [](NormQArgs& a) { a.codes = at<int8_t>(0x900 + 400); });
 }
 
 static void products() {
@@ -91,6 +107,8 @@ static void products() {
   go("w4 no rows", nullptr, [](W4Args& a) { a.rows = 0, a.x = nullptr; });
   go("w4 alignment", "aligned", [](W4Args& a) { a.out_dtype = kBF16, a.out = at<char>(0x20001); });
   go("w4 overlap", "overlaps", [](W4Args& a) { a.out = at<char>(0x10040); });
+  go("w4 out on scales", "overlaps", [](W4Args& a) { a.dtype = kI8, a.xscales = at<float>(0x20000 + 1596); });
+  go("w4 scales in a gap of out", nullptr, [](W4Args& a) { a.dtype = kI8, a.ldo = 104, a.xscales = at<float>(0x20000 + 400); });
 
   // a group of any size at or beyond the row is the row, also past what an int holds
   for (size_t group : {size_t{64}, size_t{1} << 20, (size_t{1} << 31) - 32, size_t{1} << 31, size_t{1} << 32,
@@ -204,6 +222,15 @@ static void mixers() {
   conv("conv halves of one buffer", nullptr,
        [](ConvArgs& a) { a.ldx = a.ldo = 128, a.out = at<float>(0x10000 + 256); });
 
+  conv("conv out on w", "overlaps", [](ConvArgs& a) { a.w = at<float>(0x20000 - 1020); });
+  conv("conv out behind w", nullptr, [](ConvArgs& a) { a.w = at<float>(0x20000 - 1024); });
+  conv("conv out on bias", "overlaps", [](ConvArgs& a) { a.bias = at<float>(0x20000 + 1020); });
+  conv("conv state on w", "state", [](ConvArgs& a) { a.state = at<float>(0x900 + 1020); });
+  conv("conv state on bias", "state", [](ConvArgs& a) { a.bias = at<float>(0x30000 + 1532); });
+  conv("conv bias behind the state", nullptr, [](ConvArgs& a) { a.bias = at<float>(0x30000 + 1536); });
+  conv("conv state of width 1 is none", nullptr, [](ConvArgs& a) { a.width = 1, a.state = at<float>(0x900); });
+  conv("conv state in a gap", nullptr, [](ConvArgs& a) { a.ldx = 1000, a.state = at<float>(0x10000 + 256); });
+
   auto scan = [&](const char* what, const char* part, auto&& change) {
     ScanArgs a{};
     a.out = at<float>(0x20000), a.u = at<float>(0x10000), a.dt = at<float>(0x30000), a.B = at<float>(0x40000);
@@ -226,6 +253,15 @@ static void mixers() {
   scan("scan state on out", "state", [](ScanArgs& a) { a.state = at<float>(0x20010); });
   scan("scan alignment", "aligned", [](ScanArgs& a) { a.skip = at<float>(0x902); });
   scan("scan B and C in one buffer", nullptr, [](ScanArgs& a) { a.ldb = a.ldc = 32, a.C = at<float>(0x40040); });
+  scan("scan out on A", "overlaps", [](ScanArgs& a) { a.A = at<float>(0x20000 + 1020); });
+  scan("scan A behind out", nullptr, [](ScanArgs& a) { a.A = at<float>(0x20000 + 1024); });
+  scan("scan out on skip", "overlaps", [](ScanArgs& a) { a.skip = at<float>(0x20000 - 4); });
+  scan("scan out on dt_bias", "overlaps", [](ScanArgs& a) { a.dt_bias = at<float>(0x20000); });
+  scan("scan state on A", "state", [](ScanArgs& a) { a.A = at<float>(0x60000 + 8188); });
+  scan("scan state on skip", "state", [](ScanArgs& a) { a.skip = at<float>(0x60000); });
+  scan("scan state on dt_bias", "state", [](ScanArgs& a) { a.dt_bias = at<float>(0x60000 - 252); });
+  scan("scan dt_bias before the state", nullptr, [](ScanArgs& a) { a.dt_bias = at<float>(0x60000 - 256); });
+  scan("scan state in a gap", nullptr, [](ScanArgs& a) { a.ldu = 10000, a.state = at<float>(0x10000 + 256 + 4); });
   scan("scan no rows", nullptr, [](ScanArgs& a) { a.rows = 0, a.lens = nullptr, a.u = nullptr; });
 }
 
