@@ -130,6 +130,38 @@ def _ptr(x):
     return x.data_ptr()
 
 
+# Row types of tensors' dtypes by name; -1: of none. Other dtypes (bytes, 16-bit words) are taken as storage.
+_ROW_TYPES = {"float32": F32, "bfloat16": BF16, "float16": F16, "int8": I8, "float64": -1}
+_row_types = {}  # the same by dtype object, entered as they are met
+
+
+def _row_type(x):
+    """The row type of a tensor, or None of an address or of storage."""
+    d = getattr(x, "dtype", None)
+    if d not in _row_types:
+        _row_types[d] = _ROW_TYPES.get(str(d).rpartition(".")[2])
+    return _row_types[d]
+
+
+def _rows(x, t):
+    """As _ptr, of rows of type t: a tensor of another type is refused."""
+    if x is None or x.__class__ is int:
+        return x
+    try:
+        if _row_types[x.dtype] == t:
+            return x.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    if _row_type(x) not in (t, None):
+        raise ValueError(f"a tensor of {x.dtype} in the place of rows of type {t} (F32, BF16, F16, I8 = 0, 1, 2, 3)")
+    return _ptr(x)
+
+
+def _own_type(x):
+    """The row type of a tensor; an address alone is of F32."""
+    return max(_row_type(x) or F32, F32)
+
+
 def _np(a, dtype):
     a = np.ascontiguousarray(a, dtype=dtype)
     return a, a.ctypes.data_as(C.c_void_p)
@@ -249,12 +281,16 @@ class Engine:
     def rmsnorm_swishgate(self, out, g, o, w, rows, cols, eps=1e-6):
         self._chk(self.lib.mmf_rmsnorm_swishgate(self.h, _ptr(out), _ptr(g), _ptr(o), _ptr(w), rows, cols, eps))
 
-    # ---- layer operators: rows of dtype F32, BF16 or F16, strides in elements (0: the row's length) ----
-    def add_rmsnorm_q8(self, codes, scales, x, w, rows, cols, res=None, h=None, y=None, eps=1e-6, dtype=F32, ldx=0,
+    # ---- layer operators: rows of dtype F32, BF16 or F16 (None: the first input's own, F32 for an address; tensors of
+    # another type are refused), strides in elements (0: the row's length) ----
+    def add_rmsnorm_q8(self, codes, scales, x, w, rows, cols, res=None, h=None, y=None, eps=1e-6, dtype=None, ldx=0,
                        ldres=0, ldh=0, ldy=0, ldcodes=0):
         """h = x + res, its RMS norm as int8 codes with a scale per row (mmf_add_rmsnorm_q8)."""
-        self._chk(self.lib.mmf_add_rmsnorm_q8(self.h, dtype, _ptr(codes), _ptr(scales), _ptr(x), _ptr(res), _ptr(h),
-                                              _ptr(y), _ptr(w), rows, cols, ldx, ldres, ldh, ldy, ldcodes, eps))
+        t = _own_type(x) if dtype is None else dtype
+        rc = self.lib.mmf_add_rmsnorm_q8(self.h, t, _rows(codes, I8), _ptr(scales), _rows(x, t), _rows(res, t), _rows(h, t),
+                                         _rows(y, t), _ptr(w), rows, cols, ldx, ldres, ldh, ldy, ldcodes, eps)
+        if rc:
+            self._chk(rc)
 
     def register_w4(self, codes, scales, zeros=None, K=None, group=128) -> int:
         """4-bit weights: codes uint8 [N, ceil(K/2)], scales float16 and zeros uint8 (or None: 8) [N, ceil(K/group)]."""
@@ -283,25 +319,35 @@ class Engine:
     def w4_release(self, wid):
         self._chk(self.lib.mmf_w4_release(self.h, wid))
 
-    def w4_linear(self, wid, x, out, rows, dtype=F32, out_dtype=F32, scales=None, ldx=0, ldo=0):
+    def w4_linear(self, wid, x, out, rows, dtype=None, out_dtype=None, scales=None, ldx=0, ldo=0):
         """out [rows, N] = x [rows, K] times 4-bit weights; dtype I8: codes with their scales [rows]."""
-        self._chk(self.lib.mmf_w4_linear(self.h, wid, dtype, _ptr(x), _ptr(scales), out_dtype, _ptr(out), rows, ldx, ldo))
+        t = _own_type(x) if dtype is None else dtype
+        o = _own_type(out) if out_dtype is None else out_dtype
+        rc = self.lib.mmf_w4_linear(self.h, wid, t, _rows(x, t), _ptr(scales), o, _rows(out, o), rows, ldx, ldo)
+        if rc:
+            self._chk(rc)
 
-    def short_conv(self, out, x, w, rows, D, width, bias=None, state=None, lens=None, seqs=1, silu=True, dtype=F32,
+    def short_conv(self, out, x, w, rows, D, width, bias=None, state=None, lens=None, seqs=1, silu=True, dtype=None,
                    ldx=0, ldo=0):
         """Short causal convolution of sequences of the lengths lens (None: `seqs` equal ones)."""
         _keep, lp, n = _lens(lens, seqs)
-        self._chk(self.lib.mmf_short_conv(self.h, dtype, _ptr(out), _ptr(x), _ptr(w), _ptr(bias), _ptr(state), lp, n,
-                                          rows, D, width, int(silu), ldx, ldo))
+        t = _own_type(x) if dtype is None else dtype
+        rc = self.lib.mmf_short_conv(self.h, t, _rows(out, t), _rows(x, t), _ptr(w), _ptr(bias), _ptr(state), lp, n, rows,
+                                     D, width, int(silu), ldx, ldo)
+        if rc:
+            self._chk(rc)
 
     def selective_scan(self, out, u, dt, A, B, C, rows, D, N, skip=None, z=None, dt_bias=None, state=None, lens=None,
-                       seqs=1, softplus=True, dtype=F32, ldo=0, ldu=0, lddt=0, ldb=0, ldc=0, ldz=0):
+                       seqs=1, softplus=True, dtype=None, ldo=0, ldu=0, lddt=0, ldb=0, ldc=0, ldz=0):
         """Selective state space scan of sequences of the lengths lens (None: `seqs` equal ones)."""
         _keep, lp, n = _lens(lens, seqs)
-        a = _SCAN_ARGS.pack(dtype, bool(softplus), _ptr(out) or 0, _ptr(u) or 0, _ptr(dt) or 0, _ptr(B) or 0, _ptr(C) or 0,
-                            _ptr(z) or 0, _ptr(A) or 0, _ptr(skip) or 0, _ptr(dt_bias) or 0, _ptr(state) or 0, lp or 0,
-                            n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
-        self._chk(self.lib.mmf_selective_scan(self.h, a))
+        t = _own_type(u) if dtype is None else dtype
+        a = _SCAN_ARGS.pack(t, bool(softplus), _rows(out, t) or 0, _rows(u, t) or 0, _rows(dt, t) or 0, _rows(B, t) or 0,
+                            _rows(C, t) or 0, _rows(z, t) or 0, _ptr(A) or 0, _ptr(skip) or 0, _ptr(dt_bias) or 0,
+                            _ptr(state) or 0, lp or 0, n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
+        rc = self.lib.mmf_selective_scan(self.h, a)
+        if rc:
+            self._chk(rc)
 
     # ---- model ----
     def load_blob(self, path_or_blob, mode=FLOAT, frac_bits=10):
