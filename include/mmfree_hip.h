@@ -184,12 +184,13 @@ int mmf_w4_shape(mmf_ctx* ctx, int w4_id, size_t* N, size_t* K, size_t* group);
 int mmf_w4_release(mmf_ctx* ctx, int w4_id);
 /* out [rows, N] = x [rows, K] times the transposed weights, from one token to long prompts. x of
  * dtype MMF_F32, MMF_BF16, MMF_F16, or MMF_I8 with xscales [rows] (else NULL): the codes and scales
- * of mmf_add_rmsnorm_q8. out is of out_dtype (a float type). The weights enter every sum as the
- * integers they are, with no rounding, and the scale multiplies a group's fp32 sum (int8 x: its
- * exact integer sum). An output's error is the rounding of fp32 sums of 31 |scale x| over all inputs of the
- * row, also of those that weights of 0 meet: an input 1e7 times the others leaves few of their digits. fp32
- * rows keep their digits for inputs between 1e-30 and 1e36. A row that holds an infinity or NaN has no
- * finite output. */
+ * of mmf_add_rmsnorm_q8. out is of out_dtype (a float type). The weights enter every sum as the integers they
+ * are, with no rounding. Sums are taken over runs of 32, 64 or 128 inputs (the largest of these that divides the
+ * group; 128 where a row is one group), in fp32 and for int8 x in exact integers, and each is multiplied by its scale
+ * and added in fp32: an output's error is that of fp32 sums of its own terms. In large products fp32 rows count
+ * to half a step of fp32, and fp32 and bf16 inputs to no less than 2^-40 of the largest input of their run's
+ * group. fp32 and bf16 inputs may be from 1e-30 to 1e35 in size: a run's sum has to be finite. A row that holds an
+ * infinity or NaN has no finite output. */
 int mmf_w4_linear(mmf_ctx* ctx, int w4_id, int dtype, const void* x, const float* xscales, int out_dtype, void* out,
                   size_t rows, size_t ldx, size_t ldo);
 

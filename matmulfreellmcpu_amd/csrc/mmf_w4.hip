@@ -56,41 +56,28 @@ typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 
 __device__ __forceinline__ uint32_t rotr(uint32_t w, int n) { return __builtin_amdgcn_alignbit(w, w, n); }
 
-// How a type's rows enter the matrix instructions. A code q is made a 16-bit float without a conversion:
-// its four bits are set into the mantissa of `base`, which makes it base + q, exact; base + z times the
-// sum of the inputs is taken off the group's sum again. int8 rows take the code itself.
+// The matrix operand of a word's 8 codes is q - z in every type, exact, so that a sum's roundings are those of its own
+// terms. (As base + q, with base + z times the sum of the inputs taken off the group's sum, one input 1e4 times the
+// others at weights of 0 left 1e-4 of the rest off, with a base of 128 for fp16 rows 1e-3; it is 1e-7 now.)
 template <int DT> struct Mat;
 template <> struct Mat<kBF16> {
-  static constexpr uint32_t bits = 0x41804180;  // 16: steps of 1/8, so a code sits at bits 3..6
-  static constexpr float base = 16.0f;
   using Acc = f32x4;
   static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  static constexpr uint32_t one = 0x3F803F80;
 };
 template <> struct Mat<kF16> {
-  static constexpr uint32_t bits = 0x58005800;  // 128: steps of 1/8
-  static constexpr float base = 128.0f;
   using Acc = f32x4;
   static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
-  static constexpr uint32_t one = 0x3C003C00;
 };
 template <> struct Mat<kI8> {
   using Acc = i32x4;
-  static constexpr uint32_t one = 0x01010101;
 };
 template <> struct Mat<kF32> : Mat<kBF16> {};  // three bf16 parts
 
-// The matrix operand of a word's 8 codes (16-bit floats), elements in order.
-template <int DT>
-__device__ __forceinline__ u32x4 w4_operand(uint32_t w) {
-  constexpr uint32_t m = 0x00780078, b = Mat<DT>::bits;
-  return u32x4{(w & m) | b, ((w >> 4) & m) | b, ((w >> 8) & m) | b, (rotr(w, 12) & m) | b};
-}
-// ... and as 8 bytes, elements 0 4 1 5 | 2 6 3 7; i8_operand puts the rows' bytes in that order.
+// A word's codes as 8 bytes, elements 0 4 1 5 | 2 6 3 7; i8_operand puts the rows' bytes in that order.
 __device__ __forceinline__ void w4_bytes(uint32_t w, uint32_t& lo, uint32_t& hi) {
   lo = (w >> 3) & 0x0F0F0F0F;
   hi = rotr(w, 7) & 0x0F0F0F0F;
@@ -99,21 +86,46 @@ __device__ __forceinline__ void i8_operand(uint32_t x0, uint32_t x1, uint32_t& l
   lo = __builtin_amdgcn_perm(x1, x0, 0x05010400);
   hi = __builtin_amdgcn_perm(x1, x0, 0x07030602);
 }
+// Four bytes: a code less its zero point, with b = 0x80 - z in each: their sum is at most 0x8F, so nothing carries.
+__device__ __forceinline__ uint32_t less_bytes(uint32_t a, uint32_t b) { return (a + b) ^ 0x80808080u; }
 
-// Pairs of fp16: a - b, exact for 128 + q and 128 + z.
-__device__ __forceinline__ u32x4 less(u32x4 a, uint32_t b) {
-  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// The zero point of a scale's word (above the scale) in the form that an operand takes it in: 128 + z twice, or
+// 0x80 - z four times.
+template <int DT> __device__ __forceinline__ uint32_t zero_of(uint32_t scale) {
+  if constexpr (DT == kF16) return 0x58005800u + (__builtin_amdgcn_perm(0u, scale, 0x0C020C02) << 3);
+  return 0x80808080u - __builtin_amdgcn_perm(0u, scale, 0x02020202);
+}
+// The operand of a word's 8 codes, elements in order.
+//   fp16: a code's four bits are set into the mantissa of 128 (steps of 1/8: bits 3..6), which makes it 128 + q
+//     without a conversion, and 128 + z comes off: all exact.
+//   bf16: bytes q - z, converted (an integer below 16 has few bits). bf16 has no subtraction of pairs here.
+template <int DT>
+__device__ __forceinline__ u32x4 operand(uint32_t w, uint32_t zero) {
   u32x4 r;
+  if constexpr (DT == kF16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    constexpr uint32_t m = 0x00780078, b = 0x58005800;
+    const u32x4 q = {(w & m) | b, ((w >> 4) & m) | b, ((w >> 8) & m) | b, (rotr(w, 12) & m) | b};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t v = a[i];  // (a bit_cast of the element itself takes element 0)
-    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - __builtin_bit_cast(f16x2, b));
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = q[i];  // (a bit_cast of the element itself takes element 0)
+      r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - __builtin_bit_cast(f16x2, zero));
+    }
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    uint32_t lo, hi;
+    w4_bytes(w, lo, hi);
+    lo = less_bytes(lo, zero);
+    hi = less_bytes(hi, zero);
+    auto at = [](uint32_t v, int i) { return static_cast<float>(static_cast<int8_t>(v >> (8 * i))); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = i & 1 ? hi : lo;
+      r[i] = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(at(v, i >> 1)), static_cast<__bf16>(at(v, 2 + (i >> 1)))});
+    }
   }
   return r;
 }
-
-// Four bytes: a code less its zero point, with b = 0x80 - z in each: their sum is at most 0x8F, so nothing carries.
-__device__ __forceinline__ uint32_t less_bytes(uint32_t a, uint32_t b) { return (a + b) ^ 0x80808080u; }
 
 // A lane's load of a row of 16-bit elements or bytes: the V elements from k on (16 bytes, or 8), zeros behind K.
 template <int DT, int STEP>
@@ -136,15 +148,13 @@ __device__ __forceinline__ auto row_load(const char* row, int k, int K, bool who
 // Many rows, and fp32 rows from a line on, are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
 // FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
 // l % 16; zeros behind the last row and input. Beside them stands, for fp32 and bf16, a number for each row and
-// scale's inputs, [tile][chunk][S][16]:
-//   fp32 rows are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of fp32, with 2^k
-//     bringing the largest of a scale's inputs below 2^15; the number is 2^-k (NaN where an input is none);
-//   bf16 rows are as they are, and it is the sum of the inputs;
-//   fp16 and int8 rows are as they are.
-// fp16 and int8 operands take the codes with the zero point off: 128 + q and 128 + z are exact, and so is q - z.
+// scale's inputs, [tile][chunk][S][16]. fp16 and int8 rows are as they are; the others are fp16 parts of x 2^k, with
+// 2^k bringing the largest of a scale's inputs below 2^15, and the number is 2^-k (NaN where an input is none):
+//   fp32 rows are two parts, the sum of which is x 2^k to half a step of fp32;
+//   bf16 rows are one, exact but for inputs below 2^-31 of the largest, which are off by 2^-40 of it at most.
 template <int DT> constexpr int kParts = DT == kF32 ? 2 : 1;
 template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
-template <int DT> constexpr int kOperand = DT == kF32 ? kF16 : DT;
+template <int DT> constexpr int kOperand = DT == kI8 ? kI8 : kF16;
 
 // One block a tile and chunk; 16 lanes a row, 8 inputs a thread.
 template <int DT, int STEP>
@@ -159,13 +169,13 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
   const int h = j >> 1;
   char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
   constexpr int U = STEP / 8;  // neighbouring threads that share a scale
-  if constexpr (DT == kF32) {
+  if constexpr (w4_numbers(DT)) {
     float v[8];
     uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN are the largest
-    const float* x = static_cast<const float*>(a.x) + row * a.ldx + k;
+    const typename Elem<DT>::T* x = static_cast<const typename Elem<DT>::T*>(a.x) + row * a.ldx + k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = in && k + i < g.K ? x[i] : 0.0f;
+      v[i] = in && k + i < g.K ? Elem<DT>::up(x[i]) : 0.0f;
       top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
     }
 #pragma unroll
@@ -181,13 +191,13 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
         const float y = v[2 * i + m] * f;
         const _Float16 p = static_cast<_Float16>(y);
         h[m] = __builtin_bit_cast(uint16_t, p);
-        l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
+        if (P == 2) l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
       }
       hi[i] = h[0] | h[1] << 16;
-      lo[i] = l[0] | l[1] << 16;
+      if (P == 2) lo[i] = l[0] | l[1] << 16;
     }
     *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = hi;
-    *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
+    if (P == 2) *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
     if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = e == 255 ? 0x7FC00000u : (254 - up) << 23;
   } else if constexpr (DT == kI8) {
     uint32_t x0 = 0, x1 = 0;
@@ -204,40 +214,35 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
     o[1] = hi;
   } else {
     u32x4 o = {0, 0, 0, 0};
-    float sum = 0.0f;
     const uint16_t* x = static_cast<const uint16_t*>(a.x) + row * a.ldx + k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint16_t e = in && k + i < g.K ? x[i] : static_cast<uint16_t>(0);
-      if constexpr (DT == kBF16) sum += Elem<DT>::up(e);
       o[i / 2] |= static_cast<uint32_t>(e) << (16 * (i & 1));
     }
     *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = o;
-    if constexpr (DT == kBF16) {
-#pragma unroll
-      for (int n = 1; n < U; n *= 2) sum += __shfl_xor(sum, n);
-      if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = __builtin_bit_cast(uint32_t, sum);
-    }
   }
 }
 
 // ---- few rows -------------------------------------------------------------------------------------
-// Few rows: one pass over the weights, bound by reading them (1 x 2048 x 11264, 12 MB: 5.4 us; 1 x 6912 x 2560
-// 5.5 us; int8 64 x 2048 x 2048 4.7). A block's waves split the chunks of NT
-// tiles of 16 outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix
-// operand's place and multiplies it with CT column tiles. A column is a row, or for fp32 rows one of a row's
-// three bf16 parts (hi + mid + lo = x exactly), 5 rows a tile: a wave cuts its chunk's rows into parts
-// once, in LDS of its own; or (LAID) a column is a row, of laid out parts. The waves' sums meet in LDS in one
-// fixed order.
+// Few rows: one pass over the weights, bound by a launch, their loads' way and the operands' making (1 x 2048 x 11264,
+// 12 MB: 5.8 us; 1 x 6912 x 2560 6.0; int8 64 x 2048 x 2048 4.7). A block's waves split the chunks of NT tiles of 16
+// outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix operand's place and
+// multiplies it with CT tiles of rows. fp32 rows are three bf16 parts each (hi + mid + lo = x exactly), 5 rows a
+// tile: a wave cuts its chunk's rows into parts once, in LDS of its own, the next chunk's in flight; or (LAID) they
+// were laid out, 16 a tile. The rows are the instruction's first operand, so that a lane's sums are of one output and
+// its scale and zero point one word (four words a lane spilled registers with scales for 32 inputs: bf16 108 x 2048 x
+// 11264 46 us, 31 now). The waves' sums meet in LDS in one fixed order.
 template <int DT, bool LAID> constexpr int kTileRows = DT == kF32 && !LAID ? 5 : 16;
-constexpr int kPartStride = 272;  // bytes of a column's 128 parts in LDS, 16 apart in banks
+constexpr int kPartStride = 272;  // bytes of a part's 128 inputs in LDS, 16 apart in banks
 template <int DT, int CT, bool LAID> constexpr int kPartBytes = DT == kF32 && !LAID ? CT * 15 * kPartStride : 0;
 
 template <int DT, int STEP, int NT, int CT, bool LAID>
 __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4_rows(
     W4Args a, W4Geom g, const uint32_t* codes, const uint32_t* scales, const char* frags, const uint32_t* sums, int row_tiles) {
   static_assert(!LAID || DT == kF32, "other rows are read as they are");
-  using M = Mat<LAID ? kF16 : DT>;
+  constexpr int OT = LAID ? kF16 : DT;
+  using M = Mat<OT>;
   using Acc = typename M::Acc;
   constexpr int S = 128 / STEP, R = kTileRows<DT, LAID>;
   extern __shared__ __align__(16) char lds[];
@@ -249,7 +254,7 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
   const char* x0 = static_cast<const char*>(a.x) + static_cast<size_t>(row0) * a.ldx * es;
   char* part = lds + wave * kPartBytes<DT, CT, LAID>;
 
-  const char* xr[CT];  // this lane's row of each column tile (a row past the end repeats the last one)
+  const char* xr[CT];  // this lane's row of each tile of rows (a row past the end repeats the last one)
 #pragma unroll
   for (int t = 0; t < CT; ++t) xr[t] = x0 + static_cast<size_t>(min(t * R + (DT == kF32 ? 0 : col), rows - 1)) * a.ldx * es;
   const uint32_t* cw[NT];
@@ -258,21 +263,19 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
   for (int n = 0; n < NT; ++n) {
     const size_t tile = min(tile0 + n, g.nt - 1);
     cw[n] = codes + tile * g.nc * 256 + lane * 4;
-    sw[n] = scales + tile * g.ns * 16 + q * 4;
+    sw[n] = scales + tile * g.ns * 16 + col;
   }
 
-  // LAID: this lane's place in each tile's fragments and numbers, and its operand's outputs' scales
+  // LAID: this lane's place in each tile's fragments and numbers
   const char* fr[CT];
-  const uint32_t *num[CT], *zw[NT];
+  const uint32_t* num[CT];
   if constexpr (LAID) {
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       const size_t rt = min(static_cast<int>(blockIdx.y) * CT + t, row_tiles - 1);
       fr[t] = frags + rt * g.nc * 8192 + lane * 16;
-      num[t] = sums + rt * g.ns * 16 + col;
+      num[t] = sums + rt * g.ns * 16 + 4 * q;
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) zw[n] = sw[n] - q * 4 + col;
   }
 
   f32x4 acc[NT][CT];
@@ -281,20 +284,44 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
 #pragma unroll
     for (int t = 0; t < CT; ++t) acc[n][t] = f32x4{0, 0, 0, 0};
 
-  u32x4 w[NT], sz[NT][S];
+  u32x4 w[NT];
+  uint32_t sz[NT][S];
   auto fetch = [&](int c) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       w[n] = *reinterpret_cast<const u32x4*>(cw[n] + static_cast<size_t>(c) * 256);
 #pragma unroll
-      for (int s = 0; s < S; ++s) sz[n][s] = *reinterpret_cast<const u32x4*>(sw[n] + (static_cast<size_t>(c) * S + s) * 16);
+      for (int s = 0; s < S; ++s) sz[n][s] = sw[n][(static_cast<size_t>(c) * S + s) * 16];
+    }
+  };
+  // fp32: two neighbours a lane of each row
+  constexpr int kHeld = DT == kF32 && !LAID ? CT * R : 1;
+  f32x2u held_x[kHeld];
+  auto fetch_rows = [&](int c) {
+    if constexpr (DT == kF32 && !LAID) {
+      const int k = c * 128 + 2 * lane;
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r) {
+        if (r >= rows) break;
+        const float* p = reinterpret_cast<const float*>(x0) + r * a.ldx + k;
+        if ((c + 1) * 128 <= g.K) {
+          held_x[r] = *reinterpret_cast<const f32x2u*>(p);
+        } else {
+          held_x[r].x = k < g.K ? p[0] : 0.0f;
+          held_x[r].y = k + 1 < g.K ? p[1] : 0.0f;
+        }
+      }
     }
   };
   int c = wave;
-  if (c < g.nc) fetch(c);
+  if (c < g.nc) {
+    fetch_rows(c);
+    fetch(c);
+  }
   for (; c < g.nc; c += waves) {
     const bool whole = (c + 1) * 128 <= g.K;
-    u32x4 cur[NT], csz[NT][S];
+    u32x4 cur[NT];
+    uint32_t csz[NT][S];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       cur[n] = w[n];
@@ -304,35 +331,20 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
     // the rows' operands of this chunk
     constexpr int P = LAID ? 2 : 1;
     u32x4 b[CT][4 * P];
-    uint32_t x[CT][S], z[NT][S];
+    u32x4 x[CT][S];
     if constexpr (LAID) {  // [half][part][word of the half]
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) b[t][j] = *reinterpret_cast<const u32x4*>(fr[t] + (static_cast<size_t>(c) * 8 + j) * 1024);
 #pragma unroll
-        for (int s = 0; s < S; ++s) x[t][s] = num[t][(static_cast<size_t>(c) * S + s) * 16];
+        for (int s = 0; s < S; ++s) x[t][s] = *reinterpret_cast<const u32x4*>(num[t] + (static_cast<size_t>(c) * S + s) * 16);
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const uint32_t v = zw[n][(static_cast<size_t>(c) * S + s) * 16] >> 16;
-          z[n][s] = M::bits + (v << 3 | v << 19);
-        }
     } else if constexpr (DT == kF32) {
-      for (int r = 0; r < rows; ++r) {  // two neighbours a lane, three parts each
-        const float* p = reinterpret_cast<const float*>(x0) + r * a.ldx + c * 128 + 2 * lane;
-        const int k = c * 128 + 2 * lane;
-        float v[2];
-        if (whole) {
-          const f32x2u u = *reinterpret_cast<const f32x2u*>(p);
-          v[0] = u.x;
-          v[1] = u.y;
-        } else {
-          v[0] = k < g.K ? p[0] : 0.0f;
-          v[1] = k + 1 < g.K ? p[1] : 0.0f;
-        }
+#pragma unroll
+      for (int r = 0; r < kHeld; ++r) {  // three parts each
+        if (r >= rows) break;
+        const float v[2] = {held_x[r].x, held_x[r].y};
         uint32_t h[2], m[2], l[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // cut off, not rounded: each part is exact, and what is left is too
@@ -377,11 +389,14 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
 #pragma unroll
         for (int j = 0; j < 4; ++j) b[t][j] = row_load<DT, STEP>(xr[t], c * 128 + w4_k(STEP, j, q), g.K, whole);
     }
-    if (c + waves < g.nc) fetch(c + waves);
+    if (c + waves < g.nc) {
+      fetch_rows(c + waves);
+      fetch(c + waves);
+    }
 
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      // sums of this scale's inputs: the codes' products, and the inputs themselves
+      // sums of this scale's inputs: the products, and for int8 (whose zero points come off here) the inputs themselves
       Acc d[NT][CT], sum[CT];
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
@@ -390,19 +405,19 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
         for (int n = 0; n < NT; ++n) d[n][t] = Acc{};
       }
       if constexpr (DT == kI8) {
-        constexpr uint32_t one = M::one;
+        constexpr uint32_t one = 0x01010101;
         if constexpr (STEP == 32) {  // one word a scale: 32 inputs an instruction
           const int j = s;
 #pragma unroll
           for (int t = 0; t < CT; ++t) {
             const long bx = (j & 1) ? (static_cast<long>(b[t][j / 2].w) << 32 | b[t][j / 2].z)
                                     : (static_cast<long>(b[t][j / 2].y) << 32 | b[t][j / 2].x);
-            sum[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(static_cast<long>(one) << 32 | one, bx, sum[t], 0, 0, 0);
+            sum[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(bx, static_cast<long>(one) << 32 | one, sum[t], 0, 0, 0);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               uint32_t lo, hi;
               w4_bytes(cur[n][j], lo, hi);
-              d[n][t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(static_cast<long>(hi) << 32 | lo, bx, d[n][t], 0, 0, 0);
+              d[n][t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(bx, static_cast<long>(hi) << 32 | lo, d[n][t], 0, 0, 0);
             }
           }
         } else {
@@ -420,58 +435,46 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
               const i32x4 bx = __builtin_bit_cast(i32x4, b[t][j]);
-              sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, u32x4{one, one, one, one}), bx,
+              sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bx, __builtin_bit_cast(i32x4, u32x4{one, one, one, one}),
                                                              sum[t], 0, 0, 0);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw[n], bx, d[n][t], 0, 0, 0);
+              for (int n = 0; n < NT; ++n) d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bx, aw[n], d[n][t], 0, 0, 0);
             }
           }
         }
       } else {
-        constexpr uint32_t one = M::one;
 #pragma unroll
         for (int jj = 0; jj < 4 / S; ++jj) {
           const int j = s * (4 / S) + jj;
           u32x4 aw[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            aw[n] = w4_operand<LAID ? kF16 : DT>(cur[n][j]);
-            if constexpr (LAID) aw[n] = less(aw[n], z[n][s]);
-          }
+          for (int n = 0; n < NT; ++n) aw[n] = operand<OT>(cur[n][j], zero_of<OT>(csz[n][s]));
 #pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            if constexpr (LAID) {
+          for (int t = 0; t < CT; ++t)
 #pragma unroll
-              for (int p = 0; p < P; ++p)
+            for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) d[n][t] = M::mul(aw[n], b[t][(j >> 1) * 4 + p * 2 + (j & 1)], d[n][t]);
-              continue;
-            }
-            sum[t] = M::mul(u32x4{one, one, one, one}, b[t][j], sum[t]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) d[n][t] = M::mul(aw[n], b[t][j], d[n][t]);
-          }
+              for (int n = 0; n < NT; ++n)
+                d[n][t] = M::mul(b[t][LAID ? (j >> 1) * 4 + p * 2 + (j & 1) : j], aw[n], d[n][t]);
         }
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {  // rows 4 q + i of each tile, output `col`
+        const uint32_t v = csz[n][s];
+        const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // output 4 q + i of the tile
-          const uint32_t v = csz[n][s][i];
-          const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v)));
+        for (int t = 0; t < CT; ++t)
 #pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            if constexpr (DT == kI8) {
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == kI8)
               acc[n][t][i] = __builtin_fmaf(sc, static_cast<float>(d[n][t][i] - __mul24(static_cast<int>(v >> 16), sum[t][i])),
                                             acc[n][t][i]);
-            } else if constexpr (LAID) {
-              acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(float, x[t][s]), acc[n][t][i]);
-            } else {
-              const float off = static_cast<float>(v >> 16) + M::base;
-              acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-off, sum[t][i], d[n][t][i]), acc[n][t][i]);
-            }
+            else if constexpr (LAID)
+              acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(f32x4, x[t][s])[i], acc[n][t][i]);
+            else
+              acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i], acc[n][t][i]);
           }
-        }
+      }
     }
   }
 
@@ -487,15 +490,16 @@ __global__ __launch_bounds__(CT == 1 && NT == 1 && !LAID ? 1024 : 512) void k_w4
   for (int i = threadIdx.x; i < NT * 16 * rows; i += blockDim.x) {
     const int n = i % (NT * 16), r = i / (NT * 16), t = r / R;
     if (tile0 * 16 + n >= g.N) continue;
-    const int at = (((n / 16) * CT + t) * 64 + (n % 16 / 4) * 16) * 4 + n % 4;
+    const int at = (((n / 16) * CT + t) * 64 + n % 16) * 4;
+    auto of = [](int row) { return row / 4 * 64 + row % 4; };  // of a tile
     float v = 0.0f;
     for (int wv = 0; wv < waves; ++wv) {
       const float* p = held + wv * (NT * CT * 256) + at;
       if constexpr (DT == kF32 && !LAID) {
         const int c0 = r % 5 * 3;  // the small parts first
-        v += (p[(c0 + 2) * 4] + p[(c0 + 1) * 4]) + p[c0 * 4];
+        v += (p[of(c0 + 2)] + p[of(c0 + 1)]) + p[of(c0)];
       } else {
-        v += p[r % 16 * 4];
+        v += p[of(r % 16)];
       }
     }
     if constexpr (DT == kI8) v *= a.xscales[row0 + r];
@@ -507,7 +511,7 @@ template <int DT, int STEP, int NT, int CT, bool LAID = false>
 hipError_t rows_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, int waves,
                        hipStream_t s, const char* frags = nullptr, const uint32_t* sums = nullptr) {
   const size_t part = static_cast<size_t>(waves) * kPartBytes<DT, CT, LAID>, red = static_cast<size_t>(waves) * NT * CT * 1024;
-  const size_t lds = part > red ? part : red;  // at most 64 KB: 16 waves of one column tile, 8 of two
+  const size_t lds = part > red ? part : red;  // at most 64 KB: 16 waves of one tile of rows, 8 of two
   const unsigned per = CT * kTileRows<DT, LAID>;
   k_w4_rows<DT, STEP, NT, CT, LAID>
       <<<dim3((g.nt + NT - 1) / NT, static_cast<unsigned>((a.rows + per - 1) / per)), waves * 64, lds, s>>>(
@@ -516,13 +520,13 @@ hipError_t rows_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
 }
 
 // Tiles of outputs a wave (nt) and waves a block. `units` is the tiles of outputs times the groups of rows.
-// One column tile: a wave a tile; 16 waves where the inputs are long (us: 1 x 6912 x 2560 fp32 6.6 by 8 waves,
+// One tile of rows: a wave a tile of outputs; 16 waves where the inputs are long (us: 1 x 6912 x 2560 fp32 6.6 by 8 waves,
 // 5.4 by 16; 1 x 2048 x 11264 5.2 and 6.8). Many rows of one tile share the rows' operands over four tiles of
 // outputs instead where there are enough of these (bf16 16 x 2048 x 11264 8.8 -> 6.9).
-// Two column tiles: the rows' operands are most of what is read, so a wave takes as many tiles of outputs as leave
+// Two tiles of rows: the rows' operands are most of what is read, so a wave takes as many tiles of outputs as leave
 // the chip full, and fewer waves share a block when there are more of them (bf16, one tile -> chosen: 64 x 6912 x
 // 2560 28.1 -> 17.7, 128 x 6912 x 2560 41 -> 21, 128 x 2048 x 11264 45 -> 23). fp32 rows, whose parts are made
-// anew for each column tile, take two at most.
+// anew for each of these, take two at most.
 template <int DT, int STEP>
 hipError_t rows_pick(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s) {
   constexpr size_t R = kTileRows<DT, false>;
@@ -680,20 +684,12 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
       const uint32_t* sc_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + 4 * q;
       const uint32_t* x_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + WN * 4 * S * 16 + (lane & 15);
 
-      // the zero points of this lane's outputs of the operand (lane % 16 of each tile), for less() or less_bytes()
+      // the zero points of this lane's outputs of the operand (lane % 16 of each tile)
       uint32_t zero[4];
       auto zeros = [&](int s) {
-        if constexpr (OT != kBF16) {
-          const uint32_t* z_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + (lane & 15);
+        const uint32_t* z_at = reinterpret_cast<const uint32_t*>(buf + pieces * 1024) + in * 4 * S * 16 + (lane & 15);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const uint32_t z = z_at[(n * S + s) * 16] >> 16;
-            if constexpr (OT == kI8)
-              zero[n] = 0x80808080u - z * 0x01010101u;
-            else
-              zero[n] = M::bits + (z << 3 | z << 19);
-          }
-        }
+        for (int n = 0; n < 4; ++n) zero[n] = zero_of<OT>(z_at[(n * S + s) * 16]);
       };
       auto clear = [&] {
 #pragma unroll
@@ -714,14 +710,10 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
             const float sc = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sz[i])));
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-              if constexpr (DT == kF32) {
+              if constexpr (kNumbers)
                 acc[n][t][i] = __builtin_fmaf(sc, d[n][t][i] * __builtin_bit_cast(float, x[t]), acc[n][t][i]);
-              } else if constexpr (!kNumbers) {
+              else
                 acc[n][t][i] = __builtin_fmaf(sc, static_cast<float>(d[n][t][i]), acc[n][t][i]);
-              } else {
-                const float z = static_cast<float>(sz[i] >> 16) + M::base;
-                acc[n][t][i] = __builtin_fmaf(sc, __builtin_fmaf(-z, __builtin_bit_cast(float, x[t]), d[n][t][i]), acc[n][t][i]);
-              }
             }
           }
         }
@@ -775,10 +767,7 @@ __global__ __launch_bounds__(512) void k_w4_gemm(W4Args a, W4Geom g, const uint3
             if (STEP == 32) clear(), zeros(2 * half + jj);
             u32x4 aw[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              aw[n] = w4_operand<OT>(w[n][2 * half + jj]);
-              if constexpr (OT == kF16) aw[n] = less(aw[n], zero[n]);
-            }
+            for (int n = 0; n < 4; ++n) aw[n] = operand<OT>(w[n][2 * half + jj], zero[n]);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
               u32x4 b[TT];

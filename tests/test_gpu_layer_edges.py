@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_layer import F32, FLOATS, I8, run_norm, run_w4
+from test_gpu_layer import BF16, F16, F32, FLOATS, I8, U, W4, Rows, coded, out_rows, run_norm, run_w4, value
 from test_gpu_parity import eng  # noqa: F401  (module fixture)
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +46,53 @@ def test_w4_groups_beyond_the_row(eng):  # noqa: F811
             run_w4(eng, rng, t, 3, 77, 21, group, zeros=True)
     with pytest.raises(ValueError, match="negative"):
         eng.register_w4(np.zeros((4, 10), np.uint8), np.zeros((4, 0), np.float16), K=20, group=-32)
+
+
+def way(t, rows, K, N):
+    """The kernel of a product (w4_way): of few rows, of few rows laid out, by tiles of many."""
+    work = rows * K * N
+    if rows > 16 and work > (1.6e9 if t == F32 else 2.5e9):
+        return "tiles"
+    return "laid" if t == F32 and rows > 5 and work > 0.15e9 else "few"
+
+
+WAYS = [(F32, "few", 1, 2048, 700), (F32, "few", 12, 1031, 700), (F32, "laid", 16, 2048, 8192), (F32, "laid", 20, 2048, 8192),
+        (F32, "tiles", 90, 4100, 8001), (BF16, "few", 3, 2048, 700), (BF16, "few", 40, 1031, 700), (BF16, "tiles", 90, 4100, 8001),
+        (F16, "few", 3, 2048, 700), (F16, "few", 40, 1031, 700), (F16, "tiles", 130, 1600, 13000)]
+
+
+def product(eng, w, t, x):  # noqa: F811
+    """(fp32 outputs of the rows x, which are in t's storage, the exact ones, sums of the terms' magnitudes)."""
+    rows, K = x.shape
+    X, O = Rows(eng, x, t), out_rows(eng, (rows, w.w.shape[0]), F32)
+    eng.w4_linear(w.id, X.ptr, O.ptr, rows, dtype=t, out_dtype=F32)
+    eng.sync()
+    xv = value(x, t).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        return O.get(), xv @ w.w.T, np.abs(xv) @ np.abs(w.w).T
+
+
+@pytest.mark.parametrize("t,how,rows,K,N", WAYS)
+@pytest.mark.parametrize("group", [32, 64, 128, 0])
+def test_w4_large_input_at_weights_of_zero(eng, t, how, rows, K, N, group):  # noqa: F811
+    """An input 1e4 times the others that meets weights of 0 leaves the others' sum alone: an output is off by the
+    roundings of its own terms. These are U of partial sums below the sum of magnitudes: at most 4 * 6 inside a
+    chunk's matrix instructions, of a chunk's share, and one for each scale. Independent, for 4100 inputs with a scale
+    for 32: sqrt(129 + 24 / 33) / sqrt(3) = 7 U at one standard deviation if each partial sum were the whole sum.
+    fp32 rows in two parts add U for each input, and 2^-40 * 1e4 / 0.8 < 0.2 U of the others."""
+    assert way(t, rows, K, N) == how
+    print(f"zero weights t={t} {how} rows={rows} K={K} N={N} group={group}", flush=True)
+    rng = np.random.default_rng(rows + K + group)
+    w = W4(eng, rng, N, K, group, True)
+    eng.w4_release(w.id)
+    size = group or K
+    for k in (5, K - 1):
+        w.q[:, k] = w.z[:, k // size]
+        w.w[:, k] = 0
+    q = np.concatenate([w.q, np.zeros((N, K % 2), np.uint8)], 1)
+    w.id = eng.register_w4(q[:, 0::2] | (q[:, 1::2] << 4), w.s, w.z, K=K, group=group)
+    x = rng.standard_normal((rows, K))
+    x[:, 5], x[:, K - 1] = 1e4, -2e4
+    got, want, mag = product(eng, w, t, coded(x, t))
+    assert (np.abs(got - want) <= 17 * U * mag).all(), (np.abs(got - want) / (U * mag)).max()
+    eng.w4_release(w.id)
