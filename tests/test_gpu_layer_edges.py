@@ -96,3 +96,57 @@ def test_w4_large_input_at_weights_of_zero(eng, t, how, rows, K, N, group):  # n
     got, want, mag = product(eng, w, t, coded(x, t))
     assert (np.abs(got - want) <= 17 * U * mag).all(), (np.abs(got - want) / (U * mag)).max()
     eng.w4_release(w.id)
+
+
+@pytest.mark.parametrize("t,how,rows,K,N", [c for c in WAYS if c[0] != F16])
+@pytest.mark.parametrize("group", [32, 128])
+def test_w4_ranges_by_kernel(eng, t, how, rows, K, N, group):  # noqa: F811
+    """Rows from 1e-30 to 1e30 keep their digits, and so do inputs of one row that lie far apart, down to 2^-40 of the
+    largest of their run's group; rows of 1e35 throughout stay finite. Bounds as above."""
+    assert way(t, rows, K, N) == how
+    print(f"ranges t={t} {how} rows={rows} K={K} N={N} group={group}", flush=True)
+    rng = np.random.default_rng(rows + group)
+    w = W4(eng, rng, N, K, group, True)
+    x = rng.standard_normal((rows, K)) * 10.0 ** np.linspace(-28, 30, rows)[:, None]
+    got, want, mag = product(eng, w, t, coded(x, t))
+    assert (np.abs(got - want) <= 17 * U * mag).all(), (np.abs(got - want) / (U * mag)).max(1)
+    x = rng.standard_normal((rows, K)) * 2.0 ** rng.integers(-45, 1, (rows, K))
+    got, want, mag = product(eng, w, t, coded(x, t))
+    # (the largest input of any run is below 2^3)
+    assert (np.abs(got - want) <= 17 * U * mag + 2.0 ** -37 * np.abs(w.w).sum(1)).all()
+    x = np.full((rows, K), 1e35) * rng.choice([-1, 1], (rows, 1))
+    got, want, mag = product(eng, w, t, coded(x, t))
+    over = np.abs(want) > 3e38  # an output beyond fp32
+    assert (np.abs(got - want)[~over] <= (17 * U * mag)[~over]).all()
+    eng.w4_release(w.id)
+
+
+@pytest.mark.parametrize("t,how,rows,K,N", WAYS)
+def test_w4_rows_without_a_number(eng, t, how, rows, K, N):  # noqa: F811
+    """A row with an infinity or NaN has no finite output, wherever it stands, and the other rows keep their bits."""
+    assert way(t, rows, K, N) == how
+    print(f"infinities t={t} {how} rows={rows} K={K} N={N}", flush=True)
+    rng = np.random.default_rng(rows)
+    w = W4(eng, rng, N, K, 64, True)
+    x = rng.standard_normal((rows, K))
+    got, _, _ = product(eng, w, t, coded(x, t))
+    hurt = sorted({0, rows // 2, rows - 1})
+    for r, v in zip(hurt, (np.inf, np.nan, -np.inf)):
+        x[r, (7 * r + 3) % K if r else K - 1] = v
+    again, _, _ = product(eng, w, t, coded(x, t))
+    assert not np.isfinite(again[hurt]).any()
+    keep = np.setdiff1d(np.arange(rows), hurt)
+    assert (again[keep] == got[keep]).all()
+    eng.w4_release(w.id)
+
+
+@pytest.mark.parametrize("how,rows,K,N", [c[1:] for c in WAYS if c[0] == F16])
+def test_w4_fp16_range(eng, how, rows, K, N):  # noqa: F811
+    """fp16 rows below fp16's normal range and at its largest values."""
+    assert way(F16, rows, K, N) == how
+    rng = np.random.default_rng(rows)
+    w = W4(eng, rng, N, K, 64, True)
+    for x in (rng.integers(-8, 9, (rows, K)) * 2.0 ** -24, rng.choice([-65504.0, 65504.0], (rows, K)), np.full((rows, K), 65504.0)):
+        got, want, mag = product(eng, w, F16, coded(x, F16))
+        assert (np.abs(got - want) <= 17 * U * mag).all()
+    eng.w4_release(w.id)
