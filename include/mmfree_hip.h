@@ -187,10 +187,9 @@ int mmf_w4_release(mmf_ctx* ctx, int w4_id);
  * of mmf_add_rmsnorm_q8. out is of out_dtype (a float type). The weights enter every sum as the integers they
  * are, with no rounding. Sums are taken over runs of 32, 64 or 128 inputs (the largest of these that divides the
  * group; 128 where a row is one group), in fp32 and for int8 x in exact integers, and each is multiplied by its scale
- * and added in fp32: an output's error is that of fp32 sums of its own terms. In large products fp32 rows count
- * to half a step of fp32, and fp32 and bf16 inputs to no less than 2^-40 of the largest input of their run's
- * group. fp32 and bf16 inputs may be from 1e-30 to 1e35 in size: a run's sum has to be finite. A row that holds an
- * infinity or NaN has no finite output. */
+ * and added in fp32: an output's error is that of fp32 sums of its own terms. In large products fp32 inputs count to
+ * half a step of fp32 or 2^-40 of the run's largest. fp32 and bf16 inputs may be from 1e-30 to 1e35 in size: a run's
+ * sum has to be finite. A row that holds an infinity or NaN has no finite output. */
 int mmf_w4_linear(mmf_ctx* ctx, int w4_id, int dtype, const void* x, const float* xscales, int out_dtype, void* out,
                   size_t rows, size_t ldx, size_t ldo);
 

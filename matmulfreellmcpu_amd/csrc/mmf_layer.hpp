@@ -129,8 +129,7 @@ inline NormPlan norm_plan(int dtype, size_t rows, size_t cols) {
 // ---- products with 4-bit weights ----------------------------------------------------------------
 // Weights laid out for the kernels. Outputs go in tiles of 16 and inputs in chunks of 128, padded:
 //   codes [ntile][chunk][lane 0..63][word 0..3]: lane l holds output 16 ntile + l % 16, and word j
-//     the 8 inputs from 128 chunk + w4_k(step, j, l / 16). Element e of a word sits at bits
-//     3 + 4 w4_nibble(e) (rotated by 3, so that one AND and one OR make two 16-bit floats of it).
+//     the 8 inputs from 128 chunk + w4_k(step, j, l / 16). Element e of a word is its nibble w4_nibble(e).
 //   scales [ntile][w4_subs * nchunk][16]: the fp16 scale in the low half, the zero point above it.
 // step is the kernel's scale granularity, 32, 64 or 128 inputs: the largest that divides the group
 // (of rows that are one group: 128).
@@ -170,12 +169,12 @@ inline const char* check_w4(size_t N, size_t K, size_t group) {
 }
 
 // Many rows are laid out as matrix operands first (mmf_w4.hip): bytes of 16 rows' fragments (fp32: two fp16
-// parts), and with a number for each row and scale (fp32 and bf16); rows of a pass, so that these fit the workspace.
+// parts), and with a number for each row and scale (fp32); rows of a pass, so that these fit the workspace.
 constexpr size_t kLayerWsBytes = size_t{128} << 20;
 inline size_t w4_frag_bytes(int dtype, const W4Geom& g) {
   return static_cast<size_t>(g.nc) * 128 * 16 * (dtype == kF32 ? 4 : dtype == kI8 ? 1 : 2);
 }
-MMF_HD inline constexpr bool w4_numbers(int dtype) { return dtype == kF32 || dtype == kBF16; }
+MMF_HD inline constexpr bool w4_numbers(int dtype) { return dtype == kF32; }
 inline size_t w4_lay_bytes(int dtype, const W4Geom& g, int row_tiles) {  // fragments and numbers
   return row_tiles * (w4_frag_bytes(dtype, g) + (w4_numbers(dtype) ? static_cast<size_t>(g.ns) * 64 : 0));
 }
@@ -188,20 +187,18 @@ struct W4Plan {
 };
 // The plan of the least time by this count: a chunk of inputs of 64 x 64 outputs takes a SIMD `unit` us (fp32 2.2,
 // 16-bit 1.25, int8 0.9 with a scale for 128 inputs; more scalings with more scales), 1.3 times that where a compute unit
-// has fewer than 8 waves to overlap, and up to 1.3 times where fewer outputs share the rows' operands (bf16
-// with scales for 64 inputs also spills registers then: 566 x 1498 x 8555 62, as {4, 1, 1} 48); the
+// has fewer than 8 waves to overlap, and up to 1.3 times where fewer outputs share the rows' operands; the
 // fullest compute unit counts. Split inputs cost a launch and the partial sums, written and read at 4 TB/s.
 // Measured (us): fp32 2048 x 6912 x 2560 277 as {4, 1, 1} and 220 as {4, 1, 3}; 512 x 6912 x 2560 147 and 75 as
 // {2, 4, 1}; bf16 2048 x 2048 x 2048 39 and 33 as {4, 2, 1}; fp32 2048 x 2048 x 11264 191, as {4, 2, 1} 215.
 inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
   const double unit = (dtype == kF32 ? 2.2 : dtype == kI8 ? 0.9 : 1.25) * (g.step == 32 ? 1.8 : g.step == 64 ? 1.2 : 1.0);
-  const double spill = dtype == kBF16 && g.step == 64 ? 1.4 : 1.0;
   const int rows = (row_tiles + kW4TileRows / 16 - 1) / (kW4TileRows / 16);
   const double sums = row_tiles * 16.0 * g.nt * 16.0 * 4 * 2 / 4e6;  // us of one split's
   const struct {
     int wn, bk;
     double share;
-  } forms[] = {{4, 1, 1.0}, {4, 2, 1.0}, {2, 2, 1.15 * spill}, {2, 4, 1.3 * spill}};
+  } forms[] = {{4, 1, 1.0}, {4, 2, 1.0}, {2, 2, 1.15}, {2, 4, 1.3}};
   W4Plan best{4, 1, 1};
   double least = 0;
   for (const auto& f : forms)

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256) void k_w4_pack(const uint8_t* codes, W4Geom g,
     if (n < static_cast<size_t>(g.N) && k < g.K) q = (codes[n * ((g.K + 1) / 2) + k / 2] >> (4 * (k & 1))) & 15;
     w |= q << (4 * w4_nibble(e));
   }
-  out[i] = (w << 3) | (w >> 29);
+  out[i] = w;
 }
 
 __global__ __launch_bounds__(256) void k_w4_pack_scales(const uint16_t* scales, const uint8_t* zeros, W4Geom g,
@@ -54,8 +54,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 
-__device__ __forceinline__ uint32_t rotr(uint32_t w, int n) { return __builtin_amdgcn_alignbit(w, w, n); }
-
 // The matrix operand of a word's 8 codes is q - z in every type, exact, so that a sum's roundings are those of its own
 // terms. (As base + q, with base + z times the sum of the inputs taken off the group's sum, one input 1e4 times the
 // others at weights of 0 left 1e-4 of the rest off, with a base of 128 for fp16 rows 1e-3; it is 1e-7 now.)
@@ -79,8 +77,8 @@ template <> struct Mat<kF32> : Mat<kBF16> {};  // three bf16 parts
 
 // A word's codes as 8 bytes, elements 0 4 1 5 | 2 6 3 7; i8_operand puts the rows' bytes in that order.
 __device__ __forceinline__ void w4_bytes(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  lo = (w >> 3) & 0x0F0F0F0F;
-  hi = rotr(w, 7) & 0x0F0F0F0F;
+  lo = w & 0x0F0F0F0F;
+  hi = (w >> 4) & 0x0F0F0F0F;
 }
 __device__ __forceinline__ void i8_operand(uint32_t x0, uint32_t x1, uint32_t& lo, uint32_t& hi) {
   lo = __builtin_amdgcn_perm(x1, x0, 0x05010400);
@@ -89,23 +87,23 @@ __device__ __forceinline__ void i8_operand(uint32_t x0, uint32_t x1, uint32_t& l
 // Four bytes: a code less its zero point, with b = 0x80 - z in each: their sum is at most 0x8F, so nothing carries.
 __device__ __forceinline__ uint32_t less_bytes(uint32_t a, uint32_t b) { return (a + b) ^ 0x80808080u; }
 
-// The zero point of a scale's word (above the scale) in the form that an operand takes it in: 128 + z twice, or
+// The zero point of a scale's word (above the scale) in the form that an operand takes it in: 1024 + z twice, or
 // 0x80 - z four times.
 template <int DT> __device__ __forceinline__ uint32_t zero_of(uint32_t scale) {
-  if constexpr (DT == kF16) return 0x58005800u + (__builtin_amdgcn_perm(0u, scale, 0x0C020C02) << 3);
+  if constexpr (DT == kF16) return 0x64006400u + __builtin_amdgcn_perm(0u, scale, 0x0C020C02);
   return 0x80808080u - __builtin_amdgcn_perm(0u, scale, 0x02020202);
 }
 // The operand of a word's 8 codes, elements in order.
-//   fp16: a code's four bits are set into the mantissa of 128 (steps of 1/8: bits 3..6), which makes it 128 + q
-//     without a conversion, and 128 + z comes off: all exact.
+//   fp16: a code's four bits are set into the mantissa of 1024 (steps of 1: bits 0..3), which makes it 1024 + q
+//     without a conversion, and 1024 + z comes off: all exact.
 //   bf16: bytes q - z, converted (an integer below 16 has few bits). bf16 has no subtraction of pairs here.
 template <int DT>
 __device__ __forceinline__ u32x4 operand(uint32_t w, uint32_t zero) {
   u32x4 r;
   if constexpr (DT == kF16) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    constexpr uint32_t m = 0x00780078, b = 0x58005800;
-    const u32x4 q = {(w & m) | b, ((w >> 4) & m) | b, ((w >> 8) & m) | b, (rotr(w, 12) & m) | b};
+    constexpr uint32_t m = 0x000F000F, b = 0x64006400;
+    const u32x4 q = {(w & m) | b, ((w >> 4) & m) | b, ((w >> 8) & m) | b, ((w >> 12) & m) | b};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t v = q[i];  // (a bit_cast of the element itself takes element 0)
@@ -147,14 +145,13 @@ __device__ __forceinline__ auto row_load(const char* row, int k, int K, bool who
 // ---- rows laid out --------------------------------------------------------------------------------
 // Many rows, and fp32 rows from a line on, are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
 // FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
-// l % 16; zeros behind the last row and input. Beside them stands, for fp32 and bf16, a number for each row and
-// scale's inputs, [tile][chunk][S][16]. fp16 and int8 rows are as they are; the others are fp16 parts of x 2^k, with
-// 2^k bringing the largest of a scale's inputs below 2^15, and the number is 2^-k (NaN where an input is none):
-//   fp32 rows are two parts, the sum of which is x 2^k to half a step of fp32;
-//   bf16 rows are one, exact but for inputs below 2^-31 of the largest, which are off by 2^-40 of it at most.
+// l % 16; zeros behind the last row and input. Beside fp32 rows' stands a number for each row and
+// scale's inputs, [tile][chunk][S][16]: they are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of
+// fp32 (or to 2^-40 of the largest), with 2^k bringing the largest of a scale's inputs below 2^15; the number is 2^-k
+// (NaN where an input is none). Other rows are as they are.
 template <int DT> constexpr int kParts = DT == kF32 ? 2 : 1;
 template <int DT> constexpr int kFrags = DT == kI8 ? 1 : 2;  // of a half chunk and part
-template <int DT> constexpr int kOperand = DT == kI8 ? kI8 : kF16;
+template <int DT> constexpr int kOperand = DT == kF32 ? kF16 : DT;
 
 // One block a tile and chunk; 16 lanes a row, 8 inputs a thread.
 template <int DT, int STEP>
@@ -169,13 +166,13 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
   const int h = j >> 1;
   char* to = frags + (rt * g.nc + c) * (2 * P * FR * 1024) + h * (P * FR * 1024) + (16 * q + r) * 16;
   constexpr int U = STEP / 8;  // neighbouring threads that share a scale
-  if constexpr (w4_numbers(DT)) {
+  if constexpr (DT == kF32) {
     float v[8];
     uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN are the largest
-    const typename Elem<DT>::T* x = static_cast<const typename Elem<DT>::T*>(a.x) + row * a.ldx + k;
+    const float* x = static_cast<const float*>(a.x) + row * a.ldx + k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = in && k + i < g.K ? Elem<DT>::up(x[i]) : 0.0f;
+      v[i] = in && k + i < g.K ? x[i] : 0.0f;
       top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
     }
 #pragma unroll
@@ -191,13 +188,13 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
         const float y = v[2 * i + m] * f;
         const _Float16 p = static_cast<_Float16>(y);
         h[m] = __builtin_bit_cast(uint16_t, p);
-        if (P == 2) l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
+        l[m] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y - static_cast<float>(p)));
       }
       hi[i] = h[0] | h[1] << 16;
-      if (P == 2) lo[i] = l[0] | l[1] << 16;
+      lo[i] = l[0] | l[1] << 16;
     }
     *reinterpret_cast<u32x4*>(to + (j & 1) * 1024) = hi;
-    if (P == 2) *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
+    *reinterpret_cast<u32x4*>(to + (FR + (j & 1)) * 1024) = lo;
     if (u % U == 0) sums[((rt * g.nc + c) * S + u / U) * 16 + r] = e == 255 ? 0x7FC00000u : (254 - up) << 23;
   } else if constexpr (DT == kI8) {
     uint32_t x0 = 0, x1 = 0;
