@@ -24,10 +24,11 @@ __device__ __forceinline__ float softplus(float x) {
   return __builtin_fmaxf(x, 0.0f) + log1p_unit(exp2_fast(-1.44269504f * __builtin_fabsf(x)));
 }
 
-// A in powers of two; -infinity as the lowest finite value, so that a step of 0 has the decay 1 with it too.
+// A in powers of two; infinities as the outermost finite values, so that a step of 0 has the decay 1 with them too
+// (the steps that stand behind a sequence's end are such ones).
 __device__ __forceinline__ float log2_decay(float A) {
   A *= 1.44269504f;
-  return A < -3.4e38f ? -3.4e38f : A;
+  return A < -3.4e38f ? -3.4e38f : A > 3.4e38f ? 3.4e38f : A;
 }
 
 // A lane holds a channel's NS states in registers; a wave is 64 channels, and NW waves share a channel

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from test_gpu_layer import BF16, F16, F32, FLOATS, I8, U, W4, Rows, coded, out_rows, run_norm, run_w4, value
-from test_gpu_parity import eng  # noqa: F401  (module fixture)
+from test_gpu_parity import Dev, eng  # noqa: F401  (module fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +150,29 @@ def test_w4_fp16_range(eng, how, rows, K, N):  # noqa: F811
         got, want, mag = product(eng, w, F16, coded(x, F16))
         assert (np.abs(got - want) <= 17 * U * mag).all()
     eng.w4_release(w.id)
+
+
+# ---- selective scan ---------------------------------------------------------------------------
+
+
+def test_scan_growth_beyond_fp32(eng):  # noqa: F811
+    """A rate of +infinity, or one that grows past fp32, leaves its state infinite at every length, also where the last
+    group of steps is ragged; a NaN rate stays NaN, and other channels keep their numbers."""
+    rng = np.random.default_rng(17)
+    D, N = 70, 16
+    for T in (1, 2, 3, 4, 5, 31, 33, 69):
+        print(f"growth T={T}", flush=True)
+        u, dt = rng.standard_normal((T, D)).astype(np.float32), np.full((T, D), 0.5, np.float32)
+        B, Cm = (rng.standard_normal((T, N)).astype(np.float32) for _ in range(2))
+        A = -np.ones((D, N), np.float32)
+        A[3], A[9], A[20] = np.inf, 3e38, np.nan
+        d = {k: Dev(eng, v) for k, v in dict(u=u, dt=dt, B=B, C=Cm, A=A).items()}
+        S, O = Dev(eng, np.ones((1, N, D), np.float32)), Dev(eng, shape=(T, D))
+        eng.selective_scan(O.ptr, d["u"].ptr, d["dt"].ptr, d["A"].ptr, d["B"].ptr, d["C"].ptr, T, D, N, state=S.ptr,
+                           softplus=False)
+        eng.sync()
+        o, s = O.get(), S.get()[0]
+        assert (s[:, [3, 9]] == np.inf).all() and not np.isfinite(o[:, [3, 9]]).any()
+        assert np.isnan(s[:, 20]).all() and np.isnan(o[:, 20]).all()
+        others = np.setdiff1d(np.arange(D), [3, 9, 20])
+        assert np.isfinite(s[:, others]).all() and np.isfinite(o[:, others]).all()
