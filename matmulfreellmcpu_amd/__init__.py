@@ -342,9 +342,17 @@ class Engine:
         """Selective state space scan of sequences of the lengths lens (None: `seqs` equal ones)."""
         _keep, lp, n = _lens(lens, seqs)
         t = _own_type(u) if dtype is None else dtype
-        a = _SCAN_ARGS.pack(t, bool(softplus), _rows(out, t) or 0, _rows(u, t) or 0, _rows(dt, t) or 0, _rows(B, t) or 0,
-                            _rows(C, t) or 0, _rows(z, t) or 0, _ptr(A) or 0, _ptr(skip) or 0, _ptr(dt_bias) or 0,
-                            _ptr(state) or 0, lp or 0, n, rows, D, N, ldo, ldu, lddt, ldb, ldc, ldz)
+        up = _rows(u, t) or 0
+        d = getattr(u, "dtype", None)
+        k = None if d is None else u.__class__  # a tensor like u is of u's type: no call for each
+        a = _SCAN_ARGS.pack(t, bool(softplus),
+                            out.data_ptr() if out.__class__ is k and out.dtype is d else _rows(out, t) or 0, up,
+                            dt.data_ptr() if dt.__class__ is k and dt.dtype is d else _rows(dt, t) or 0,
+                            B.data_ptr() if B.__class__ is k and B.dtype is d else _rows(B, t) or 0,
+                            C.data_ptr() if C.__class__ is k and C.dtype is d else _rows(C, t) or 0,
+                            z.data_ptr() if z.__class__ is k and z.dtype is d else _rows(z, t) or 0,
+                            _ptr(A) or 0, _ptr(skip) or 0, _ptr(dt_bias) or 0, _ptr(state) or 0, lp or 0, n, rows, D, N,
+                            ldo, ldu, lddt, ldb, ldc, ldz)
         rc = self.lib.mmf_selective_scan(self.h, a)
         if rc:
             self._chk(rc)
