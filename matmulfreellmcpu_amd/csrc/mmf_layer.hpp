@@ -189,8 +189,8 @@ struct W4Plan {
 // 16-bit 1.25, int8 0.9 with a scale for 128 inputs; more scalings with more scales), 1.3 times that where a compute unit
 // has fewer than 8 waves to overlap, and up to 1.3 times where fewer outputs share the rows' operands; the
 // fullest compute unit counts. Split inputs cost a launch and the partial sums, written and read at 4 TB/s.
-// Measured (us): fp32 2048 x 6912 x 2560 277 as {4, 1, 1} and 220 as {4, 1, 3}; 512 x 6912 x 2560 147 and 75 as
-// {2, 4, 1}; bf16 2048 x 2048 x 2048 39 and 33 as {4, 2, 1}; fp32 2048 x 2048 x 11264 191, as {4, 2, 1} 215.
+// Measured (us): fp32 2048 x 6912 x 2560 232 as {4, 1, 1} and 195 as {4, 1, 3}; 512 x 6912 x 2560 149 and 80 as
+// {2, 4, 1}; bf16 2048 x 2048 x 2048 44 and 39 as {4, 2, 1}; fp32 2048 x 2048 x 11264 201, as {4, 2, 1} 224.
 inline W4Plan w4_pick(int dtype, const W4Geom& g, int row_tiles) {
   const double unit = (dtype == kF32 ? 2.2 : dtype == kI8 ? 0.9 : 1.25) * (g.step == 32 ? 1.8 : g.step == 64 ? 1.2 : 1.0);
   const int rows = (row_tiles + kW4TileRows / 16 - 1) / (kW4TileRows / 16);
@@ -223,15 +223,16 @@ inline W4Plan w4_plan(int dtype, const W4Geom& g, int row_tiles) {
   return p;
 }
 // The kernel of a call: of few rows, as they are or (fp32) laid out, or by tiles of many, which are laid out.
-// Lines by the products of a call, measured (us): fp32 rows laid out from 0.15 G on (16 x 2048 x 2048 6.6 as they
-// are, 6.8 laid out; 10 x 6912 x 2560 23 and 11; 128 x 2048 x 2048 20 and 11.5), by tiles from 1.6 G on (64 x 6912
-// x 2560 20 laid out, 25 by tiles; 128 x 2048 x 11264 38 and 26). Others by tiles from 2.5 G on (bf16 128 x 6912 x
-// 2560 21 by few rows' kernel, 25 by tiles; 128 x 2048 x 11264 23 and 18).
+// Lines by the products of a call, measured (us): fp32 rows laid out from 0.102 G on (24 x 2048 x 2048 7.3 as they
+// are, 8.4 laid out; 16 x 2560 x 2560 8.5 and 7.3; 10 x 6912 x 2560 15.1 and 10.3; 128 x 2048 x 2048 23.8 and 11.1), by
+// tiles from 1.6 G on (64 x 6912 x 2560 19.3 laid out, 24.6 by tiles; 128 x 2048 x 11264 38.8 and 29.0). Others by
+// tiles from 2.5 G on (bf16 128 x 6912 x 2560 22.6 by few rows' kernel, 24.5 by tiles; 128 x 2048 x 11264 27.4 and
+// 21.3).
 enum W4Way { kRowsAsIs, kLaidRows, kTiles };
 inline W4Way w4_way(int dtype, const W4Geom& g, size_t rows) {
   const double work = static_cast<double>(rows) * g.K * g.N;
   if (rows > 16 && work > (dtype == kF32 ? 1.6e9 : 2.5e9)) return kTiles;
-  return dtype == kF32 && rows > 5 && work > 0.15e9 ? kLaidRows : kRowsAsIs;
+  return dtype == kF32 && rows > 5 && work > 0.102e9 ? kLaidRows : kRowsAsIs;
 }
 inline bool w4_lays(int dtype, const W4Geom& g, size_t rows) { return w4_way(dtype, g, rows) != kRowsAsIs; }
 inline size_t w4_rows_most(int dtype, const W4Geom& g, size_t rows) {

@@ -3,8 +3,9 @@
 // h = x + res, y = h * rstd * w with rstd = 1 / sqrt(mean(h^2) + eps), m = max(max|y|, 1e-5):
 // scale = m / 127 and code = round(y * 127 / m), ties to even. rstd cancels in the code, so one pass over
 // the row finds all it needs, the sum of squares and the largest |h w|, and the row stays in registers
-// until its codes are known: each input is read once and each output written once, which is the bound
-// (2048 x 2560 bf16 with h, 37 MB: 11.4 us alone, 3.2 TB/s; one row 2.5 us, a launch and a load).
+// until its codes are known: each input is read once and each output written once. Alone, 2048 x 2560 bf16 with h, 37
+// MB, takes 11.4 us, 3.2 TB/s, for 7.8 at a copy's rate: all rows start at once, so that loads, arithmetic and stores
+// stand one after another; 2048 x 6912 fp32, 184 MB, 30 us; one row 2.6 us, a launch and a load.
 //
 // The codes are taken in 64 bits: h * w is exact there, and a value's code hangs on its last bits where it
 // lies between two codes. fp64 runs at fp32's rate here (about 11 such operations an element, a third of

@@ -328,7 +328,7 @@ hipError_t scan_launch(const ScanArgs& a, const SeqTab& t, const ScanWs& ws, siz
 // states; it goes through `per` sequences with the decay rates in registers (their rows of N floats are
 // the dearest to read: 64 cache lines a load), the next sequence's state in flight. B and C are one
 // load a wave, handed out by v_readlane. The waves' sums meet in LDS. 64 x 5120 x 16 bf16, 45 MB: 11.2 us, 4.0 TB/s
-// (by k_scan, whose registers leave half the waves, 19); one sequence of 2048 channels 3.2.
+// (by k_scan, whose registers leave half the waves, 19); one sequence of 2048 channels 4.5, a launch.
 constexpr int kStepSeqs = 8;  // most sequences of a block
 template <int DT, int NQ>
 __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, size_t seq0, size_t row0, int seqs, int per) {

@@ -143,8 +143,8 @@ __device__ __forceinline__ auto row_load(const char* row, int k, int K, bool who
 }
 
 // ---- rows laid out --------------------------------------------------------------------------------
-// Many rows, and fp32 rows from a line on, are first laid out as matrix operands: for each tile of 16 rows, chunk, half chunk and part,
-// FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
+// Many rows, and fp32 rows from a line on, are first laid out as matrix operands: for each tile of 16 rows, chunk,
+// half chunk and part, FR fragments of 1 KB (two of 16-bit elements, one of bytes) in which lane l holds 16 bytes of row
 // l % 16; zeros behind the last row and input. Beside fp32 rows' stands a number for each row and
 // scale's inputs, [tile][chunk][S][16]: they are two fp16 parts of x 2^k, the sum of which is x 2^k to half a step of
 // fp32 (or to 2^-40 of the largest), with 2^k bringing the largest of a scale's inputs below 2^15; the number is 2^-k
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
 
 // ---- few rows -------------------------------------------------------------------------------------
 // Few rows: one pass over the weights, bound by a launch, their loads' way and the operands' making (1 x 2048 x 11264,
-// 12 MB: 5.8 us; 1 x 6912 x 2560 6.0; int8 64 x 2048 x 2048 4.7). A block's waves split the chunks of NT tiles of 16
+// 12 MB: 6.2 us alone; 1 x 6912 x 2560 6.4; int8 64 x 2048 x 2048 5.3). A block's waves split the chunks of NT tiles of 16
 // outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix operand's place and
 // multiplies it with CT tiles of rows. fp32 rows are three bf16 parts each (hi + mid + lo = x exactly), 5 rows a
 // tile: a wave cuts its chunk's rows into parts once, in LDS of its own, the next chunk's in flight; or (LAID) they
@@ -517,12 +517,12 @@ hipError_t rows_launch(const W4Args& a, const W4Geom& g, const uint32_t* codes, 
 }
 
 // Tiles of outputs a wave (nt) and waves a block. `units` is the tiles of outputs times the groups of rows.
-// One tile of rows: a wave a tile of outputs; 16 waves where the inputs are long (us: 1 x 6912 x 2560 fp32 6.6 by 8 waves,
-// 5.4 by 16; 1 x 2048 x 11264 5.2 and 6.8). Many rows of one tile share the rows' operands over four tiles of
-// outputs instead where there are enough of these (bf16 16 x 2048 x 11264 8.8 -> 6.9).
+// One tile of rows: a wave a tile of outputs; 16 waves where the inputs are long (us: 1 x 6912 x 2560 fp32 6.5 by 8 waves,
+// 6.0 by 16; 1 x 2048 x 11264 5.7 and 6.3). Many rows of one tile share the rows' operands over four tiles of
+// outputs instead where there are enough of these (bf16 16 x 2048 x 11264 8.7 -> 7.5).
 // Two tiles of rows: the rows' operands are most of what is read, so a wave takes as many tiles of outputs as leave
 // the chip full, and fewer waves share a block when there are more of them (bf16, one tile -> chosen: 64 x 6912 x
-// 2560 28.1 -> 17.7, 128 x 6912 x 2560 41 -> 21, 128 x 2048 x 11264 45 -> 23). fp32 rows, whose parts are made
+// 2560 27.8 -> 17.3, 128 x 6912 x 2560 44 -> 22, 100 x 2048 x 11264 41 -> 26.5). fp32 rows, whose parts are made
 // anew for each of these, take two at most.
 template <int DT, int STEP>
 hipError_t rows_pick(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, hipStream_t s) {
@@ -576,12 +576,12 @@ hipError_t rows_step(const W4Args& a, const W4Geom& g, const uint32_t* codes, co
 // ahead through registers; codes go straight to their operand's place. The codes' products are summed for a
 // scale's inputs alone, and the scale multiplies that sum, so the weights enter unrounded.
 //
-// 2048 x 2048 x 11264 fp32: 182 us and 13 for laying out, 1.04 PFLOP/s of fp16 products; a large library product
-// reaches 1.13 here. The matrix cores are busy 0.48 of the time and the vector ALUs (codes to operands, scales)
+// 2048 x 2048 x 11264 fp32: 179 us and 13 for laying out, 1.06 PFLOP/s of fp16 products; a large library product
+// reaches 1.13 here (bf16 123 and 8, fp16 112 and 8, int8 81 and 5). The matrix cores are busy 0.48 of the time and the vector ALUs (codes to operands, scales)
 // 0.40, and overlap little. Measured and slower: blocks' tiles dealt to the L2 caches (213 to 220 us against
 // 200 then), a later stage brought into L2 by a word of each line (294 against 216: the registers spill), a
 // higher priority for the multiplying wave (215), and for 16-bit rows one tile of outputs after the other, so that
-// a tile's scaling stands beside the next one's products (bf16 124 against 117).
+// a tile's scaling stands beside the next one's products (bf16 124 against 117 then).
 constexpr int kRowTiles = 4;                                // of a wave: what the registers hold
 template <int DT> constexpr int kHalves = DT == kF32 ? 1 : 2;    // half chunks of a stage
 template <int DT> constexpr int kStageKB = kHalves<DT>* kParts<DT>* kFrags<DT>;  // of a tile of rows

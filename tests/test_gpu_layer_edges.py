@@ -53,7 +53,7 @@ def way(t, rows, K, N):
     work = rows * K * N
     if rows > 16 and work > (1.6e9 if t == F32 else 2.5e9):
         return "tiles"
-    return "laid" if t == F32 and rows > 5 and work > 0.15e9 else "few"
+    return "laid" if t == F32 and rows > 5 and work > 0.102e9 else "few"
 
 
 WAYS = [(F32, "few", 1, 2048, 700), (F32, "few", 12, 1031, 700), (F32, "laid", 16, 2048, 8192), (F32, "laid", 20, 2048, 8192),
