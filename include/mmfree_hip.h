@@ -149,9 +149,9 @@ int mmf_rmsnorm_swishgate(mmf_ctx* ctx, float* out, const float* g, const float*
  * and ld elements apart (0: as long as a row; never less). Sums, states and scales are fp32 or
  * wider, and each output is rounded to its type once, to nearest even. Outputs may not overlap
  * other tensors of the call unless said otherwise (MMF_ERR_ARG where the addresses show it).
- * Long scans and products of many rows use a workspace of the context (mmf_workspace_bytes counts it):
- * the first such call allocates it, and fails with MMF_ERR_STATE under stream capture; nothing else
- * is allocated, and it never moves or grows, so calls can be captured into graphs of the context's
+ * Long scans, products of many rows and products of more than 5 fp32 rows with large weights use a workspace of
+ * the context (mmf_workspace_bytes counts it): the first such call allocates it, and fails with MMF_ERR_STATE under
+ * stream capture; nothing else is allocated, and it never moves or grows, so calls can be captured into graphs of the context's
  * stream. Like calls, replays on one context must not overlap. Calls with no rows do nothing.
  *
  * Several sequences stand one after the other in the rows. lens (host, may be NULL) holds their
