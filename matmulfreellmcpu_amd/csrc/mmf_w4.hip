@@ -222,9 +222,9 @@ __global__ __launch_bounds__(256) void k_w4_lay(W4Args a, W4Geom g, char* frags,
 }
 
 // ---- few rows -------------------------------------------------------------------------------------
-// Few rows: one pass over the weights, bound by a launch, their loads' way and the operands' making (1 x 2048 x 11264,
-// 12 MB: 6.2 us alone; 1 x 6912 x 2560 6.4; int8 64 x 2048 x 2048 5.3). A block's waves split the chunks of NT tiles of 16
-// outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix operand's place and
+// Few rows: one pass over the weights, bound by a launch, their loads' way and the operands' making (alone, 1 x 2048 x
+// 11264, 12 MB: 6.2 us; 1 x 6912 x 2560 6.4; int8 64 x 2048 x 2048 5.3). A block's waves split the chunks of NT tiles of
+// 16 outputs; each wave reads its 1 KB of codes per tile and chunk straight into the matrix operand's place and
 // multiplies it with CT tiles of rows. fp32 rows are three bf16 parts each (hi + mid + lo = x exactly), 5 rows a
 // tile: a wave cuts its chunk's rows into parts once, in LDS of its own, the next chunk's in flight; or (LAID) they
 // were laid out, 16 a tile. The rows are the instruction's first operand, so that a lane's sums are of one output and
