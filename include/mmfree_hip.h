@@ -219,6 +219,87 @@ typedef struct {
 } mmf_scan_args;
 int mmf_selective_scan(mmf_ctx* ctx, const mmf_scan_args* args);
 
+/* ---- layer operators: linear attention with 8-bit weights, and what logits say, dev pointers ----
+ * The conventions of the layer operators above: row types, strides, alignment, sequences, states, overlaps, the
+ * workspace, capture. No counterparts in the reference. */
+
+/* Register weights codes [N, K] of 8 bits with scales [N] (host memory): a weight is code * scale of its output. K is at
+ * most 131071, so that sums fit 32 bits. They are repacked on the device; the id is mmf_w8_linear's. */
+int mmf_w8_register(mmf_ctx* ctx, const int8_t* codes, const float* scales, size_t N, size_t K, int* w8_id);
+int mmf_w8_shape(mmf_ctx* ctx, int w8_id, size_t* N, size_t* K);
+/* Free registered weights; the id is invalid afterwards (calls that pass it fail with MMF_ERR_ARG). */
+int mmf_w8_release(mmf_ctx* ctx, int w8_id);
+/* out [rows, N] = x [rows, K] times the transposed weights, plus bias [N] (may be NULL): x int8 codes with xscales [rows],
+ * those of mmf_add_rmsnorm_q8 and mmf_block_norm_q8; out of out_dtype (a float type). Sums are exact integers; an output is
+ * (float(sum) * xscale) * scale + bias in fp32, the last product and sum in one rounding. */
+int mmf_w8_linear(mmf_ctx* ctx, int w8_id, const int8_t* x, const float* xscales, const float* bias, int out_dtype,
+                  void* out, size_t rows, size_t ldx, size_t ldo);
+
+/* Linear attention with a decay for each head. Row by row of a sequence, for each of `heads` heads,
+ *   a = decay[head] + gates[row, head]            (log decays; either may be NULL: 0)
+ *   S = exp(a) * S + k v^T,   out = scale * q^T S
+ * q [rows, q_heads * Dk], k [rows, k_heads * Dk], v [rows, v_heads * Dv] and out [rows, heads * Dv] of dtype, Dk and Dv
+ * 1..256; decay [heads], gates [rows, heads] and state [seqs, heads, Dk, Dv] (may be NULL) in fp32. q_heads, k_heads and
+ * v_heads (0: heads) divide heads, and neighbouring heads share one: head h takes the h / (heads / k_heads)-th of k. A log
+ * decay of -infinity forgets the state; log decays above 0 are taken as they are, and results have to be finite in fp32. A
+ * row whose q, k or v holds an infinity or NaN does not touch the rows before it. */
+typedef struct {
+  int dtype;
+  float scale;
+  void* out;
+  const void *q, *k, *v;
+  const float *decay, *gates;
+  float* state;
+  const size_t* lens;
+  size_t seqs, rows, heads, q_heads, k_heads, v_heads, Dk, Dv;
+  size_t ldo, ldq, ldk, ldv, ldg;
+} mmf_decay_args;
+int mmf_decay_attention(mmf_ctx* ctx, const mmf_decay_args* args);
+
+/* A block's output through its norm, gate and residual scale onto the residual, then the next block's norm with its int8
+ * codes. Row by row,
+ *   p = b / sqrt(mean(b^2) + eps) * w_post        (w_post NULL: p = b)
+ *   h = x + scale * channels * act(gate) * p      (x NULL: 0; channels NULL: 1; gate NULL: 1)
+ *   y = h / sqrt(mean(h^2) + eps) * w_pre         (w_pre NULL: y = h)
+ * and codes and scales of y as mmf_add_rmsnorm_q8 makes them (both or neither). b, x, gate, h, y [rows, cols] of dtype;
+ * w_post, w_pre, channels [cols] fp32; act an MMF_ACT_* (of a gate; sigmoid(g), or silu(g) = g * sigmoid(g)). All steps are
+ * in 64 bits but h, which is rounded to fp32 before the second norm. h (may be NULL) may be b, x or the gate itself with the
+ * same stride; y may be NULL; one of h, y and codes is needed. Rows whose h or y holds an infinity or NaN have codes 0 and
+ * the scale NaN. */
+enum { MMF_ACT_NONE = 0, MMF_ACT_SIGMOID = 1, MMF_ACT_SILU = 2 };
+typedef struct {
+  int dtype, act;
+  const void *b, *x, *gate;
+  const float *w_post, *w_pre, *channels;
+  void *h, *y;
+  int8_t* codes;
+  float* scales;
+  size_t rows, cols;
+  size_t ldb, ldx, ldgate, ldh, ldy, ldcodes;
+  float scale, eps;
+} mmf_block_args;
+int mmf_block_norm_q8(mmf_ctx* ctx, const mmf_block_args* args);
+
+/* Log probabilities under softmax(logits / temperature), row by row of logits [rows, V] of dtype:
+ *   logprobs[row] = log p(ids[row])      (an id outside 0..V-1: NaN)
+ *   entropy[row]  = -sum p log p
+ *   top_ids, top_logprobs [rows, top]    the `top` (0..64, at most V) most likely tokens, likeliest first, equal logits by
+ *                                        the lower id
+ * all but the ids in fp32. ids goes with logprobs (both may be NULL), entropy may be NULL, top may be 0. Logits of -infinity
+ * are tokens that cannot come. Of a row that has no others every log probability is -infinity and the entropy 0; a row with
+ * a NaN or +infinity has no log probabilities (NaN), and its top tokens are ordered with NaN above all. */
+typedef struct {
+  int dtype;
+  float temperature;
+  const void* logits;
+  const int64_t* ids;
+  float *logprobs, *entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  size_t rows, V, top, ld;
+} mmf_logp_args;
+int mmf_token_logprobs(mmf_ctx* ctx, const mmf_logp_args* args);
+
 /* ---- model (model.hpp:33-120) ----------------------------------------------------------- */
 typedef struct {
   size_t vocab_size, hidden_size, num_hidden_layers, intermediate_size; /* config.hpp:8-21 */
@@ -314,6 +395,13 @@ int mmf_model_state(mmf_ctx* ctx, float* out);
 
 /* Model::forward (model.hpp:40-41, hgrn_model.cpp:239-247): stateless, logits [T, V] host. */
 int mmf_model_forward(mmf_ctx* ctx, const int64_t* ids, size_t T, float* logits);
+
+/* What the model gives the tokens of a text: the logits of a stateless forward of T ids (T at least 2), which stay on the
+ * device, through mmf_token_logprobs. Host outputs for positions 0..T-2: logprobs [T-1] of ids[t+1] after ids[0..t], entropy
+ * [T-1], top_ids and top_logprobs [T-1, top]; each may be NULL (top 0). No counterpart in the reference engine, whose callers
+ * take the whole logits. */
+int mmf_model_score(mmf_ctx* ctx, const int64_t* ids, size_t T, float* logprobs, float* entropy, size_t top,
+                    int64_t* top_ids, float* top_logprobs);
 
 /* Layer-by-layer prefill trace for parity checks: after each layer l, h [L][T][H], the
  * state [L][H] and the block internals [L][5][T][H] (i, gated f, g, scan input,

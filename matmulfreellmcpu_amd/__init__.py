@@ -27,6 +27,7 @@ MKBLOB = os.path.join(HERE, "_lib", "mmfree-mkblob")
 
 FLOAT, FIXED_Q510, INT8_ABSMAX = 0, 1, 2
 F32, BF16, F16, I8 = 0, 1, 2, 3  # row types of the layer operators
+ACT_NONE, ACT_SIGMOID, ACT_SILU = 0, 1, 2  # of block_norm_q8's gate
 MODES = {"float": FLOAT, "fixed": FIXED_Q510, "int8": INT8_ABSMAX}
 
 _vp = C.c_void_p
@@ -43,6 +44,10 @@ class MmfConfig(C.Structure):
 # mmf_scan_args: dtype, softplus; eleven pointers (out ... lens); ten sizes (seqs ... ldz). Packed at once, as a
 # ctypes.Structure of as many fields takes longer than the launch.
 _SCAN_ARGS = Struct("@2i21Q")
+
+# mmf_decay_args: dtype, scale; eight pointers; thirteen sizes. mmf_block_args: dtype, act; ten pointers; eight sizes; scale,
+# eps. mmf_logp_args: dtype, temperature; six pointers; four sizes.
+_DECAY_ARGS, _BLOCK_ARGS, _LOGP_ARGS = Struct("@if21Q"), Struct("@2i18Q2f"), Struct("@if10Q")
 
 TOKEN_CB = C.CFUNCTYPE(None, _vp, C.c_int64)
 
@@ -89,6 +94,14 @@ def load_library(path: str = LIB_PATH):
         "mmf_w4_linear": (i, [_vp, i, i, _vp, _vp, i, _vp, _sz, _sz, _sz]),
         "mmf_short_conv": (i, [_vp, i] + [_vp] * 6 + [_sz] * 4 + [i, _sz, _sz]),
         "mmf_selective_scan": (i, [_vp, C.c_char_p]),
+        "mmf_w8_register": (i, [_vp, _vp, _vp, _sz, _sz, C.POINTER(i)]),
+        "mmf_w8_shape": (i, [_vp, i, C.POINTER(_sz), C.POINTER(_sz)]),
+        "mmf_w8_release": (i, [_vp, i]),
+        "mmf_w8_linear": (i, [_vp, i, _vp, _vp, _vp, i, _vp, _sz, _sz, _sz]),
+        "mmf_decay_attention": (i, [_vp, C.c_char_p]),
+        "mmf_block_norm_q8": (i, [_vp, C.c_char_p]),
+        "mmf_token_logprobs": (i, [_vp, C.c_char_p]),
+        "mmf_model_score": (i, [_vp, _i64p, _sz, _fp, _fp, _sz, _i64p, _fp]),
         "mmf_model_begin": (i, [_vp, C.POINTER(MmfConfig)]),
         "mmf_model_tensor": (i, [_vp, C.c_char_p, i, C.POINTER(_sz), i, _vp]),
         "mmf_model_finalize": (i, [_vp, i, i]),
@@ -160,6 +173,13 @@ def _rows(x, t):
 def _own_type(x):
     """The row type of a tensor; an address alone is of F32."""
     return max(_row_type(x) or F32, F32)
+
+
+def _ids(x):
+    """As _ptr, of 64-bit integers: a tensor of another type is refused."""
+    if getattr(x, "dtype", None) is not None and str(x.dtype).rpartition(".")[2] != "int64":
+        raise ValueError(f"a tensor of {x.dtype} in the place of int64 ids")
+    return _ptr(x)
 
 
 def _np(a, dtype):
@@ -357,6 +377,70 @@ class Engine:
         if rc:
             self._chk(rc)
 
+    def register_w8(self, codes, scales) -> int:
+        """8-bit weights: codes int8 [N, K], scales float32 [N]."""
+        codes, cp = _np(codes, np.int8)
+        scales, sp = _np(scales, np.float32)
+        if codes.ndim != 2 or scales.shape != codes.shape[:1]:
+            raise ValueError(f"codes {codes.shape} and scales {scales.shape} are not [N, K] and [N]")
+        wid = C.c_int()
+        self._chk(self.lib.mmf_w8_register(self.h, cp, sp, codes.shape[0], codes.shape[1], C.byref(wid)))
+        return wid.value
+
+    def w8_shape(self, wid):
+        n, k = _sz(), _sz()
+        self._chk(self.lib.mmf_w8_shape(self.h, wid, C.byref(n), C.byref(k)))
+        return n.value, k.value
+
+    def w8_release(self, wid):
+        self._chk(self.lib.mmf_w8_release(self.h, wid))
+
+    def w8_linear(self, wid, x, scales, out, rows, bias=None, out_dtype=None, ldx=0, ldo=0):
+        """out [rows, N] = int8 codes x [rows, K] with scales [rows] times 8-bit weights, plus bias [N] (mmf_w8_linear)."""
+        o = _own_type(out) if out_dtype is None else out_dtype
+        rc = self.lib.mmf_w8_linear(self.h, wid, _rows(x, I8), _rows(scales, F32), _rows(bias, F32), o, _rows(out, o), rows,
+                                    ldx, ldo)
+        if rc:
+            self._chk(rc)
+
+    def decay_attention(self, out, q, k, v, rows, heads, Dk, Dv, decay=None, gates=None, state=None, lens=None, seqs=1,
+                        q_heads=0, k_heads=0, v_heads=0, scale=None, dtype=None, ldo=0, ldq=0, ldk=0, ldv=0, ldg=0):
+        """Linear attention with a decay for each head, of sequences of the lengths lens (None: `seqs` equal ones); decay
+        [heads] and gates [rows, heads] are log decays, scale None is Dk ** -0.5 (mmf_decay_attention)."""
+        _keep, lp, n = _lens(lens, seqs)
+        t = _own_type(q) if dtype is None else dtype
+        a = _DECAY_ARGS.pack(t, Dk ** -0.5 if scale is None else scale, _rows(out, t) or 0, _rows(q, t) or 0, _rows(k, t) or 0,
+                             _rows(v, t) or 0, _rows(decay, F32) or 0, _rows(gates, F32) or 0, _rows(state, F32) or 0, lp or 0,
+                             n, rows, heads, q_heads, k_heads, v_heads, Dk, Dv, ldo, ldq, ldk, ldv, ldg)
+        rc = self.lib.mmf_decay_attention(self.h, a)
+        if rc:
+            self._chk(rc)
+
+    def block_norm_q8(self, codes, scales, b, rows, cols, x=None, gate=None, act=ACT_NONE, w_post=None, w_pre=None,
+                      channels=None, scale=1.0, h=None, y=None, eps=1e-6, dtype=None, ldb=0, ldx=0, ldgate=0, ldh=0, ldy=0,
+                      ldcodes=0):
+        """h = x + scale * channels * act(gate) * norm(b) w_post, then norm(h) w_pre as y and as int8 codes with a scale per
+        row; codes and scales may both be None (mmf_block_norm_q8)."""
+        t = _own_type(b) if dtype is None else dtype
+        a = _BLOCK_ARGS.pack(t, act, _rows(b, t) or 0, _rows(x, t) or 0, _rows(gate, t) or 0, _rows(w_post, F32) or 0,
+                             _rows(w_pre, F32) or 0, _rows(channels, F32) or 0, _rows(h, t) or 0, _rows(y, t) or 0,
+                             _rows(codes, I8) or 0, _rows(scales, F32) or 0, rows, cols, ldb, ldx, ldgate, ldh, ldy, ldcodes,
+                             scale, eps)
+        rc = self.lib.mmf_block_norm_q8(self.h, a)
+        if rc:
+            self._chk(rc)
+
+    def token_logprobs(self, logits, rows, V, ids=None, logprobs=None, entropy=None, top=0, top_ids=None, top_logprobs=None,
+                       temperature=1.0, dtype=None, ld=0):
+        """Log probabilities of ids [rows] (int64), entropies and the `top` most likely tokens of logits [rows, V]
+        (mmf_token_logprobs)."""
+        t = _own_type(logits) if dtype is None else dtype
+        a = _LOGP_ARGS.pack(t, temperature, _rows(logits, t) or 0, _ids(ids) or 0, _rows(logprobs, F32) or 0,
+                            _rows(entropy, F32) or 0, _ids(top_ids) or 0, _rows(top_logprobs, F32) or 0, rows, V, top, ld)
+        rc = self.lib.mmf_token_logprobs(self.h, a)
+        if rc:
+            self._chk(rc)
+
     # ---- model ----
     def load_blob(self, path_or_blob, mode=FLOAT, frac_bits=10):
         """Upload every tensor of an MMFREE1 blob and prepare the engine for `mode`."""
@@ -439,6 +523,19 @@ class Engine:
         lg = np.empty((ids.size, self.cfg.vocab_size), np.float32)
         self._chk(self.lib.mmf_model_forward(self.h, ids.ctypes.data_as(_i64p), ids.size, lg.ctypes.data_as(_fp)))
         return lg
+
+    def score(self, ids, top=0):
+        """(log probability of each token after the first, entropies [T-1]) of a text of T ids, and with top the most likely
+        tokens: (..., their ids [T-1, top], their log probabilities). The logits stay on the device (mmf_model_score)."""
+        ids = np.ascontiguousarray(ids, np.int64)
+        if top < 0:
+            raise ValueError(f"top {top} is negative")
+        n = max(ids.size - 1, 0)
+        lp, ent = np.empty(n, np.float32), np.empty(n, np.float32)
+        tid, tlp = np.empty((n, top), np.int64), np.empty((n, top), np.float32)
+        self._chk(self.lib.mmf_model_score(self.h, ids.ctypes.data_as(_i64p), ids.size, lp.ctypes.data_as(_fp),
+                                           ent.ctypes.data_as(_fp), top, tid.ctypes.data_as(_i64p), tlp.ctypes.data_as(_fp)))
+        return (lp, ent, tid, tlp) if top else (lp, ent)
 
     def trace(self, ids, internals=True):
         c = self.cfg

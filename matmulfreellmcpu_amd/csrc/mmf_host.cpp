@@ -105,6 +105,14 @@ struct W4 {
   const uint32_t *codes = nullptr, *scales = nullptr;
 };
 
+// 8-bit weights (mmf_w8_register): codes and scales in one allocation.
+struct W8 {
+  W8Geom g{};
+  void* mem = nullptr;
+  const int8_t* codes = nullptr;
+  const float* scales = nullptr;
+};
+
 struct DevTensor {
   void* p = nullptr;
   std::vector<size_t> shape;
@@ -128,6 +136,7 @@ struct LayerDev {
 struct RowScratch {
   DBuf ids, h, resid, i, f, g, recur, scan, z, logits, state0, am;
   DBuf acty, actq, actct, actsa;
+  DBuf score;  // the outputs of mmf_model_score
   DBuf segs;  // stacked prompts: nseg + 1 row offsets, then the nseg last-row indices
   DBuf chunk;  // chunk summaries and starting states of the chunked scan
 };
@@ -206,6 +215,7 @@ struct mmf_ctx {
   std::string err;
   std::vector<Proj> projs;
   std::vector<W4> w4s;
+  std::vector<W8> w8s;
   Model model;
   DBuf raw;  // staging for int8 weights before the repack
   DBuf opy, opq, opct, opsa, opstate;
@@ -1081,6 +1091,8 @@ void mmf_destroy(mmf_ctx* c) {
   }
   for (auto& w : c->w4s)
     if (w.mem) (void)hipFree(w.mem);
+  for (auto& w : c->w8s)
+    if (w.mem) (void)hipFree(w.mem);
   for (auto& kv : c->model.tensors)
     if (kv.second.p) (void)hipFree(kv.second.p);
   Model& m = c->model;
@@ -1089,7 +1101,8 @@ void mmf_destroy(mmf_ctx* c) {
     b->release();
   RowScratch& s = m.rs;
   for (DBuf* b : {&s.ids, &s.h, &s.resid, &s.i, &s.f, &s.g, &s.recur, &s.scan, &s.z, &s.logits, &s.state0, &s.am,
-                  &s.acty, &s.actq, &s.actct, &s.actsa, &s.segs, &s.chunk})
+                  &s.acty, &s.actq, &s.actct, &s.actsa, &s.score, &s.segs,
+                  &s.chunk})
     b->release();
   StepScratch& ss = m.ss;
   for (DBuf* b : {&ss.h, &ss.resid, &ss.g, &ss.recur, &ss.z, &ss.keys}) b->release();
@@ -1556,6 +1569,11 @@ static const W4& w4_of(mmf_ctx* c, int id) {
   if (!c->w4s[id].mem) fail(MMF_ERR_ARG, "w4_id " + std::to_string(id) + " was released");
   return c->w4s[id];
 }
+static const W8& w8_of(mmf_ctx* c, int id) {
+  if (id < 0 || id >= static_cast<int>(c->w8s.size())) fail(MMF_ERR_ARG, "invalid w8_id " + std::to_string(id));
+  if (!c->w8s[id].mem) fail(MMF_ERR_ARG, "w8_id " + std::to_string(id) + " was released");
+  return c->w8s[id];
+}
 }  // extern "C++"
 
 int mmf_add_rmsnorm_q8(mmf_ctx* c, int dtype, int8_t* codes, float* scales, const void* x, const void* res, void* h,
@@ -1647,6 +1665,91 @@ int mmf_selective_scan(mmf_ctx* c, const mmf_scan_args* s) {
                s->lens, s->seqs, s->rows, s->D, s->N, s->ldo, s->ldu, s->lddt, s->ldb, s->ldc, s->ldz};
     refuse(check(a));
     MMF_HIP(launch_sel_scan(a, scan_splits(a) ? reinterpret_cast<float*>(layer_ws(c)) : nullptr, c->stream));
+  });
+}
+
+int mmf_w8_register(mmf_ctx* c, const int8_t* codes, const float* scales, size_t N, size_t K, int* w8_id) {
+  return guard(c, [&] {
+    if (!codes || !scales || !w8_id) fail(MMF_ERR_ARG, "null argument");
+    refuse(check_w8(N, K));
+    W8 w;
+    w.g = w8_geom(N, K);
+    char* raw = static_cast<char*>(c->raw.get(N * K));
+    MMF_HIP(hipMemcpyAsync(raw, codes, N * K, hipMemcpyHostToDevice, c->stream));
+    c->w8s.reserve(c->w8s.size() + 1);  // so that nothing below throws away the allocation
+    const size_t bytes = w8_code_bytes(w.g);
+    MMF_HIP(hipMalloc(&w.mem, bytes + N * sizeof(float)));
+    w.codes = static_cast<const int8_t*>(w.mem);
+    w.scales = reinterpret_cast<const float*>(w.codes + bytes);
+    hipError_t e = hipMemcpyAsync(const_cast<float*>(w.scales), scales, N * sizeof(float), hipMemcpyHostToDevice, c->stream);
+    if (e == hipSuccess) e = launch_w8_pack(reinterpret_cast<const int8_t*>(raw), w.g, const_cast<int8_t*>(w.codes), c->stream);
+    const hipError_t done = hipStreamSynchronize(c->stream);  // the caller's arrays have been read
+    if (e == hipSuccess) e = done;
+    if (e != hipSuccess) {
+      (void)hipFree(w.mem);
+      MMF_HIP(e);
+    }
+    c->w8s.push_back(w);
+    *w8_id = static_cast<int>(c->w8s.size() - 1);
+  });
+}
+
+int mmf_w8_shape(mmf_ctx* c, int id, size_t* N, size_t* K) {
+  return guard(c, [&] {
+    const W8& w = w8_of(c, id);
+    if (N) *N = w.g.N;
+    if (K) *K = w.g.K;
+  });
+}
+
+int mmf_w8_release(mmf_ctx* c, int id) {
+  return guard(c, [&] {
+    (void)w8_of(c, id);
+    MMF_HIP(hipStreamSynchronize(c->stream));
+    MMF_HIP(hipFree(c->w8s[id].mem));
+    c->w8s[id] = W8{};
+  });
+}
+
+int mmf_w8_linear(mmf_ctx* c, int id, const int8_t* x, const float* xscales, const float* bias, int out_dtype, void* out,
+                  size_t rows, size_t ldx, size_t ldo) {
+  return guard(c, [&] {
+    const W8& w = w8_of(c, id);
+    W8Args a{out_dtype, x, xscales, bias, out, rows, ldx, ldo};
+    refuse(check(a, w.g.N, w.g.K));
+    MMF_HIP(launch_w8(a, w.g, w.codes, w.scales, nullptr, c->stream));
+  });
+}
+
+int mmf_decay_attention(mmf_ctx* c, const mmf_decay_args* s) {
+  return guard(c, [&] {
+    if (!s) fail(MMF_ERR_ARG, "null argument");
+    DecayArgs a{s->dtype, s->out, s->q, s->k, s->v, s->decay, s->gates, s->state, s->lens, s->seqs, s->rows, s->heads,
+                s->q_heads, s->k_heads, s->v_heads, s->Dk, s->Dv, s->ldo, s->ldq, s->ldk, s->ldv, s->ldg, s->scale};
+    refuse(check(a));
+    MMF_HIP(launch_decay(a, nullptr, c->stream));
+  });
+}
+
+int mmf_block_norm_q8(mmf_ctx* c, const mmf_block_args* s) {
+  return guard(c, [&] {
+    if (!s) fail(MMF_ERR_ARG, "null argument");
+    BlockArgs a{s->dtype, s->act, s->b, s->x, s->gate, s->w_post, s->w_pre, s->channels, s->h, s->y, s->codes, s->scales,
+                s->rows, s->cols, s->ldb, s->ldx, s->ldgate, s->ldh, s->ldy, s->ldcodes, s->scale, s->eps};
+    refuse(check(a));
+    MMF_HIP(launch_block(a, c->stream));
+  });
+}
+
+int mmf_token_logprobs(mmf_ctx* c, const mmf_logp_args* s) {
+  return guard(c, [&] {
+    if (!s) fail(MMF_ERR_ARG, "null argument");
+    LogpArgs a{s->dtype, s->logits, s->ids, s->logprobs, s->entropy, s->top_ids, s->top_logprobs, s->rows, s->V, s->top,
+               s->ld, s->temperature};
+    refuse(check(a));
+    if (!a.rows) return;
+    const bool parts = logp_plan(a.dtype, a.V).segs > 1;
+    MMF_HIP(launch_logp(a, parts ? reinterpret_cast<float*>(layer_ws(c)) : nullptr, c->stream));
   });
 }
 
@@ -2101,25 +2204,61 @@ int mmf_model_state(mmf_ctx* c, float* out) {
   });
 }
 
+// Stateless forward of T checked ids: the logits [T, V] on the device; the ids stay in m.rs.ids.
+extern "C++" {
+static float* forward_rows(mmf_ctx* c, Model& m, const int64_t* ids, size_t T) {
+  const size_t H = m.cfg.hidden_size, V = m.cfg.vocab_size;
+  RowScratch& s = m.rs;
+  int64_t* d = s.ids.as<int64_t>(T);
+  MMF_HIP(hipMemcpyAsync(d, ids, T * sizeof(int64_t), hipMemcpyHostToDevice, c->stream));
+  float* h = s.h.as<float>(T * H);
+  MMF_HIP(launch_embed(m.emb, d, h, static_cast<int>(T), static_cast<int>(H), c->stream));
+  float* st = s.state0.as<float>(H);
+  for (size_t l = 0; l < m.cfg.num_hidden_layers; ++l) {
+    MMF_HIP(hipMemsetAsync(st, 0, H * sizeof(float), c->stream));  // fresh state (hgrn_model.cpp:233)
+    layer_rows(c, m, static_cast<int>(l), static_cast<int>(T), h, st, false, nullptr);
+  }
+  float* lg = s.logits.as<float>(T * V);
+  lm_rows(c, m, static_cast<int>(T), h, lg);
+  return lg;
+}
+}  // extern "C++"
+
 int mmf_model_forward(mmf_ctx* c, const int64_t* ids, size_t T, float* logits) {
   return guard(c, [&] {
     Model& m = model_of(c);
     if (!ids || T == 0 || !logits) fail(MMF_ERR_ARG, "invalid forward arguments");
     check_ids(m, ids, T);
-    const size_t H = m.cfg.hidden_size, V = m.cfg.vocab_size;
-    RowScratch& s = m.rs;
-    int64_t* d = s.ids.as<int64_t>(T);
-    MMF_HIP(hipMemcpyAsync(d, ids, T * sizeof(int64_t), hipMemcpyHostToDevice, c->stream));
-    float* h = s.h.as<float>(T * H);
-    MMF_HIP(launch_embed(m.emb, d, h, static_cast<int>(T), static_cast<int>(H), c->stream));
-    float* st = s.state0.as<float>(H);
-    for (size_t l = 0; l < m.cfg.num_hidden_layers; ++l) {
-      MMF_HIP(hipMemsetAsync(st, 0, H * sizeof(float), c->stream));  // fresh state (hgrn_model.cpp:233)
-      layer_rows(c, m, static_cast<int>(l), static_cast<int>(T), h, st, false, nullptr);
-    }
-    float* lg = s.logits.as<float>(T * V);
-    lm_rows(c, m, static_cast<int>(T), h, lg);
-    MMF_HIP(hipMemcpyAsync(logits, lg, T * V * sizeof(float), hipMemcpyDeviceToHost, c->stream));
+    const float* lg = forward_rows(c, m, ids, T);
+    MMF_HIP(hipMemcpyAsync(logits, lg, T * m.cfg.vocab_size * sizeof(float), hipMemcpyDeviceToHost, c->stream));
+    MMF_HIP(hipStreamSynchronize(c->stream));
+  });
+}
+
+int mmf_model_score(mmf_ctx* c, const int64_t* ids, size_t T, float* logprobs, float* entropy, size_t top, int64_t* top_ids,
+                    float* top_logprobs) {
+  return guard(c, [&] {
+    Model& m = model_of(c);
+    if (!ids || T < 2 || T - 1 > kMaxRows || (!logprobs && !entropy && !top)) fail(MMF_ERR_ARG, "invalid score arguments");
+    const size_t n = T - 1, V = m.cfg.vocab_size;
+    if (top > kMaxTop || top > V || (top && (!top_ids || !top_logprobs))) fail(MMF_ERR_ARG, "invalid top alternatives");
+    check_ids(m, ids, T);
+    char* ws = logp_plan(kF32, V).segs > 1 ? layer_ws(c) : nullptr;
+    const float* lg = forward_rows(c, m, ids, T);
+    // top ids first: they are 8 bytes each
+    int64_t* d_ids = reinterpret_cast<int64_t*>(m.rs.score.as<char>(n * (top * 12 + 8)));
+    float* d_top = reinterpret_cast<float*>(d_ids + n * top);
+    float *d_lp = d_top + n * top, *d_ent = d_lp + n;
+    LogpArgs a{kF32, lg, static_cast<const int64_t*>(m.rs.ids.p) + 1, d_lp, d_ent, d_ids, d_top, n, V, top, V, 1.0f};
+    refuse(check(a));
+    MMF_HIP(launch_logp(a, reinterpret_cast<float*>(ws), c->stream));
+    auto give = [&](void* to, const void* from, size_t bytes) {
+      if (to && bytes) MMF_HIP(hipMemcpyAsync(to, from, bytes, hipMemcpyDeviceToHost, c->stream));
+    };
+    give(logprobs, d_lp, n * sizeof(float));
+    give(entropy, d_ent, n * sizeof(float));
+    give(top_ids, d_ids, n * top * sizeof(int64_t));
+    give(top_logprobs, d_top, n * top * sizeof(float));
     MMF_HIP(hipStreamSynchronize(c->stream));
   });
 }

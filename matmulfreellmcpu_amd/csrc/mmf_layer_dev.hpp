@@ -3,7 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
-#include "mmf_layer.hpp"
+#include "mmf_layer8.hpp"
 
 namespace mmf {
 
@@ -19,6 +19,12 @@ hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const ui
 // ws: kLayerWsBytes where w4_lays(a.dtype, g, a.rows)
 hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
                      hipStream_t s);
+hipError_t launch_w8_pack(const int8_t* codes, const W8Geom& g, int8_t* out, hipStream_t s);
+hipError_t launch_w8(const W8Args& a, const W8Geom& g, const int8_t* codes, const float* scales, char* ws, hipStream_t s);
+hipError_t launch_block(const BlockArgs& a, hipStream_t s);
+hipError_t launch_decay(const DecayArgs& a, float* ws, hipStream_t s);
+// ws: kLayerWsBytes where logp_plan(a.dtype, a.V).segs > 1
+hipError_t launch_logp(const LogpArgs& a, float* ws, hipStream_t s);
 
 // Element type DT of a row tensor: V neighbouring elements in one 16-byte access at any address that
 // the type is aligned at (gfx950 takes vector accesses at element alignment).
