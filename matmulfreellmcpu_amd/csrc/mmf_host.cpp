@@ -1727,7 +1727,7 @@ int mmf_decay_attention(mmf_ctx* c, const mmf_decay_args* s) {
     DecayArgs a{s->dtype, s->out, s->q, s->k, s->v, s->decay, s->gates, s->state, s->lens, s->seqs, s->rows, s->heads,
                 s->q_heads, s->k_heads, s->v_heads, s->Dk, s->Dv, s->ldo, s->ldq, s->ldk, s->ldv, s->ldg, s->scale};
     refuse(check(a));
-    MMF_HIP(launch_decay(a, nullptr, c->stream));
+    MMF_HIP(launch_decay(a, decay_splits(a) ? reinterpret_cast<float*>(layer_ws(c)) : nullptr, c->stream));
   });
 }
 

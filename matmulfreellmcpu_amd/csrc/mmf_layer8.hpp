@@ -162,6 +162,95 @@ inline const char* check(DecayArgs& a) {
   return nullptr;
 }
 
+// Sequences of a launch: `len` rows from row `row` on, with the state of sequence `seq`. In tiles of `step` rows (a tile is
+// a block's share of a long sequence); those of more than one tile stand first, so that their tiles are numbered from 0
+// and only they need slots of the workspace.
+constexpr int kDecaySeqs = 192;
+struct DecayTab {
+  int n, step, many;             // sequences, rows of a tile, sequences of more than one tile
+  int row[kDecaySeqs], len[kDecaySeqs], seq[kDecaySeqs];
+  int tile[kDecaySeqs + 1];      // first tile of each; behind the last, their number
+};
+struct DecaySeq {
+  int row, len, seq;
+};
+// Rows that a block multiplies at a time.
+inline int decay_chunk(int dtype) { return dtype == kBF16 ? 64 : 32; }
+// The table of n sequences cut into tiles of `step` rows.
+inline void fill_decay(DecayTab& t, const DecaySeq* s, int n, int step) {
+  t.n = n;
+  t.step = step;
+  int k = 0, tiles = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i = 0; i < n; ++i) {
+      if ((s[i].len > step) != (pass == 0)) continue;
+      t.row[k] = s[i].row;
+      t.len[k] = s[i].len;
+      t.seq[k] = s[i].seq;
+      t.tile[k++] = tiles;
+      tiles += (s[i].len + step - 1) / step;
+    }
+    if (pass == 0) t.many = k;
+  }
+  t.tile[k] = tiles;
+}
+// Rows of a tile: so many that the tiles of all heads fill the chip twice, and that those of long sequences have room in
+// the workspace. No sequence is cut into two: that would be three launches for one.
+inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
+  const int chunk = decay_chunk(a.dtype);
+  size_t chunks = 0;
+  int most = 0;
+  for (int i = 0; i < n; ++i) {
+    chunks += (s[i].len + chunk - 1) / chunk;
+    most = s[i].len > most ? s[i].len : most;
+  }
+  const size_t blocks = a.heads * ((a.Dv + 127) / 128), per = a.heads * (a.Dk * a.Dv + 1);
+  size_t step = (chunks * blocks + 511) / 512 * chunk;
+  if (step < 128) step = 128;
+  for (;; step *= 2) {
+    if (step * 2 >= static_cast<size_t>(most)) return most;
+    size_t slots = 0;
+    for (int i = 0; i < n; ++i)
+      if (static_cast<size_t>(s[i].len) > step) slots += (s[i].len + step - 1) / step;
+    if (slots * per <= kLayerWsBytes / 4) return static_cast<int>(step);
+  }
+}
+// Calls steps(tab) for sequences of up to kDecayShort rows and tiles(tab) for longer ones, up to kDecaySeqs at a time,
+// until one returns a value other than `ok`.
+constexpr int kDecayShort = 1;
+template <class R, class Steps, class Tiles>
+R each_decay(const DecayArgs& a, R ok, Steps&& steps, Tiles&& tiles) {
+  DecaySeq few[kDecaySeqs], many[kDecaySeqs];
+  int nf = 0, nm = 0, row = 0;
+  DecayTab t;
+  R r = ok;
+  auto flush = [&](bool of_few) {
+    if (of_few ? nf : nm) {
+      if (of_few)
+        fill_decay(t, few, nf, 1 << 25);
+      else
+        fill_decay(t, many, nm, decay_step(a, many, nm));
+      r = of_few ? steps(t) : tiles(t);
+    }
+    (of_few ? nf : nm) = 0;
+  };
+  for (size_t i = 0; i < a.seqs && r == ok; ++i) {
+    const int len = static_cast<int>(a.lens ? a.lens[i] : a.rows / a.seqs);
+    if (!len) continue;
+    const bool is_few = len <= kDecayShort;
+    (is_few ? few[nf++] : many[nm++]) = {row, len, static_cast<int>(i)};
+    row += len;
+    if ((is_few ? nf : nm) == kDecaySeqs) flush(is_few);
+  }
+  if (r == ok) flush(true);
+  if (r == ok) flush(false);
+  return r;
+}
+// Whether a call needs the workspace.
+inline bool decay_splits(const DecayArgs& a) {
+  return each_decay(a, 0, [](const DecayTab&) { return 0; }, [](const DecayTab& t) { return t.many ? 1 : 0; }) != 0;
+}
+
 // ---- log probabilities of tokens ------------------------------------------------------------------
 constexpr size_t kMaxTop = 64;
 struct LogpArgs {
