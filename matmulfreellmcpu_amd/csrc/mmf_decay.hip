@@ -14,6 +14,7 @@ typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The log decay of a row in powers of two. 2^-300 times any fp32 number is 0, as 2^-infinity is, and leaves the sums
@@ -39,8 +40,8 @@ __global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, DecayTab t, si
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int Dk = static_cast<int>(a.Dk), Dv = static_cast<int>(a.Dv);
   const bool listed = t.n > 0;  // else a row of each
-  const size_t first = listed ? t.row[blockIdx.y] : first_seq + blockIdx.y, seq = listed ? t.seq[blockIdx.y] : first;
-  const int len = listed ? t.len[blockIdx.y] : 1;
+  const size_t first = listed ? t.of[blockIdx.y].row : first_seq + blockIdx.y, seq = listed ? t.of[blockIdx.y].seq : first;
+  const int len = listed ? t.of[blockIdx.y].len : 1;
   float* state = a.state ? a.state + (seq * a.heads + head) * a.Dk * a.Dv : nullptr;
   const T* q = static_cast<const T*>(a.q) + first * a.ldq + head / (a.heads / a.q_heads) * a.Dk;
   const T* k = static_cast<const T*>(a.k) + first * a.ldk + head / (a.heads / a.k_heads) * a.Dk;
@@ -126,8 +127,8 @@ hipError_t steps_launch(const DecayArgs& a, const DecayTab& t, size_t first_seq,
 }
 
 // ---- chunks of rows ----------------------------------------------------------------------------------
-// A block takes 64 NT columns of one head's state over a tile of a sequence, a chunk of C rows at a time; each of its 4
-// waves holds the state of its 16 NT columns in registers, as the matrix instructions leave it: lane l, column l % 16,
+// A block takes 16 columns a wave of one head's state over a tile of a sequence, a chunk of 32 rows at a time; each of its
+// waves holds the state of its 16 columns in registers, as the matrix instructions leave it: lane l, column l % 16,
 // rows 4 (l / 16) + 0..3 of each 16. A lane's rows of two such tiles are also one operand of the next product over
 // these rows, as are the weights of a chunk's rows (k q^T): neither goes through LDS to change its layout. An operand's 32
 // inputs then are, for lane group g = l / 16, 4 g + 0..3 and 16 + 4 g + 0..3 of them, in this order, in all products.
@@ -140,6 +141,7 @@ template <int DT>
 inline constexpr int kParts = DT == kF32 ? 3 : DT == kF16 ? 2 : 1;
 template <int DT>
 inline constexpr int kSumParts = DT == kF32 ? 3 : 2;  // of the state and the weights
+constexpr int kChunk = kDecayChunk;
 enum DecayPass { kEnds = 0, kOutputs = 1 };
 
 // Place of 4 neighbouring elements (unit u of a row) of a tile of COLS columns, in such units: rows are turned against each
@@ -154,6 +156,13 @@ __device__ __forceinline__ float upper(float v) {  // the upper 16 bits, a bf16 
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u);
 }
 __device__ __forceinline__ uint16_t upper_bits(float v) { return static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v) >> 16); }
+
+// A uniform address and 32 bits of a lane's own.
+template <class T>
+__device__ __forceinline__ T& at_bytes(T* base, uint32_t bytes) {
+  using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+  return *reinterpret_cast<T*>(reinterpret_cast<Byte*>(base) + bytes);
+}
 
 // v in N bf16 parts: the first ones cut off, the last one rounded (of three: exact).
 template <int N>
@@ -210,37 +219,54 @@ __device__ __forceinline__ void mma(const bf16x8* a, const bf16x8* b, f32x4& c) 
       if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
 }
 
-// C rows of COLS columns from global memory, 8 neighbouring columns at a time, in registers and then in LDS.
-template <int DT, int C, int COLS>
+// kChunk rows of COLS columns from global memory, 8 neighbouring columns at a time, in registers and then in LDS. Loads have no
+// conditions, so that all are in flight together: rows and columns past the end are read from the last ones and then
+// set to 0.
+template <int DT, int COLS, int TH>
 struct Tile {
   using E = Elem<DT>;
   using T = typename E::T;
-  static constexpr int kEach = C * COLS / 8 / 256, N = kParts<DT>;
-  typename E::Vec v[kEach][8 / E::V];
-  __device__ __forceinline__ void fetch(const T* p, size_t ld, int rows, int cols) {
+  static constexpr int kVecs = kChunk * COLS / 8, kUsed = kVecs < TH ? kVecs : TH;
+  static constexpr int kEach = kVecs / kUsed, kRows = kUsed / (COLS / 8), N = kParts<DT>, H = 8 / E::V;
+  typename E::Vec v[kEach][H];
+  // The thread's first element of a chunk that starts at p, where columns come in groups of 8.
+  __device__ __forceinline__ static const T* place(const T* p, size_t ld, int cols) {
+    return p + (threadIdx.x % kUsed / (COLS / 8)) * ld + max(min(static_cast<int>(threadIdx.x) % (COLS / 8) * 8, cols - 8), 0);
+  }
+  // mine: place() of the chunk at p, of which `rows` are left
+  __device__ __forceinline__ void fetch(const T* mine, const T* p, size_t ld, int rows, int cols) {
+    if (kUsed < TH && threadIdx.x >= kUsed) return;
+    const int r0 = threadIdx.x / (COLS / 8), c = threadIdx.x % (COLS / 8) * 8;
+    if (cols % 8 == 0) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = i * 256 + threadIdx.x, r = at / (COLS / 8), c = at % (COLS / 8) * 8;
-      const T* from = p + r * ld + c;
+      for (int i = 0; i < kEach; ++i) {
+        const T* from = mine + i * kRows * ld;
+        if (rows < kChunk) from -= max(r0 + i * kRows - rows + 1, 0) * ld;
 #pragma unroll
-      for (int h = 0; h < 8 / E::V; ++h) {
-        v[i][h] = typename E::Vec{};
-        if (r >= rows) continue;
-        if (c + (h + 1) * E::V <= cols) {
-          v[i][h] = *reinterpret_cast<const typename E::Vec*>(from + h * E::V);
-        } else {
-#pragma unroll
-          for (int j = 0; j < E::V; ++j)
-            if (c + h * E::V + j < cols) v[i][h][j] = from[h * E::V + j];
-        }
+        for (int h = 0; h < H; ++h) v[i][h] = *reinterpret_cast<const typename E::Vec*>(from + h * E::V);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const T* from = p + min(r0 + i * kRows, rows - 1) * ld;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j / E::V][j % E::V] = from[min(c + j, cols - 1)];
+      }
+    }
+    if (rows < kChunk || cols < COLS) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (r0 + i * kRows >= rows || c + j >= cols) v[i][j / E::V][j % E::V] = T{};
     }
   }
   __device__ __forceinline__ void store(uint16_t* tile) const {
+    if (kUsed < TH && threadIdx.x >= kUsed) return;
+    const int r0 = threadIdx.x / (COLS / 8), u = threadIdx.x % (COLS / 8) * 2;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int at = i * 256 + threadIdx.x, r = at / (COLS / 8), c = at % (COLS / 8) * 8;
-      uint16_t* to = tile + unit_at<COLS>(r, c / 4) * 4;
+      uint16_t* to = tile + unit_at<COLS>(r0 + i * kRows, u) * 4;
       if constexpr (DT == kBF16) {
         *reinterpret_cast<u16x8*>(to) = v[i][0];
       } else {
@@ -250,342 +276,362 @@ struct Tile {
         for (int j = 0; j < 8; ++j) f[j] = E::up(v[i][j / E::V][j % E::V]);
         cut8<N>(f, p);
 #pragma unroll
-        for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(to + k * C * COLS) = p[k];
+        for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(to + k * kChunk * COLS) = p[k];
       }
     }
   }
 };
 
-template <int DT, int DKP, int NT>
+// Running sums over the first 32 lanes.
+__device__ __forceinline__ double running_sum(double x) {
+  auto moved = [](double v, auto ctrl) {  // of the lane that many places before it in its row of 16, else 0
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    constexpr int k = decltype(ctrl)::value;
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u), k, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(u >> 32), k, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+  };
+  x += moved(x, std::integral_constant<int, 0x111>{});  // row_shr 1, 2, 4, 8
+  x += moved(x, std::integral_constant<int, 0x112>{});
+  x += moved(x, std::integral_constant<int, 0x114>{});
+  x += moved(x, std::integral_constant<int, 0x118>{});
+  const double first = __shfl(x, 15);
+  return (threadIdx.x & 63) < 16 ? x : x + first;
+}
+
+template <int DT, int DKP, int NW>
 struct DecayShape {
-  static constexpr int C = DT == kBF16 ? 64 : 32, DVP = 64 * NT, N = kParts<DT>, NS = kSumParts<DT>;
-  static constexpr int kSlabs = C / 16, kSteps = C / 32;
-  static constexpr int kRowTile = C * DKP * N, kColTile = C * DVP * N, kWeights = kSlabs * kSteps * NS * 512;
-  static constexpr int kEndsBytes = (kRowTile + kColTile) * 2, kOutBytes = (2 * kRowTile + kColTile + kWeights) * 2;
+  static constexpr int DVP = 16 * NW, N = kParts<DT>, NS = kSumParts<DT>;
+  static constexpr int kRowTile = kChunk * DKP * N, kColTile = kChunk * DVP * N, kWeights = 2 * NS * 512;
+  static constexpr int kEndsOne = kRowTile + kColTile, kOutOne = 2 * kRowTile + kColTile + kWeights;
+  // two buffers where they fit: the next chunk's rows are stored beside the products of this one
+  static constexpr int kSumBytes = NW * kChunk * 16, kLds = 160 * 1024 - 512;
+  static constexpr int kEndsBuffers = kEndsOne * 4 + kSumBytes <= kLds ? 2 : 1, kOutBuffers = kOutOne * 4 + kSumBytes <= kLds ? 2 : 1;
+  static constexpr int kEndsBytes = kEndsOne * 2 * kEndsBuffers, kOutBytes = kOutOne * 2 * kOutBuffers;
+  static_assert(kOutBytes + kSumBytes <= kLds && kEndsBytes + kSumBytes <= kLds, "LDS");
 };
 
-struct DecayWs {
-  float* ends;   // [slot][head][Dk][Dv]: the states from zeros at the tiles' ends, then those before the tiles
-  float* keeps;  // [slot][head]: the decay over a tile
+// A launch's arguments: heads of q, k and v as how many neighbouring heads share one.
+struct DecayDev {
+  const void *q, *k, *v;
+  void* out;
+  const float *decay, *gates;
+  float *state, *ends, *keeps;  // ends [slot][head][Dk][Dv]: the states from zeros at the tiles' ends, then those
+  size_t ldq, ldk, ldv, ldo, ldg;  // before the tiles; keeps [slot][head]: the decay over a tile
+  int heads, q_each, k_each, v_each, Dk, Dv;
+  float scale;
 };
 
-template <int DT, int DKP, int NT, int PASS>
-__global__ __launch_bounds__(256, DT == kBF16 && DKP <= 128 ? 2 : 1) void k_decay(DecayArgs a, DecayTab t, DecayWs ws) {
-  using Sh = DecayShape<DT, DKP, NT>;
+template <int DT, int DKP, int NW, int PASS>
+__global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
+  using Sh = DecayShape<DT, DKP, NW>;
   using E = Elem<DT>;
   using T = typename E::T;
-  constexpr int C = Sh::C, DVP = Sh::DVP, N = Sh::N, NS = Sh::NS, KT = DKP / 16;
-  extern __shared__ __align__(16) uint16_t lds[];
-  uint16_t* const sK = lds;
-  uint16_t* const sV = lds + Sh::kRowTile;
-  uint16_t* const sQ = sV + Sh::kColTile;      // of kOutputs alone
-  uint16_t* const sP = sQ + Sh::kRowTile;      // [slab][step][part][lane][8]
-  __shared__ double sG[2][C];
-  __shared__ float sFrom[2][C], sTo[2][C];     // exp(G_i), exp(G - G_i)
+  constexpr int C = kChunk, DVP = Sh::DVP, N = Sh::N, NS = Sh::NS, KT = DKP / 16;
+  constexpr int kBuffers = PASS == kEnds ? Sh::kEndsBuffers : Sh::kOutBuffers, kOne = PASS == kEnds ? Sh::kEndsOne : Sh::kOutOne;
+  extern __shared__ __align__(16) uint16_t lds[];  // a buffer: k, v, and of kOutputs q and the weights [slab][part][lane][8]
+  __shared__ double sG[NW][C];
+  __shared__ float sFrom[NW][C], sTo[NW][C];       // exp(G_i), exp(G - G_i)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
 
   // this block's sequence and rows
-  int at = 0;
-  for (int i = 0; i < t.n; i += 64) at += __popcll(__ballot(i + lane < t.n && t.tile[i + lane] <= static_cast<int>(blockIdx.x)));
-  const int s = __builtin_amdgcn_readfirstlane(at - 1);
-  const int p0 = (blockIdx.x - t.tile[s]) * t.step, len = t.len[s], p1 = min(p0 + t.step, len);
+  int s = 0;
+  DecaySeq seq = t.of[0];
+  if (t.n > 1) {
+    for (int i = 0; i < t.n; i += 64)
+      s += __popcll(__ballot(i + lane < t.n && t.of[min(i + lane, kDecaySeqs - 1)].tile <= static_cast<int>(blockIdx.x)));
+    s = __builtin_amdgcn_readfirstlane(s - 1);
+    seq = t.of[s];
+  }
+  const int p0 = (blockIdx.x - seq.tile) * t.step, len = seq.len, p1 = min(p0 + t.step, len);
   if (PASS == kEnds && p1 == len) return;  // nothing comes after the last tile
-  const int slices = static_cast<int>((a.Dv + DVP - 1) / DVP);
-  const size_t head = blockIdx.y / slices;
-  const int Dk = static_cast<int>(a.Dk), Dv = static_cast<int>(a.Dv), c0 = blockIdx.y % slices * DVP;
-  const size_t first = t.row[s] + p0;
-  const T* qp = static_cast<const T*>(a.q) + first * a.ldq + head / (a.heads / a.q_heads) * a.Dk;
-  const T* kp = static_cast<const T*>(a.k) + first * a.ldk + head / (a.heads / a.k_heads) * a.Dk;
-  const T* vp = static_cast<const T*>(a.v) + first * a.ldv + head / (a.heads / a.v_heads) * a.Dv + c0;
-  T* out = static_cast<T*>(a.out) + first * a.ldo + head * a.Dv;
+  const int Dk = a.Dk, Dv = a.Dv, head = blockIdx.z, c0 = blockIdx.y * DVP;
+  const size_t first = seq.row + p0;
+  const T* qp = static_cast<const T*>(a.q) + first * a.ldq + head / a.q_each * Dk;
+  const T* kp = static_cast<const T*>(a.k) + first * a.ldk + head / a.k_each * Dk;
+  const T* vp = static_cast<const T*>(a.v) + first * a.ldv + head / a.v_each * Dv + c0;
+  T* out = static_cast<T*>(a.out) + first * a.ldo + head * Dv;
   const float* gates = a.gates ? a.gates + first * a.ldg + head : nullptr;
   const double decay = a.decay ? a.decay[head] : 0.0;
-  const int rows = p1 - p0, vcols = Dv - c0;
+  const int rows = p1 - p0;
   const bool cut_up = s < t.many, last = p1 == len;
-  float* slot = cut_up ? ws.ends + (blockIdx.x * a.heads + head) * a.Dk * a.Dv : nullptr;
-  float* state = a.state ? a.state + (static_cast<size_t>(t.seq[s]) * a.heads + head) * a.Dk * a.Dv : nullptr;
+  const int held = Dk * Dv;
+  float* slot = cut_up ? a.ends + (static_cast<size_t>(blockIdx.x) * a.heads + head) * held : nullptr;
+  float* state = a.state ? a.state + (static_cast<size_t>(seq.seq) * a.heads + head) * held : nullptr;
   float* put = PASS == kEnds ? slot : last ? state : nullptr;
 
-  Tile<DT, C, DKP> tk, tq;
-  Tile<DT, C, DVP> tv;
+  Tile<DT, DKP, 64 * NW> tk, tq;
+  Tile<DT, DVP, 64 * NW> tv;
+  const int vcols = min(Dv - c0, DVP);
+  const T* const kt = tk.place(kp, a.ldk, Dk);
+  const T* const vt = tv.place(vp, a.ldv, vcols);
+  const T* const qt = tq.place(qp, a.ldq, Dk);
   auto fetch = [&](int p) {
-    tk.fetch(kp + p * a.ldk, a.ldk, rows - p, Dk);
-    tv.fetch(vp + p * a.ldv, a.ldv, rows - p, vcols);
-    if (PASS == kOutputs) tq.fetch(qp + p * a.ldq, a.ldq, rows - p, Dk);
-  };
-  // the decays of the chunk from row p on, by one wave: running sums of its lanes' rows
-  auto gate_of = [&](int p) { return gates && lane < C && p + lane < rows ? gates[static_cast<size_t>(p + lane) * a.ldg] : 0.0f; };
-  double total = 0.0;
-  auto sums = [&](int p, int b, float gate) {
-    double x = lane < C && p + lane < rows ? log2_step(decay + gate) : 0.0;
-#pragma unroll
-    for (int n = 1; n < C; n *= 2) {
-      const double y = __shfl_up(x, n);
-      if (lane >= n) x += y;
-    }
-    const double end = __shfl(x, C - 1);
-    total += end;
-    if (lane < C) {
-      sG[b][lane] = x;
-      sFrom[b][lane] = exp2_fast(static_cast<float>(x));
-      sTo[b][lane] = exp2_fast(static_cast<float>(end - x));
-    }
+    tk.fetch(kt + p * a.ldk, kp + p * a.ldk, a.ldk, rows - p, Dk);
+    tv.fetch(vt + p * a.ldv, vp + p * a.ldv, a.ldv, rows - p, vcols);
+    if (PASS == kOutputs) tq.fetch(qt + p * a.ldq, qp + p * a.ldq, a.ldq, rows - p, Dk);
   };
   fetch(0);
-  if (wave == 0) sums(0, 0, gate_of(0));
+  // the decays of the next NW chunks, one by each wave: running sums of its lanes' rows
+  double total = 0.0;
+  auto gate_of = [&](int p) {
+    const int r = p + wave * C + (lane & (C - 1));
+    return gates ? gates[min(r, rows - 1) * a.ldg] : 0.0f;
+  };
+  auto sums = [&](int p, float gate) {
+    const bool in = lane < C && p + wave * C + lane < rows;
+    const double x = running_sum(in ? log2_step(decay + gate) : 0.0), end = __shfl(x, C - 1);
+    total += end;
+    if (lane < C) {
+      sG[wave][lane] = x;
+      sFrom[wave][lane] = exp2_fast(static_cast<float>(x));
+      sTo[wave][lane] = exp2_fast(static_cast<float>(end - x));
+    }
+  };
+  float gate = gate_of(0);
 
-  // the state of this wave's columns
-  const int n0 = wave * NT * 16;  // of the block's
-  f32x4 S[KT][NT];
+  // the state of this wave's columns: lane l, column l % 16, rows 4 (l / 16) + e of each 16
+  const int n0 = wave * 16, col = c0 + n0 + c;
+  f32x4 S[KT] = {};
   const float* from = PASS == kEnds ? nullptr : cut_up ? slot : state;
+  const bool whole = Dk == DKP && c0 + DVP <= Dv;  // no row or column of the state is past its end
+  const uint32_t own = (4 * g * Dv + col) * 4;
+  if (from && whole) {
 #pragma unroll
-  for (int k = 0; k < KT; ++k)
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < 4; ++e) S[k][e] = at_bytes(from + (k * 16 + e) * Dv, own);
+  } else if (from) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = k * 16 + 4 * g + e, col = c0 + n0 + n * 16 + c;
-        S[k][n][e] = from && row < Dk && col < Dv ? from[static_cast<size_t>(row) * Dv + col] : 0.0f;
+        const int row = k * 16 + 4 * g + e;
+        const float f = at_bytes(from, (min(row, Dk - 1) * Dv + min(col, Dv - 1)) * 4);
+        S[k][e] = row < Dk && col < Dv ? f : 0.0f;
       }
+  }
   bool any = from != nullptr;  // the state may be other than 0
-
-  for (int p = 0, b = 0; p < rows; p += C, b ^= 1) {
-    __syncthreads();
-    tk.store(sK);
-    tv.store(sV);
-    if (PASS == kOutputs) tq.store(sQ);
-    __syncthreads();
-    const bool more = p + C < rows;
-    float gate = 0.0f;
-    if (more) {
-      fetch(p + C);
-      if (wave == 0) gate = gate_of(p + C);
+  T* const mine = out + c * a.ldo + c0 + n0 + 4 * g;
+  auto store = [&](int b) {
+    uint16_t* to = lds + b * kOne;
+    tk.store(to);
+    tv.store(to + Sh::kRowTile);
+    if (PASS == kOutputs) tq.store(to + Sh::kRowTile + Sh::kColTile);
+  };
+  // two buffers: a chunk's rows are stored while the one before is multiplied
+  if (kBuffers == 2) {
+    store(0);
+    if (C < rows) fetch(C);
+  }
+  for (int p = 0, ch = 0, buf = 0; p < rows; p += C) {
+    if (ch == 0) {
+      if (kBuffers == 2 && p) __syncthreads();  // the last chunk's readers of the sums
+      if (kBuffers == 1) __syncthreads();
+      sums(p, gate);
+      if (p + NW * C < rows) gate = gate_of(p + NW * C);
+    } else if (kBuffers == 1) {
+      __syncthreads();
     }
-    f32x4 O[Sh::kSlabs][NT] = {};
+    if (kBuffers == 1) store(0);
+    if (kBuffers == 1 || ch == 0) __syncthreads();
+    const int b = ch;
+    const bool more = p + C < rows;
+    if (kBuffers == 1 && more) fetch(p + C);
+    uint16_t* const sK = lds + buf * kOne;
+    uint16_t* const sV = sK + Sh::kRowTile;
+    uint16_t* const sQ = sV + Sh::kColTile;
+    uint16_t* const sP = sQ + Sh::kRowTile;
+    f32x4 O[2] = {};
     if constexpr (PASS == kOutputs) {
-      // weights of rows 16 wave.. of the chunk: lane l, row i, inputs j = 16 jt + 4 g + e
-      if (wave < Sh::kSlabs) {
-        f32x4 W[Sh::kSlabs] = {};
+      // Weights of the chunk's rows (16 slab + i) by rows (16 jt + j): three of the four tiles hold any, a wave each; lane l, row
+      // l % 16, inputs 4 g + e. The tile that stands for later rows is 0.
+      if (wave < 3) {
+        const int slab = wave ? 1 : 0, jt = wave == 2;
+        f32x4 W = {};
 #pragma unroll
         for (int ks = 0; ks < DKP / 32; ++ks) {
           bf16x8 q[N], k[N];
 #pragma unroll
-          for (int i = 0; i < N; ++i) q[i] = by_columns<DKP>(sQ + i * C * DKP, wave * 16, ks * 32, lane);
-#pragma unroll
-          for (int jt = 0; jt < Sh::kSlabs; ++jt) {
-            if (jt > wave) break;
-#pragma unroll
-            for (int i = 0; i < N; ++i) k[i] = by_columns<DKP>(sK + i * C * DKP, jt * 16, ks * 32, lane);
-            mma<N, N>(k, q, W[jt]);
+          for (int i = 0; i < N; ++i) {
+            q[i] = by_columns<DKP>(sQ + i * C * DKP, slab * 16, ks * 32, lane);
+            k[i] = by_columns<DKP>(sK + i * C * DKP, jt * 16, ks * 32, lane);
           }
+          mma<N, N>(k, q, W);
         }
-        const int i = wave * 16 + c;
+        const int i = slab * 16 + c;
         const double Gi = sG[b][i];
+        u16x4 part[NS];
 #pragma unroll
-        for (int js = 0; js < Sh::kSteps; ++js) {
-          if (2 * js > wave) break;
-          float w[8];
+        for (int e = 0; e < 4; ++e) {
+          const int j = jt * 16 + 4 * g + e;
+          const float d = exp2_fast(static_cast<float>(Gi - sG[b][j]));
+          uint16_t w[NS];
+          cut<NS>(j <= i ? W[e] * d : 0.0f, w);  // (rows after i may hold anything)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int j = js * 32 + (e >> 2) * 16 + 4 * g + (e & 3);
-            const float d = exp2_fast(static_cast<float>(Gi - sG[b][j]));
-            w[e] = j <= i ? W[2 * js + (e >> 2)][e & 3] * d : 0.0f;  // (rows after i may hold anything)
-          }
-          bf16x8 part[NS];
-          cut8<NS>(w, part);
+          for (int k = 0; k < NS; ++k) part[k][e] = w[k];
+        }
 #pragma unroll
-          for (int k = 0; k < NS; ++k)
-            *reinterpret_cast<bf16x8*>(sP + (((wave * Sh::kSteps + js) * NS + k) * 64 + lane) * 8) = part[k];
+        for (int k = 0; k < NS; ++k) {
+          uint16_t* to = sP + ((slab * NS + k) * 64 + lane) * 8;
+          *reinterpret_cast<u16x4*>(to + jt * 4) = part[k];
+          if (wave == 0) *reinterpret_cast<u16x4*>(to + 4) = u16x4{};
         }
       }
+    }
+    if constexpr (PASS == kOutputs) {
       // what the state gives: lane l, row 16 slab + l % 16, columns 4 g + e
       if (any) {
 #pragma unroll
         for (int ks = 0; ks < DKP / 32; ++ks) {
-          bf16x8 h[NT][NS];
+          float f[8];
+          bf16x8 h[NS];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float v[8];
+          for (int e = 0; e < 8; ++e) f[e] = S[2 * ks + (e >> 2)][e & 3];
+          cut8<NS>(f, h);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = S[2 * ks + (e >> 2)][n][e & 3];
-            cut8<NS>(v, h[n]);
-          }
-#pragma unroll
-          for (int sl = 0; sl < Sh::kSlabs; ++sl) {
+          for (int sl = 0; sl < 2; ++sl) {
             bf16x8 q[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) q[i] = by_columns<DKP>(sQ + i * C * DKP, sl * 16, ks * 32, lane);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma<NS, N>(h[n], q, O[sl][n]);
+            mma<NS, N>(h, q, O[sl]);
           }
         }
 #pragma unroll
-        for (int sl = 0; sl < Sh::kSlabs; ++sl) {
-          const float f = sFrom[b][sl * 16 + c];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) O[sl][n] *= f;
-        }
+        for (int sl = 0; sl < 2; ++sl) O[sl] *= sFrom[b][sl * 16 + c];
       }
       __syncthreads();
     }
+    if (kBuffers == 2 && more) {
+      store(buf ^ 1);
+      if (p + 2 * C < rows) fetch(p + 2 * C);
+    }
     // this wave's columns of v, as an operand over rows. A weight of 0 would make a NaN of an infinity or NaN in a row that
     // comes later: such numbers are taken out, and the outputs from their row on have none
-    bf16x8 v[Sh::kSteps][NT][N];
-    bool odd = false;
+    bf16x8 v[N];
+    uint32_t odd = 0;
 #pragma unroll
-    for (int js = 0; js < Sh::kSteps; ++js)
+    for (int i = 0; i < N; ++i) v[i] = by_rows<DVP>(sV + i * C * DVP, 0, n0, lane);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+    for (int e = 0; e < 4; ++e) odd |= (__builtin_bit_cast(u32x4, v[0])[e] & 0x7F807F80u) + 0x00800080u;  // an exponent of all ones carries
+    int from_row = C;  // the first row without a number of this lane's column
+    const bool some = __ballot(odd & 0x80008000u) != 0;
+    if (some) {
+      u16x8 h[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[js][n][i] = by_rows<DVP>(sV + i * C * DVP, js * 32, n0 + n * 16, lane);
-        const u16x8 h = __builtin_bit_cast(u16x8, v[js][n][0]);
+      for (int i = 0; i < N; ++i) h[i] = __builtin_bit_cast(u16x8, v[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) odd |= (h[e] & 0x7F80) == 0x7F80;
-      }
-    int from_row[NT];  // the first row without a number of this lane's column
+      for (int e = 0; e < 8; ++e)
+        if ((h[0][e] & 0x7F80) == 0x7F80) {
+          from_row = min(from_row, (e >> 2) * 16 + 4 * g + (e & 3));
 #pragma unroll
-    for (int n = 0; n < NT; ++n) from_row[n] = C;
-    odd = __ballot(odd) != 0;
-    if (odd) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int js = 0; js < Sh::kSteps; ++js) {
-          u16x8 h[N];
-#pragma unroll
-          for (int i = 0; i < N; ++i) h[i] = __builtin_bit_cast(u16x8, v[js][n][i]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if ((h[0][e] & 0x7F80) == 0x7F80) {
-              from_row[n] = min(from_row[n], js * 32 + (e >> 2) * 16 + 4 * g + (e & 3));
-#pragma unroll
-              for (int i = 0; i < N; ++i) h[i][e] = 0;
-            }
-#pragma unroll
-          for (int i = 0; i < N; ++i) v[js][n][i] = __builtin_bit_cast(bf16x8, h[i]);
+          for (int i = 0; i < N; ++i) h[i][e] = 0;
         }
-        from_row[n] = min(from_row[n], __shfl_xor(from_row[n], 16));
-        from_row[n] = min(from_row[n], __shfl_xor(from_row[n], 32));
-      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = __builtin_bit_cast(bf16x8, h[i]);
+      from_row = min(from_row, __shfl_xor(from_row, 16));
+      from_row = min(from_row, __shfl_xor(from_row, 32));
     }
     if constexpr (PASS == kOutputs) {
-#pragma unroll
-      for (int sl = 0; sl < Sh::kSlabs; ++sl) {
-#pragma unroll
-        for (int js = 0; js < Sh::kSteps; ++js) {
-          if (2 * js > sl) break;
-          bf16x8 w[NS];
-#pragma unroll
-          for (int k = 0; k < NS; ++k)
-            w[k] = *reinterpret_cast<const bf16x8*>(sP + (((sl * Sh::kSteps + js) * NS + k) * 64 + lane) * 8);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma<N, NS>(v[js][n], w, O[sl][n]);
-        }
-      }
-      if (odd) {
-#pragma unroll
-        for (int sl = 0; sl < Sh::kSlabs; ++sl)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (sl * 16 + c >= __shfl(from_row[n], 4 * g + e)) O[sl][n][e] = __builtin_nanf("");
-      }
       typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 #pragma unroll
-      for (int sl = 0; sl < Sh::kSlabs; ++sl) {
-        const int r = p + sl * 16 + c;
+      for (int sl = 0; sl < 2; ++sl) {
+        bf16x8 w[NS];
+#pragma unroll
+        for (int k = 0; k < NS; ++k) w[k] = *reinterpret_cast<const bf16x8*>(sP + ((sl * NS + k) * 64 + lane) * 8);
+        mma<N, NS>(v, w, O[sl]);
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (sl * 16 + c >= __shfl(from_row, 4 * g + e)) O[sl][e] = __builtin_nanf("");
+        }
+        const int r = p + sl * 16 + c, first_col = c0 + n0 + 4 * g;
         if (r >= rows) continue;
+        T* to = mine + (p + sl * 16) * a.ldo;
+        T4 o;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int col = c0 + n0 + n * 16 + 4 * g;
-          T4 o;
+        for (int e = 0; e < 4; ++e) o[e] = E::down(O[sl][e] * a.scale);
+        if (first_col + 4 <= Dv) {
+          *reinterpret_cast<T4*>(to) = o;
+        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = E::down(O[sl][n][e] * a.scale);
-          T* to = out + r * a.ldo + col;
-          if (col + 4 <= Dv) {
-            *reinterpret_cast<T4*>(to) = o;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + e < Dv) to[e] = o[e];
-          }
+          for (int e = 0; e < 4; ++e)
+            if (first_col + e < Dv) to[e] = o[e];
         }
       }
     }
     if (PASS == kEnds || more || put) {
-      const float keep = sFrom[b][C - 1];
       if (any) {
+        const float keep = sFrom[b][C - 1];
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) S[k][n] *= keep;
+        for (int k = 0; k < KT; ++k) S[k] *= keep;
       }
       any = true;
+      bf16x8 w[3];
+      float f[8];
 #pragma unroll
-      for (int js = 0; js < Sh::kSteps; ++js) {
-        float to[8];
+      for (int e = 0; e < 8; ++e) {
+        f[e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = sTo[b][js * 32 + (e >> 2) * 16 + 4 * g + (e & 3)];
-        bf16x8 w[NT][3];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float f[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] = 0.0f;
-#pragma unroll
-            for (int i = N - 1; i >= 0; --i) f[e] += Elem<kBF16>::up(__builtin_bit_cast(u16x8, v[js][n][i])[e]);
-            f[e] *= to[e];
-          }
-          cut8<3>(f, w[n]);
-        }
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          bf16x8 kk[N];
-#pragma unroll
-          for (int i = 0; i < N; ++i) kk[i] = by_rows<DKP>(sK + i * C * DKP, js * 32, k * 16, lane);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma<N, 3>(kk, w[n], S[k][n]);
-        }
+        for (int i = N - 1; i >= 0; --i) f[e] += Elem<kBF16>::up(__builtin_bit_cast(u16x8, v[i])[e]);
+        f[e] *= sTo[b][(e >> 2) * 16 + 4 * g + (e & 3)];
       }
-      if (odd) {
+      cut8<3>(f, w);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          if (from_row[n] < C) {
+      for (int k = 0; k < KT; ++k) {
+        bf16x8 kk[N];
 #pragma unroll
-            for (int k = 0; k < KT; ++k) S[k][n] = f32x4{} + __builtin_nanf("");
-          }
+        for (int i = 0; i < N; ++i) kk[i] = by_rows<DKP>(sK + i * C * DKP, 0, k * 16, lane);
+        mma<N, 3>(kk, w, S[k]);
+      }
+      if (some && from_row < C) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k) S[k] = f32x4{} + __builtin_nanf("");
       }
     }
-    if (more && wave == 0) sums(p + C, b ^ 1, gate);
+    if (kBuffers == 2) {
+      buf ^= 1;
+      if (more && ch != NW - 1) __syncthreads();
+    }
+    ch = ch == NW - 1 ? 0 : ch + 1;
   }
-  if (put) {
+  if (put && whole) {
 #pragma unroll
     for (int k = 0; k < KT; ++k)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < 4; ++e) at_bytes(put + (k * 16 + e) * Dv, own) = S[k][e];
+  } else if (put && col < Dv) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = k * 16 + 4 * g + e, col = c0 + n0 + n * 16 + c;
-          if (row < Dk && col < Dv) put[static_cast<size_t>(row) * Dv + col] = S[k][n][e];
-        }
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k * 16 + 4 * g + e < Dk) at_bytes(put + (k * 16 + e) * Dv, own) = S[k][e];
   }
-  if (PASS == kEnds && threadIdx.x == 0 && c0 == 0) ws.keeps[blockIdx.x * a.heads + head] = exp2_fast(static_cast<float>(total));
+  if (PASS == kEnds && blockIdx.y == 0) {  // each wave has the sums of its chunks
+    __syncthreads();
+    if (lane == 0) sG[wave][0] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      total = 0.0;
+      for (int w = 0; w < NW; ++w) total += sG[w][0];
+      a.keeps[static_cast<size_t>(blockIdx.x) * a.heads + head] = exp2_fast(static_cast<float>(total));
+    }
+  }
 }
 
 // The states before the tiles in the place of those at their ends, in order: a thread an element, a head and a sequence of
 // more than one tile a row of blocks, kBatch tiles' loads in flight.
-__global__ __launch_bounds__(256) void k_decay_carry(DecayArgs a, DecayTab t, DecayWs ws) {
+__global__ __launch_bounds__(256) void k_decay_carry(DecayDev a, DecayTab t) {
   constexpr int kBatch = 8;
   const size_t n = a.Dk * a.Dv, i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n) return;
-  const int s = blockIdx.z, tiles = t.tile[s + 1] - t.tile[s];
+  const DecaySeq seq = t.of[blockIdx.z];
+  const int tiles = (seq.len + t.step - 1) / t.step;
   const size_t head = blockIdx.y, step = a.heads * n;
-  float* ends = ws.ends + (t.tile[s] * a.heads + head) * n + i;
-  const float* keeps = ws.keeps + t.tile[s] * a.heads + head;
-  float h = a.state ? a.state[(static_cast<size_t>(t.seq[s]) * a.heads + head) * n + i] : 0.0f;
+  float* ends = a.ends + (static_cast<size_t>(seq.tile) * a.heads + head) * n + i;
+  const float* keeps = a.keeps + static_cast<size_t>(seq.tile) * a.heads + head;
+  float h = a.state ? a.state[(static_cast<size_t>(seq.seq) * a.heads + head) * n + i] : 0.0f;
   for (int j = 0; j < tiles; j += kBatch) {
     float e[kBatch], f[kBatch];
 #pragma unroll
@@ -604,34 +650,37 @@ __global__ __launch_bounds__(256) void k_decay_carry(DecayArgs a, DecayTab t, De
   }
 }
 
-template <int DT, int DKP, int NT>
-hipError_t tiles_launch(const DecayArgs& a, const DecayTab& t, const DecayWs& ws, hipStream_t s) {
-  using Sh = DecayShape<DT, DKP, NT>;
-  const unsigned heads = static_cast<unsigned>(a.heads), slices = static_cast<unsigned>((a.Dv + Sh::DVP - 1) / Sh::DVP);
+template <int DT, int DKP, int NW>
+hipError_t tiles_launch(const DecayDev& a, const DecayTab& t, hipStream_t s) {
+  using Sh = DecayShape<DT, DKP, NW>;
+  const unsigned heads = a.heads, slices = (a.Dv + Sh::DVP - 1) / Sh::DVP;
   hipError_t e;
   if (t.many) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NT, kEnds>), hipFuncAttributeMaxDynamicSharedMemorySize,
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kEnds>), hipFuncAttributeMaxDynamicSharedMemorySize,
                             Sh::kEndsBytes);
     if (e != hipSuccess) return e;
-    k_decay<DT, DKP, NT, kEnds><<<dim3(t.tile[t.many], heads * slices), 256, Sh::kEndsBytes, s>>>(a, t, ws);
+    k_decay<DT, DKP, NW, kEnds><<<dim3(t.cut_tiles, slices, heads), 64 * NW, Sh::kEndsBytes, s>>>(a, t);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    k_decay_carry<<<dim3(static_cast<unsigned>((a.Dk * a.Dv + 255) / 256), heads, t.many), 256, 0, s>>>(a, t, ws);
+    k_decay_carry<<<dim3((a.Dk * a.Dv + 255) / 256, heads, t.many), 256, 0, s>>>(a, t);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NT, kOutputs>), hipFuncAttributeMaxDynamicSharedMemorySize,
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kOutputs>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           Sh::kOutBytes);
   if (e != hipSuccess) return e;
-  k_decay<DT, DKP, NT, kOutputs><<<dim3(t.tile[t.n], heads * slices), 256, Sh::kOutBytes, s>>>(a, t, ws);
+  k_decay<DT, DKP, NW, kOutputs><<<dim3(t.tiles, slices, heads), 64 * NW, Sh::kOutBytes, s>>>(a, t);
   return hipGetLastError();
 }
 
 template <int DT>
-hipError_t tiles_of(const DecayArgs& a, const DecayTab& t, float* ws_mem, hipStream_t s) {
-  DecayWs ws{ws_mem, ws_mem ? ws_mem + static_cast<size_t>(t.tile[t.many]) * a.heads * a.Dk * a.Dv : nullptr};
+hipError_t tiles_of(const DecayArgs& a, const DecayTab& t, float* ws, hipStream_t s) {
+  DecayDev d{a.q, a.k, a.v, a.out, a.decay, a.gates, a.state, ws, nullptr, a.ldq, a.ldk, a.ldv, a.ldo, a.ldg,
+             static_cast<int>(a.heads), static_cast<int>(a.heads / a.q_heads), static_cast<int>(a.heads / a.k_heads),
+             static_cast<int>(a.heads / a.v_heads), static_cast<int>(a.Dk), static_cast<int>(a.Dv), a.scale};
+  if (t.many) d.keeps = ws + static_cast<size_t>(t.cut_tiles) * a.heads * a.Dk * a.Dv;
   const bool wide = a.Dv > 64;
-  if (a.Dk <= 64) return wide ? tiles_launch<DT, 64, 2>(a, t, ws, s) : tiles_launch<DT, 64, 1>(a, t, ws, s);
-  if (a.Dk <= 128) return wide ? tiles_launch<DT, 128, 2>(a, t, ws, s) : tiles_launch<DT, 128, 1>(a, t, ws, s);
-  return wide ? tiles_launch<DT, 256, 2>(a, t, ws, s) : tiles_launch<DT, 256, 1>(a, t, ws, s);
+  if (a.Dk <= 64) return wide ? tiles_launch<DT, 64, 8>(d, t, s) : tiles_launch<DT, 64, 4>(d, t, s);
+  if (a.Dk <= 128) return wide ? tiles_launch<DT, 128, 8>(d, t, s) : tiles_launch<DT, 128, 4>(d, t, s);
+  return wide ? tiles_launch<DT, 256, 8>(d, t, s) : tiles_launch<DT, 256, 4>(d, t, s);
 }
 
 }  // namespace

@@ -166,16 +166,16 @@ inline const char* check(DecayArgs& a) {
 // a block's share of a long sequence); those of more than one tile stand first, so that their tiles are numbered from 0
 // and only they need slots of the workspace.
 constexpr int kDecaySeqs = 192;
+struct DecaySeq {
+  int row, len, seq, tile;       // tile: its first
+};
 struct DecayTab {
   int n, step, many;             // sequences, rows of a tile, sequences of more than one tile
-  int row[kDecaySeqs], len[kDecaySeqs], seq[kDecaySeqs];
-  int tile[kDecaySeqs + 1];      // first tile of each; behind the last, their number
-};
-struct DecaySeq {
-  int row, len, seq;
+  int tiles, cut_tiles;          // of all sequences, and of those of more than one
+  DecaySeq of[kDecaySeqs];
 };
 // Rows that a block multiplies at a time.
-inline int decay_chunk(int dtype) { return dtype == kBF16 ? 64 : 32; }
+constexpr int kDecayChunk = 32;
 // The table of n sequences cut into tiles of `step` rows.
 inline void fill_decay(DecayTab& t, const DecaySeq* s, int n, int step) {
   t.n = n;
@@ -184,20 +184,21 @@ inline void fill_decay(DecayTab& t, const DecaySeq* s, int n, int step) {
   for (int pass = 0; pass < 2; ++pass) {
     for (int i = 0; i < n; ++i) {
       if ((s[i].len > step) != (pass == 0)) continue;
-      t.row[k] = s[i].row;
-      t.len[k] = s[i].len;
-      t.seq[k] = s[i].seq;
-      t.tile[k++] = tiles;
+      t.of[k] = s[i];
+      t.of[k++].tile = tiles;
       tiles += (s[i].len + step - 1) / step;
     }
-    if (pass == 0) t.many = k;
+    if (pass == 0) {
+      t.many = k;
+      t.cut_tiles = tiles;
+    }
   }
-  t.tile[k] = tiles;
+  t.tiles = tiles;
 }
 // Rows of a tile: so many that the tiles of all heads fill the chip twice, and that those of long sequences have room in
 // the workspace. No sequence is cut into two: that would be three launches for one.
 inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
-  const int chunk = decay_chunk(a.dtype);
+  constexpr int chunk = kDecayChunk;
   size_t chunks = 0;
   int most = 0;
   for (int i = 0; i < n; ++i) {
@@ -238,7 +239,7 @@ R each_decay(const DecayArgs& a, R ok, Steps&& steps, Tiles&& tiles) {
     const int len = static_cast<int>(a.lens ? a.lens[i] : a.rows / a.seqs);
     if (!len) continue;
     const bool is_few = len <= kDecayShort;
-    (is_few ? few[nf++] : many[nm++]) = {row, len, static_cast<int>(i)};
+    (is_few ? few[nf++] : many[nm++]) = {row, len, static_cast<int>(i), 0};
     row += len;
     if ((is_few ? nf : nm) == kDecaySeqs) flush(is_few);
   }
