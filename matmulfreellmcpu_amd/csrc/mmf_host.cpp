@@ -1717,7 +1717,7 @@ int mmf_w8_linear(mmf_ctx* c, int id, const int8_t* x, const float* xscales, con
     const W8& w = w8_of(c, id);
     W8Args a{out_dtype, x, xscales, bias, out, rows, ldx, ldo};
     refuse(check(a, w.g.N, w.g.K));
-    MMF_HIP(launch_w8(a, w.g, w.codes, w.scales, nullptr, c->stream));
+    MMF_HIP(launch_w8(a, w.g, w.codes, w.scales, c->stream));
   });
 }
 

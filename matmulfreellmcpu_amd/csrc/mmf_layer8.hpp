@@ -37,6 +37,23 @@ MMF_HD inline size_t w8_at(const W8Geom& g, size_t n, size_t k) {
   return ((n / 32 * g.nk + k / 32) * 64 + n % 32 + 32 * (k / 16 % 2)) * 16 + k % 16;
 }
 
+// The kernel of a call: few rows by blocks of 16 outputs, or tiles of 32 x 128 (two or four groups of waves share the
+// inputs), 64 x 128 and 128 x 256 rows and outputs. Lines by measured times (us):
+//   rows       24 x 6912 x 2560 7.8, tiles of 32 12.7; 40 x 2048 x 2048 5.2 and 6.6; 33 x 2048 x 11264 10.7 and 7.1
+//   32, four   64 x 6912 x 2560 12.8 (two groups 14.1); 64 x 2048 x 11264 7.4 (7.2)
+//   64         512 x 6912 x 2560 22.8, tiles of 32 24.9; 512 x 2048 x 11264 23.0 and 27.1; 256 x 2048 x 11264 15.3 and 15.3
+//   128        2048 x 2048 x 11264 58.7, tiles of 64 67; 2048 x 2560 x 6912 48 and 55; 512 x 2048 x 11264 23.5 and 21 to 23
+enum W8Way { kW8Rows, kW8Tile32x4, kW8Tile32, kW8Tile64, kW8Tile128 };
+inline W8Way w8_way(const W8Geom& g, size_t rows) {
+  const size_t weights = static_cast<size_t>(g.N) * g.K;
+  auto tiles = [&](size_t r, size_t n) { return (rows + r - 1) / r * ((g.N + n - 1) / n); };
+  if (rows <= 16 || (rows <= 32 && weights < (size_t{20} << 20)) || (rows <= 64 && weights <= (size_t{6} << 20))) return kW8Rows;
+  if (tiles(128, 256) >= 256) return kW8Tile128;
+  if (tiles(32, 128) > 256) return kW8Tile64;
+  return g.nk >= 128 && tiles(32, 128) <= 128 ? kW8Tile32x4 : kW8Tile32;
+}
+constexpr size_t kW8RowsMost = 65535;  // of a launch: tiles count in 32 bits, and so does a grid's threads
+
 struct W8Args {
   int out_dtype;
   const int8_t* x;

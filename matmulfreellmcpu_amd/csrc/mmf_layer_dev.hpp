@@ -20,7 +20,7 @@ hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const ui
 hipError_t launch_w4(const W4Args& a, const W4Geom& g, const uint32_t* codes, const uint32_t* scales, char* ws,
                      hipStream_t s);
 hipError_t launch_w8_pack(const int8_t* codes, const W8Geom& g, int8_t* out, hipStream_t s);
-hipError_t launch_w8(const W8Args& a, const W8Geom& g, const int8_t* codes, const float* scales, char* ws, hipStream_t s);
+hipError_t launch_w8(const W8Args& a, const W8Geom& g, const int8_t* codes, const float* scales, hipStream_t s);
 hipError_t launch_block(const BlockArgs& a, hipStream_t s);
 // ws: kLayerWsBytes where decay_splits(a)
 hipError_t launch_decay(const DecayArgs& a, float* ws, hipStream_t s);

@@ -72,6 +72,25 @@ static void products() {
   }
 }
 
+// Every kernel is reached, and its grid counts fewer than 2^32 threads at the largest sizes.
+static void ways() {
+  auto way = [](size_t rows, size_t K, size_t N) { return static_cast<long>(w8_way(w8_geom(N, K), rows)); };
+  is("w8 one row", way(1, 2048, 11264), kW8Rows);
+  is("w8 16 rows of large weights", way(16, 131071, kMaxCols), kW8Rows);
+  is("w8 24 rows", way(24, 6912, 2560), kW8Rows);
+  is("w8 40 rows of small weights", way(40, 2048, 2048), kW8Rows);
+  is("w8 64 rows", way(64, 2048, 11264), kW8Tile32);
+  is("w8 64 rows of many inputs", way(64, 6912, 2560), kW8Tile32x4);
+  is("w8 512 rows", way(512, 6912, 2560), kW8Tile64);
+  is("w8 2048 rows", way(2048, 2048, 11264), kW8Tile128);
+  for (size_t rows : {size_t{65}, size_t{1000}, size_t{65535}})
+    for (size_t N : {size_t{1}, size_t{129}, kMaxCols}) {
+      const long w = way(rows, 4097, N);
+      const size_t r = w == kW8Tile128 ? 128 : w == kW8Tile64 ? 64 : 32, n = w == kW8Tile128 ? 256 : 128;
+      is("w8 grid", ((rows + r - 1) / r * ((N + n - 1) / n) + 8) * 1024 < (size_t{1} << 32), 1);
+    }
+}
+
 static void blocks() {
   auto go = [](const char* what, const char* part, auto&& change) {
     BlockArgs a{kF32, kActSilu, at<float>(0x10000), at<float>(0x20000), at<float>(0x30000), at<float>(0x900), at<float>(0x1900), at<float>(0x2900),
@@ -214,6 +233,7 @@ static void logps() {
 
 int main() {
   products();
+  ways();
   blocks();
   attention();
   logps();
