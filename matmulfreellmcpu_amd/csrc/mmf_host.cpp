@@ -1748,7 +1748,7 @@ int mmf_token_logprobs(mmf_ctx* c, const mmf_logp_args* s) {
                s->ld, s->temperature};
     refuse(check(a));
     if (!a.rows) return;
-    const bool parts = logp_plan(a.dtype, a.V).segs > 1;
+    const bool parts = logp_plan(a.dtype, a.V, a.rows).segs > 1;
     MMF_HIP(launch_logp(a, parts ? reinterpret_cast<float*>(layer_ws(c)) : nullptr, c->stream));
   });
 }
@@ -2243,7 +2243,7 @@ int mmf_model_score(mmf_ctx* c, const int64_t* ids, size_t T, float* logprobs, f
     const size_t n = T - 1, V = m.cfg.vocab_size;
     if (top > kMaxTop || top > V || (top && (!top_ids || !top_logprobs))) fail(MMF_ERR_ARG, "invalid top alternatives");
     check_ids(m, ids, T);
-    char* ws = logp_plan(kF32, V).segs > 1 ? layer_ws(c) : nullptr;
+    char* ws = logp_plan(kF32, V, n).segs > 1 ? layer_ws(c) : nullptr;
     const float* lg = forward_rows(c, m, ids, T);
     // top ids first: they are 8 bytes each
     int64_t* d_ids = reinterpret_cast<int64_t*>(m.rs.score.as<char>(n * (top * 12 + 8)));

@@ -312,17 +312,23 @@ inline const char* check(LogpArgs& a) {
   }
   return nullptr;
 }
-// A row is cut into `segs` parts of `vecs` vectors of 16 bytes for each of a block's kLogpThreads threads, which
-// hold them in registers.
-constexpr int kLogpThreads = 1024;
+// A row is cut into `segs` parts of at most kLogpPart logits, for blocks of `threads` threads, which hold `vecs` (1, 2, 4
+// or 8) vectors of 16 bytes each in registers. Many rows take small blocks, so that several rows are at work on a
+// compute unit; few rows large ones, so that each is soon done.
+constexpr size_t kLogpPart = 32768;
 struct LogpPlan {
-  int vecs, segs;
+  int threads, vecs, segs;
 };
-inline LogpPlan logp_plan(int dtype, size_t V) {
-  const size_t v = 16 / dtype_size(dtype), most = dtype == kF32 ? 8 : 4, all = (V + v - 1) / v;  // 32768 elements
-  for (size_t vecs = 1; vecs <= most; vecs *= 2)
-    if (all <= kLogpThreads * vecs) return {static_cast<int>(vecs), 1};
-  return {static_cast<int>(most), static_cast<int>((all + kLogpThreads * most - 1) / (kLogpThreads * most))};
+inline LogpPlan logp_plan(int dtype, size_t V, size_t rows) {
+  const size_t v = 16 / dtype_size(dtype), part = V < kLogpPart ? V : kLogpPart, all = (part + v - 1) / v;
+  const int segs = static_cast<int>((V + kLogpPart - 1) / kLogpPart);
+  for (size_t threads : {size_t{256}, size_t{512}, size_t{1024}}) {
+    if (rows * segs < 256 && threads < 1024) continue;
+    for (size_t vecs : {1, 2, 4, 8})
+      if (all <= threads * vecs && threads * vecs * v <= kLogpPart && (segs == 1 || threads * vecs * v == kLogpPart))
+        return {static_cast<int>(threads), static_cast<int>(vecs), segs};
+  }
+  return {0, 0, 0};
 }
 // Workspace of a row in several parts: for each its maximum, sum, weighted sum, and top values with their indices.
 inline size_t logp_row_floats(const LogpPlan& p, size_t top) { return p.segs > 1 ? p.segs * (4 + 2 * top) : 0; }

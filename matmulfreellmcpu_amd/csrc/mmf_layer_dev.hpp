@@ -24,7 +24,7 @@ hipError_t launch_w8(const W8Args& a, const W8Geom& g, const int8_t* codes, cons
 hipError_t launch_block(const BlockArgs& a, hipStream_t s);
 // ws: kLayerWsBytes where decay_splits(a)
 hipError_t launch_decay(const DecayArgs& a, float* ws, hipStream_t s);
-// ws: kLayerWsBytes where logp_plan(a.dtype, a.V).segs > 1
+// ws: kLayerWsBytes where logp_plan(a.dtype, a.V, a.rows).segs > 1
 hipError_t launch_logp(const LogpArgs& a, float* ws, hipStream_t s);
 
 // Element type DT of a row tensor: V neighbouring elements in one 16-byte access at any address that

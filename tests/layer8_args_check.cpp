@@ -221,14 +221,15 @@ static void logps() {
   go("logp top ids on top", "overlaps", [](LogpArgs& a) { a.top_ids = at<int64_t>(0x60000 + 72); });
   go("logp unused top on logits", nullptr, [](LogpArgs& a) { a.top = 0, a.top_logprobs = at<float>(0x10000); });
   for (int t : {kF32, kF16})
-    for (size_t V : {1, 100, 4096, 4097, 8192, 8193, 32000, 32768, 32769, 200000, 1048576}) {
-      const LogpPlan p = logp_plan(t, V);
-      const size_t part = static_cast<size_t>(p.vecs) * kLogpThreads * (16 / dtype_size(t));
-      is("logp plan holds the row", part * p.segs >= V && part * (p.segs - 1) < V, 1);
-      is("logp parts joined in one list", p.segs * kMaxTop <= 2048, 1);
-      is("logp pass", logp_rows_most(p, kMaxTop) > 0, 1);
-      is("logp workspace", logp_rows_most(p, kMaxTop) * logp_row_floats(p, kMaxTop) * 4 <= kLayerWsBytes, 1);
-    }
+    for (size_t rows : {1, 100, 5000})
+      for (size_t V : {1, 100, 4096, 4097, 8192, 8193, 16384, 16385, 32000, 32768, 32769, 65536, 200000, 1048576}) {
+        const LogpPlan p = logp_plan(t, V, rows);
+        const size_t part = static_cast<size_t>(p.threads) * p.vecs * (16 / dtype_size(t));
+        is("logp plan holds the row", part && part * p.segs >= V && part * (p.segs - 1) < V, 1);
+        is("logp parts joined in one list", p.segs * kMaxTop <= 2048, 1);
+        is("logp pass", logp_rows_most(p, kMaxTop) > 0, 1);
+        is("logp workspace", logp_rows_most(p, kMaxTop) * logp_row_floats(p, kMaxTop) * 4 <= kLayerWsBytes, 1);
+      }
 }
 
 int main() {
