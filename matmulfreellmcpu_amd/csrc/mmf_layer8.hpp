@@ -121,16 +121,16 @@ inline const char* check(BlockArgs& a) {
   }
   return nullptr;
 }
-// The kernel of a call: `threads` a row (whole waves), each with `vecs` (1, 2, 4 or 8) vectors of 16 bytes in
-// registers; threads 0: rows too long for that, read three times.
+// The kernel of a call: `threads` a row (whole waves), each with `vecs` (1 or 2) vectors of 16 bytes in registers;
+// threads 0: rows too long for that, read three times (from a cache).
 struct BlockPlan {
   int threads, vecs;
 };
 inline BlockPlan block_plan(int dtype, size_t cols) {
   const size_t v = 16 / dtype_size(dtype), all = (cols + v - 1) / v;
-  for (int vecs : {1, 2, 4, 8}) {
+  for (int vecs : {1, 2}) {
     const size_t t = ((all + vecs - 1) / vecs + 63) / 64 * 64;
-    if (t <= 512 || (vecs == 8 && t <= 1024)) return {static_cast<int>(t), vecs};
+    if (t <= 1024) return {static_cast<int>(t), vecs};
   }
   return {0, 0};
 }

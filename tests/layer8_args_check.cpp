@@ -135,8 +135,8 @@ static void blocks() {
     for (size_t cols = 1; cols < 70000; cols += cols < 5000 ? 1 : 97) {
       const BlockPlan p = block_plan(t, cols);
       const size_t v = 16 / dtype_size(t);
-      is("block plan holds the row", !p.threads ? cols > 8 * 1024 * v : static_cast<size_t>(p.threads) * p.vecs * v >= cols, 1);
-      is("block plan's waves", p.threads % 64 == 0 && p.threads <= (p.vecs == 8 ? 1024 : 512), 1);
+      is("block plan holds the row", !p.threads ? cols > 2 * 1024 * v : static_cast<size_t>(p.threads) * p.vecs * v >= cols, 1);
+      is("block plan's waves", p.threads % 64 == 0 && p.threads <= 1024, 1);
     }
 }
 
