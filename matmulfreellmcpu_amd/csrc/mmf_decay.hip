@@ -28,8 +28,9 @@ __device__ __forceinline__ double log2_step(double a) {
 // A block takes kCols columns of one head's state of one sequence, in registers: 8 lanes of 4 columns, 32 strips of
 // rows, row strip + 32 i each. Step by step down the sequence.
 constexpr int kCols = 32, kStrips = 32;
-template <int DT, int NK>
-__global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, DecayTab t, size_t first_seq) {
+struct NoTab {};
+template <int DT, int NK, class Tab>
+__global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, Tab t, size_t first_seq) {
   using E = Elem<DT>;
   using T = typename E::T;
   typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -39,9 +40,13 @@ __global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, DecayTab t, si
   const int c0 = blockIdx.x % slices * kCols + (threadIdx.x & 7) * 4, strip = threadIdx.x >> 3;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int Dk = static_cast<int>(a.Dk), Dv = static_cast<int>(a.Dv);
-  const bool listed = t.n > 0;  // else a row of each
-  const size_t first = listed ? t.of[blockIdx.y].row : first_seq + blockIdx.y, seq = listed ? t.of[blockIdx.y].seq : first;
-  const int len = listed ? t.of[blockIdx.y].len : 1;
+  size_t first = first_seq + blockIdx.y, seq = first;  // a row of each, where there is no table
+  int len = 1;
+  if constexpr (std::is_same_v<Tab, DecayTab>) {
+    first = t.of[blockIdx.y].row;
+    seq = t.of[blockIdx.y].seq;
+    len = t.of[blockIdx.y].len;
+  }
   float* state = a.state ? a.state + (seq * a.heads + head) * a.Dk * a.Dv : nullptr;
   const T* q = static_cast<const T*>(a.q) + first * a.ldq + head / (a.heads / a.q_heads) * a.Dk;
   const T* k = static_cast<const T*>(a.k) + first * a.ldk + head / (a.heads / a.k_heads) * a.Dk;
@@ -114,15 +119,15 @@ __global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, DecayTab t, si
   }
 }
 
-template <int DT>
-hipError_t steps_launch(const DecayArgs& a, const DecayTab& t, size_t first_seq, int n, hipStream_t s) {
+template <int DT, class Tab>
+hipError_t steps_launch(const DecayArgs& a, const Tab& t, size_t first_seq, int n, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.heads * ((a.Dv + kCols - 1) / kCols)), n);
   if (a.Dk <= 64)
-    k_decay_steps<DT, 2><<<grid, 256, 0, s>>>(a, t, first_seq);
+    k_decay_steps<DT, 2, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
   else if (a.Dk <= 128)
-    k_decay_steps<DT, 4><<<grid, 256, 0, s>>>(a, t, first_seq);
+    k_decay_steps<DT, 4, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
   else
-    k_decay_steps<DT, 8><<<grid, 256, 0, s>>>(a, t, first_seq);
+    k_decay_steps<DT, 8, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
   return hipGetLastError();
 }
 
@@ -144,13 +149,11 @@ inline constexpr int kSumParts = DT == kF32 ? 3 : 2;  // of the state and the we
 constexpr int kChunk = kDecayChunk;
 enum DecayPass { kEnds = 0, kOutputs = 1 };
 
-// Place of 4 neighbouring elements (unit u of a row) of a tile of COLS columns, in such units: rows are turned against each
-// other so that 16 rows' same unit, 4 rows' 4 neighbouring units and one row's neighbours all lie in other LDS banks.
+// Elements from row to row of a tile of COLS columns: 16 bytes more than a row, so that 16 rows' same elements lie in other
+// LDS banks, and every place is one lane's own plus a constant. (Rows turned against each other are free of conflicts in
+// every product, but each place is a register then: 195 of them a thread, 2048 x 16 x 128 x 128 bf16 40 us.)
 template <int COLS>
-__device__ __forceinline__ int unit_at(int r, int u) {
-  if constexpr (COLS == 64) return r * 16 + (u ^ ((r >> 1 & 1) << 2 | (r >> 2 & 1) << 3 | (r >> 3 & 1) << 1));
-  return r * (COLS / 4) + (u ^ ((r & 3) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1) << 4));
-}
+inline constexpr int kStride = COLS + 8;
 
 __device__ __forceinline__ float upper(float v) {  // the upper 16 bits, a bf16 number
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u);
@@ -191,21 +194,27 @@ __device__ __forceinline__ void cut8(const float* v, bf16x8* to) {
 __device__ __forceinline__ bf16x8 join(u16x4 a, u16x4 b) {
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-// Inputs of 16 rows of a row tile as an operand over columns: lane l, row r0 + l % 16, columns from c0 on.
+// Inputs of 16 rows of a tile as an operand over columns: lane l, row r0 + l % 16, columns from c0 on. at: by_columns_at().
 template <int COLS>
-__device__ __forceinline__ bf16x8 by_columns(const uint16_t* tile, int r0, int c0, int lane) {
-  const int r = r0 + (lane & 15), u = c0 / 4 + (lane >> 4);
-  return join(*reinterpret_cast<const u16x4*>(tile + unit_at<COLS>(r, u) * 4),
-              *reinterpret_cast<const u16x4*>(tile + unit_at<COLS>(r, u + 4) * 4));
+__device__ __forceinline__ int by_columns_at(int lane) {
+  return (lane & 15) * kStride<COLS> + (lane >> 4) * 4;
 }
-// 16 columns of a row tile as an operand over rows: lane l, column c0 + l % 16, rows from r0 on. The LDS hands 16 lanes the
+template <int COLS>
+__device__ __forceinline__ bf16x8 by_columns(const uint16_t* at, int r0, int c0) {
+  at += r0 * kStride<COLS> + c0;
+  return join(*reinterpret_cast<const u16x4*>(at), *reinterpret_cast<const u16x4*>(at + 16));
+}
+// 16 columns of a tile as an operand over 32 rows: lane l, column c0 + l % 16. at: by_rows_at(). The LDS hands 16 lanes the
 // columns of the 4 rows that they address 4 elements of each.
 template <int COLS>
-__device__ __forceinline__ bf16x8 by_rows(const uint16_t* tile, int r0, int c0, int lane) {
+__device__ __forceinline__ int by_rows_at(int lane) {
+  return (4 * (lane >> 4) + (lane >> 2 & 3)) * kStride<COLS> + (lane & 3) * 4;
+}
+template <int COLS>
+__device__ __forceinline__ bf16x8 by_rows(const uint16_t* at, int c0) {
   typedef __attribute__((address_space(3))) s16x4* lds;
-  const int r = r0 + 4 * (lane >> 4) + (lane >> 2 & 3), u = c0 / 4 + (lane & 3);
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(tile + unit_at<COLS>(r, u) * 4));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(tile + unit_at<COLS>(r + 16, u) * 4));
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(at + c0));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(at + 16 * kStride<COLS> + c0));
   return join(__builtin_bit_cast(u16x4, a), __builtin_bit_cast(u16x4, b));
 }
 // c += a b over all pairs of parts that count.
@@ -222,22 +231,23 @@ __device__ __forceinline__ void mma(const bf16x8* a, const bf16x8* b, f32x4& c) 
 // kChunk rows of COLS columns from global memory, 8 neighbouring columns at a time, in registers and then in LDS. Loads have no
 // conditions, so that all are in flight together: rows and columns past the end are read from the last ones and then
 // set to 0.
-template <int DT, int COLS, int TH>
+template <int DT, int COLS, int TH, bool EVEN>
 struct Tile {
   using E = Elem<DT>;
   using T = typename E::T;
-  static constexpr int kVecs = kChunk * COLS / 8, kUsed = kVecs < TH ? kVecs : TH;
-  static constexpr int kEach = kVecs / kUsed, kRows = kUsed / (COLS / 8), N = kParts<DT>, H = 8 / E::V;
+  static constexpr int kVecs = COLS / 8;  // of a row
+  static constexpr int kRows = TH >= 32 * kVecs ? 32 : TH >= 16 * kVecs ? 16 : 8, kUsed = kRows * kVecs;  // rows and threads at a time
+  static constexpr int kEach = kChunk / kRows, N = kParts<DT>, H = 8 / E::V;
   typename E::Vec v[kEach][H];
   // The thread's first element of a chunk that starts at p, where columns come in groups of 8.
   __device__ __forceinline__ static const T* place(const T* p, size_t ld, int cols) {
-    return p + (threadIdx.x % kUsed / (COLS / 8)) * ld + max(min(static_cast<int>(threadIdx.x) % (COLS / 8) * 8, cols - 8), 0);
+    return p + (threadIdx.x % kUsed / kVecs) * ld + max(min(static_cast<int>(threadIdx.x % kVecs) * 8, cols - 8), 0);
   }
   // mine: place() of the chunk at p, of which `rows` are left
   __device__ __forceinline__ void fetch(const T* mine, const T* p, size_t ld, int rows, int cols) {
     if (kUsed < TH && threadIdx.x >= kUsed) return;
-    const int r0 = threadIdx.x / (COLS / 8), c = threadIdx.x % (COLS / 8) * 8;
-    if (cols % 8 == 0) {
+    const int r0 = threadIdx.x / kVecs, c = threadIdx.x % kVecs * 8;
+    if constexpr (EVEN) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         const T* from = mine + i * kRows * ld;
@@ -263,10 +273,10 @@ struct Tile {
   }
   __device__ __forceinline__ void store(uint16_t* tile) const {
     if (kUsed < TH && threadIdx.x >= kUsed) return;
-    const int r0 = threadIdx.x / (COLS / 8), u = threadIdx.x % (COLS / 8) * 2;
+    const int r0 = threadIdx.x / kVecs, c = threadIdx.x % kVecs * 8;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      uint16_t* to = tile + unit_at<COLS>(r0 + i * kRows, u) * 4;
+      uint16_t* to = tile + (r0 + i * kRows) * kStride<COLS> + c;
       if constexpr (DT == kBF16) {
         *reinterpret_cast<u16x8*>(to) = v[i][0];
       } else {
@@ -276,7 +286,7 @@ struct Tile {
         for (int j = 0; j < 8; ++j) f[j] = E::up(v[i][j / E::V][j % E::V]);
         cut8<N>(f, p);
 #pragma unroll
-        for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(to + k * kChunk * COLS) = p[k];
+        for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(to + k * kChunk * kStride<COLS>) = p[k];
       }
     }
   }
@@ -302,7 +312,8 @@ __device__ __forceinline__ double running_sum(double x) {
 template <int DT, int DKP, int NW>
 struct DecayShape {
   static constexpr int DVP = 16 * NW, N = kParts<DT>, NS = kSumParts<DT>;
-  static constexpr int kRowTile = kChunk * DKP * N, kColTile = kChunk * DVP * N, kWeights = 2 * NS * 512;
+  static constexpr int kRowPart = kChunk * kStride<DKP>, kColPart = kChunk * kStride<DVP>;
+  static constexpr int kRowTile = kRowPart * N, kColTile = kColPart * N, kWeights = 2 * NS * 512;
   static constexpr int kEndsOne = kRowTile + kColTile, kOutOne = 2 * kRowTile + kColTile + kWeights;
   // two buffers where they fit: the next chunk's rows are stored beside the products of this one
   static constexpr int kSumBytes = NW * kChunk * 16, kLds = 160 * 1024 - 512;
@@ -322,8 +333,8 @@ struct DecayDev {
   float scale;
 };
 
-template <int DT, int DKP, int NW, int PASS>
-__global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
+template <int DT, int DKP, int NW, int PASS, bool EVEN>
+__global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVEN ? 4 : 2) void k_decay(DecayDev a, DecayTab t) {
   using Sh = DecayShape<DT, DKP, NW>;
   using E = Elem<DT>;
   using T = typename E::T;
@@ -361,8 +372,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
   float* state = a.state ? a.state + (static_cast<size_t>(seq.seq) * a.heads + head) * held : nullptr;
   float* put = PASS == kEnds ? slot : last ? state : nullptr;
 
-  Tile<DT, DKP, 64 * NW> tk, tq;
-  Tile<DT, DVP, 64 * NW> tv;
+  Tile<DT, DKP, 64 * NW, EVEN> tk, tq;
+  Tile<DT, DVP, 64 * NW, EVEN> tv;
   const int vcols = min(Dv - c0, DVP);
   const T* const kt = tk.place(kp, a.ldk, Dk);
   const T* const vt = tv.place(vp, a.ldv, vcols);
@@ -443,6 +454,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
     uint16_t* const sV = sK + Sh::kRowTile;
     uint16_t* const sQ = sV + Sh::kColTile;
     uint16_t* const sP = sQ + Sh::kRowTile;
+    const uint16_t* const kc = sK + by_columns_at<DKP>(lane);
+    const uint16_t* const qc = sQ + by_columns_at<DKP>(lane);
+    const uint16_t* const kr = sK + by_rows_at<DKP>(lane);
+    const uint16_t* const vr = sV + by_rows_at<DVP>(lane) + n0;
     f32x4 O[2] = {};
     if constexpr (PASS == kOutputs) {
       // Weights of the chunk's rows (16 slab + i) by rows (16 jt + j): three of the four tiles hold any, a wave each; lane l, row
@@ -455,8 +470,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
           bf16x8 q[N], k[N];
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            q[i] = by_columns<DKP>(sQ + i * C * DKP, slab * 16, ks * 32, lane);
-            k[i] = by_columns<DKP>(sK + i * C * DKP, jt * 16, ks * 32, lane);
+            q[i] = by_columns<DKP>(qc + i * Sh::kRowPart, slab * 16, ks * 32);
+            k[i] = by_columns<DKP>(kc + i * Sh::kRowPart, jt * 16, ks * 32);
           }
           mma<N, N>(k, q, W);
         }
@@ -494,7 +509,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
           for (int sl = 0; sl < 2; ++sl) {
             bf16x8 q[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) q[i] = by_columns<DKP>(sQ + i * C * DKP, sl * 16, ks * 32, lane);
+            for (int i = 0; i < N; ++i) q[i] = by_columns<DKP>(qc + i * Sh::kRowPart, sl * 16, ks * 32);
             mma<NS, N>(h, q, O[sl]);
           }
         }
@@ -512,7 +527,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
     bf16x8 v[N];
     uint32_t odd = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = by_rows<DVP>(sV + i * C * DVP, 0, n0, lane);
+    for (int i = 0; i < N; ++i) v[i] = by_rows<DVP>(vr + i * Sh::kColPart, 0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) odd |= (__builtin_bit_cast(u32x4, v[0])[e] & 0x7F807F80u) + 0x00800080u;  // an exponent of all ones carries
     int from_row = C;  // the first row without a number of this lane's column
@@ -582,7 +597,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_decay(DecayDev a, DecayTab t) {
       for (int k = 0; k < KT; ++k) {
         bf16x8 kk[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) kk[i] = by_rows<DKP>(sK + i * C * DKP, 0, k * 16, lane);
+        for (int i = 0; i < N; ++i) kk[i] = by_rows<DKP>(kr + i * Sh::kRowPart, k * 16);
         mma<N, 3>(kk, w, S[k]);
       }
       if (some && from_row < C) {
@@ -650,24 +665,24 @@ __global__ __launch_bounds__(256) void k_decay_carry(DecayDev a, DecayTab t) {
   }
 }
 
-template <int DT, int DKP, int NW>
+template <int DT, int DKP, int NW, bool EVEN>
 hipError_t tiles_launch(const DecayDev& a, const DecayTab& t, hipStream_t s) {
   using Sh = DecayShape<DT, DKP, NW>;
   const unsigned heads = a.heads, slices = (a.Dv + Sh::DVP - 1) / Sh::DVP;
   hipError_t e;
   if (t.many) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kEnds>), hipFuncAttributeMaxDynamicSharedMemorySize,
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kEnds, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize,
                             Sh::kEndsBytes);
     if (e != hipSuccess) return e;
-    k_decay<DT, DKP, NW, kEnds><<<dim3(t.cut_tiles, slices, heads), 64 * NW, Sh::kEndsBytes, s>>>(a, t);
+    k_decay<DT, DKP, NW, kEnds, EVEN><<<dim3(t.cut_tiles, slices, heads), 64 * NW, Sh::kEndsBytes, s>>>(a, t);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     k_decay_carry<<<dim3((a.Dk * a.Dv + 255) / 256, heads, t.many), 256, 0, s>>>(a, t);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kOutputs>), hipFuncAttributeMaxDynamicSharedMemorySize,
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kOutputs, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           Sh::kOutBytes);
   if (e != hipSuccess) return e;
-  k_decay<DT, DKP, NW, kOutputs><<<dim3(t.tiles, slices, heads), 64 * NW, Sh::kOutBytes, s>>>(a, t);
+  k_decay<DT, DKP, NW, kOutputs, EVEN><<<dim3(t.tiles, slices, heads), 64 * NW, Sh::kOutBytes, s>>>(a, t);
   return hipGetLastError();
 }
 
@@ -677,10 +692,17 @@ hipError_t tiles_of(const DecayArgs& a, const DecayTab& t, float* ws, hipStream_
              static_cast<int>(a.heads), static_cast<int>(a.heads / a.q_heads), static_cast<int>(a.heads / a.k_heads),
              static_cast<int>(a.heads / a.v_heads), static_cast<int>(a.Dk), static_cast<int>(a.Dv), a.scale};
   if (t.many) d.keeps = ws + static_cast<size_t>(t.cut_tiles) * a.heads * a.Dk * a.Dv;
-  const bool wide = a.Dv > 64;
-  if (a.Dk <= 64) return wide ? tiles_launch<DT, 64, 8>(d, t, s) : tiles_launch<DT, 64, 4>(d, t, s);
-  if (a.Dk <= 128) return wide ? tiles_launch<DT, 128, 8>(d, t, s) : tiles_launch<DT, 128, 4>(d, t, s);
-  return wide ? tiles_launch<DT, 256, 8>(d, t, s) : tiles_launch<DT, 256, 4>(d, t, s);
+  auto sized = [&](auto wide, auto even) {
+    constexpr int NW = decltype(wide)::value ? 8 : 4;
+    constexpr bool EVEN = decltype(even)::value;
+    if (a.Dk <= 64) return tiles_launch<DT, 64, NW, EVEN>(d, t, s);
+    if (a.Dk <= 96) return tiles_launch<DT, 96, NW, EVEN>(d, t, s);
+    if (a.Dk <= 128) return tiles_launch<DT, 128, NW, EVEN>(d, t, s);
+    return tiles_launch<DT, 256, NW, EVEN>(d, t, s);
+  };
+  const bool even = a.Dk % 8 == 0 && a.Dv % 8 == 0;
+  if (a.Dv > 64) return even ? sized(std::true_type{}, std::true_type{}) : sized(std::true_type{}, std::false_type{});
+  return even ? sized(std::false_type{}, std::true_type{}) : sized(std::false_type{}, std::false_type{});
 }
 
 }  // namespace
@@ -690,10 +712,8 @@ hipError_t launch_decay(const DecayArgs& a, float* ws, hipStream_t s) {
   return with_type(a.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (!a.lens && a.rows == a.seqs) {  // a row of each
-      DecayTab none;
-      none.n = 0;
       for (size_t q = 0; q < a.seqs; q += 65535) {
-        const hipError_t e = steps_launch<DT>(a, none, q, static_cast<int>(a.seqs - q < 65535 ? a.seqs - q : 65535), s);
+        const hipError_t e = steps_launch<DT>(a, NoTab{}, q, static_cast<int>(a.seqs - q < 65535 ? a.seqs - q : 65535), s);
         if (e != hipSuccess) return e;
       }
       return hipSuccess;
