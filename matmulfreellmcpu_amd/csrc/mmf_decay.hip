@@ -635,32 +635,37 @@ __global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVE
   }
 }
 
-// The states before the tiles in the place of those at their ends, in order: a thread an element, a head and a sequence of
-// more than one tile a row of blocks, kBatch tiles' loads in flight.
+// The states before the tiles in the place of those at their ends, in order: a thread V neighbouring elements, a head and a
+// sequence of more than one tile a row of blocks, kBatch tiles' loads in flight.
+template <int V>
 __global__ __launch_bounds__(256) void k_decay_carry(DecayDev a, DecayTab t) {
+  typedef float Vec __attribute__((ext_vector_type(V), aligned(4)));
   constexpr int kBatch = 8;
-  const size_t n = a.Dk * a.Dv, i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const size_t n = a.Dk * a.Dv, i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * V;
   if (i >= n) return;
   const DecaySeq seq = t.of[blockIdx.z];
   const int tiles = (seq.len + t.step - 1) / t.step;
   const size_t head = blockIdx.y, step = a.heads * n;
   float* ends = a.ends + (static_cast<size_t>(seq.tile) * a.heads + head) * n + i;
   const float* keeps = a.keeps + static_cast<size_t>(seq.tile) * a.heads + head;
-  float h = a.state ? a.state[(static_cast<size_t>(seq.seq) * a.heads + head) * n + i] : 0.0f;
+  Vec h = {};
+  if (a.state) h = *reinterpret_cast<const Vec*>(a.state + (static_cast<size_t>(seq.seq) * a.heads + head) * n + i);
   for (int j = 0; j < tiles; j += kBatch) {
-    float e[kBatch], f[kBatch];
+    Vec e[kBatch];
+    float f[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const size_t q = min(j + k, tiles - 2);  // (the last tile's end is not needed)
-      e[k] = ends[q * step];
+      e[k] = *reinterpret_cast<const Vec*>(ends + q * step);
       f[k] = keeps[q * a.heads];
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       if (j + k >= tiles) break;
-      ends[(j + k) * step] = h;
+      *reinterpret_cast<Vec*>(ends + (j + k) * step) = h;
       // a state of 0 stays out of the product: a growing head's factor may be infinite over a tile where no row's is
-      h = h != 0.0f ? __builtin_fmaf(f[k], h, e[k]) : e[k];
+#pragma unroll
+      for (int c = 0; c < V; ++c) h[c] = h[c] != 0.0f ? __builtin_fmaf(f[k], h[c], e[k][c]) : e[k][c];
     }
   }
 }
@@ -676,7 +681,10 @@ hipError_t tiles_launch(const DecayDev& a, const DecayTab& t, hipStream_t s) {
     if (e != hipSuccess) return e;
     k_decay<DT, DKP, NW, kEnds, EVEN><<<dim3(t.cut_tiles, slices, heads), 64 * NW, Sh::kEndsBytes, s>>>(a, t);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    k_decay_carry<<<dim3((a.Dk * a.Dv + 255) / 256, heads, t.many), 256, 0, s>>>(a, t);
+    if (a.Dk * a.Dv % 4 == 0)
+      k_decay_carry<4><<<dim3((a.Dk * a.Dv + 1023) / 1024, heads, t.many), 256, 0, s>>>(a, t);
+    else
+      k_decay_carry<1><<<dim3((a.Dk * a.Dv + 255) / 256, heads, t.many), 256, 0, s>>>(a, t);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<DT, DKP, NW, kOutputs, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize,

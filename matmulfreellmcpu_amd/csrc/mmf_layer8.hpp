@@ -213,7 +213,9 @@ inline void fill_decay(DecayTab& t, const DecaySeq* s, int n, int step) {
   t.tiles = tiles;
 }
 // Rows of a tile: so many that the tiles of all heads fill the chip twice, and that those of long sequences have room in
-// the workspace. No sequence is cut into two: that would be three launches for one.
+// the workspace. At least 128, as each tile writes a state and reads it three times (2048 rows of 16 heads: 38.8 us, and
+// 44.7 by tiles of 64), but 64 where such tiles have a compute unit each (one head: 22.0 us, and 27.3 by 128). No sequence
+// is cut into two: that would be three launches for one.
 inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
   constexpr int chunk = kDecayChunk;
   size_t chunks = 0;
@@ -224,7 +226,8 @@ inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
   }
   const size_t blocks = a.heads * ((a.Dv + 127) / 128), per = a.heads * (a.Dk * a.Dv + 1);
   size_t step = (chunks * blocks + 511) / 512 * chunk;
-  if (step < 128) step = 128;
+  const size_t least = chunks * blocks <= 512 ? 64 : 128;
+  if (step < least) step = least;
   for (;; step *= 2) {
     if (step * 2 >= static_cast<size_t>(most)) return most;
     size_t slots = 0;
