@@ -108,8 +108,8 @@ __device__ __forceinline__ void block_reduce(RowSums& s, int& slot, double& sum,
   slot ^= 1;
 }
 
-// A block goes through rows, NV vectors of 16 bytes a thread, the next row's on their way meanwhile; one vector's weights stay
-// in registers. EVEN: rows are whole vectors.
+// A block goes through rows, NV vectors of 16 bytes a thread. One vector's weights stay in registers, and the next row's
+// vector is on its way meanwhile; two would not fit there. EVEN: rows are whole vectors.
 template <int DT, int NV, bool EVEN>
 __global__ __launch_bounds__(1024, 4) void k_block(BlockArgs a) {
   using E = Elem<DT>;
@@ -196,10 +196,11 @@ __global__ __launch_bounds__(1024, 4) void k_block(BlockArgs a) {
     }
   };
   Row next = {};
-  fetch(next, blockIdx.x);
+  if (kKeep) fetch(next, blockIdx.x);
   for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (!kKeep) fetch(next, row);
     const Row now = next;
-    if (row + gridDim.x < a.rows) fetch(next, row + gridDim.x);
+    if (kKeep && row + gridDim.x < a.rows) fetch(next, row + gridDim.x);
     double rstd = 1.0, sum = 0.0, top = 0.0;
     if (a.w_post) {
 #pragma unroll
@@ -221,32 +222,36 @@ __global__ __launch_bounds__(1024, 4) void k_block(BlockArgs a) {
         weights(kw, a.w_pre, place(i));
         fine = i ? fine + unfit(kw) : unfit(kw);
       }
-      double p[V];
+      // four at a time: more at once go out of the registers
 #pragma unroll
-      for (int j = 0; j < V; ++j) p[j] = static_cast<double>(E::up(now.b[i][j])) * rstd * kf[j];
-      if (a.gate) {
-        if (a.act == kActNone) {
+      for (int q = 0; q < V; q += 4) {
+        double p[4];
 #pragma unroll
-          for (int j = 0; j < V; ++j) p[j] *= E::up(now.g[i][j]);
-        } else {
+        for (int j = 0; j < 4; ++j) p[j] = static_cast<double>(E::up(now.b[i][q + j])) * rstd * kf[q + j];
+        if (a.gate) {
+          if (a.act == kActNone) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) p[j] *= sigmoid(E::up(now.g[i][j]));
-          if (a.act == kActSilu) {
+            for (int j = 0; j < 4; ++j) p[j] *= E::up(now.g[i][q + j]);
+          } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) p[j] *= E::up(now.g[i][j]);
+            for (int j = 0; j < 4; ++j) p[j] *= sigmoid(E::up(now.g[i][q + j]));
+            if (a.act == kActSilu) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) p[j] *= E::up(now.g[i][q + j]);
+            }
           }
         }
-      }
-      if (a.x) {
+        if (a.x) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] += E::up(now.x[i][j]);
-      }
+          for (int j = 0; j < 4; ++j) p[j] += E::up(now.x[i][q + j]);
+        }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        h[i][j] = static_cast<float>(p[j]);
-        const double d = h[i][j];
-        sum = __builtin_fma(d, d, sum);
-        top = larger(top, __builtin_fabs(d * static_cast<double>(kw[j])));
+        for (int j = 0; j < 4; ++j) {
+          h[i][q + j] = static_cast<float>(p[j]);
+          const double d = h[i][q + j];
+          sum = __builtin_fma(d, d, sum);
+          top = larger(top, __builtin_fabs(d * static_cast<double>(kw[q + j])));
+        }
       }
     }
     double rstd2 = 1.0, inv = 0.0;
@@ -369,8 +374,11 @@ hipError_t launch_block(const BlockArgs& all, hipStream_t s) {
         a.codes += r * a.ldcodes;
         a.scales += r;
       }
-      // as many blocks as the chip holds, of as many rows each
-      const size_t held = 256 * std::max(1, 1024 / std::max(p.threads, 64)), each = (a.rows + held - 1) / held;
+      // As many blocks as the chip holds, of as many rows each. A compute unit's four SIMDs hold four waves each: two blocks
+      // of five to eight waves (2048 x 2560 bf16 with silu: 25.0 us, by three blocks of five waves 27.8, by one block
+      // of three rows 25.8).
+      const int waves = std::max(p.threads / 64, 1);
+      const size_t held = 256 * (waves <= 4 ? 16 / waves : 4 / ((waves + 3) / 4)), each = (a.rows + held - 1) / held;
       const unsigned rows = static_cast<unsigned>(a.rows), blocks = static_cast<unsigned>((a.rows + each - 1) / each);
       const bool even = a.cols % Elem<DT>::V == 0;
       if (p.vecs == 1)
