@@ -214,8 +214,8 @@ inline void fill_decay(DecayTab& t, const DecaySeq* s, int n, int step) {
 }
 // Rows of a tile: so many that the tiles of all heads fill the chip twice, and that those of long sequences have room in
 // the workspace. At least 128, as each tile writes a state and reads it three times (2048 rows of 16 heads: 38.8 us, and
-// 44.7 by tiles of 64), but 64 where such tiles have a compute unit each (one head: 22.0 us, and 27.3 by 128). No sequence
-// is cut into two: that would be three launches for one.
+// 44.7 by tiles of 64), but 64 where such tiles have a compute unit each (one head: 22.0 us, and 27.3 by 128). Nothing is
+// cut where the longest sequence would be cut into two: that would be three launches for one.
 inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
   constexpr int chunk = kDecayChunk;
   size_t chunks = 0;
