@@ -242,8 +242,8 @@ int mmf_w8_linear(mmf_ctx* ctx, int w8_id, const int8_t* x, const float* xscales
  * 1..256; decay [heads], gates [rows, heads] and state [seqs, heads, Dk, Dv] (may be NULL) in fp32. q_heads, k_heads and
  * v_heads (0: heads) divide heads, and neighbouring heads share one: head h takes the h / (heads / k_heads)-th of k. A log
  * decay of -infinity forgets the state; log decays above 0 are taken as they are, and results and the growth over 32 rows
- * have to be finite in fp32. A row whose q, k or v holds an infinity or NaN does not touch the rows before it. Sequences that
- * are cut into tiles (of more than 128 rows, by the heads and rows of a call) use the workspace. */
+ * have to be finite in fp32. A row whose q, k or v holds an infinity or NaN does not touch the rows before it. Calls with a
+ * sequence of more than 128 rows may use the workspace. */
 typedef struct {
   int dtype;
   float scale;
@@ -287,8 +287,9 @@ int mmf_block_norm_q8(mmf_ctx* ctx, const mmf_block_args* args);
  *   top_ids, top_logprobs [rows, top]    the `top` (0..64, at most V) most likely tokens, likeliest first, equal logits by
  *                                        the lower id
  * all but the ids in fp32. ids goes with logprobs (both may be NULL), entropy may be NULL, top may be 0. Logits of -infinity
- * are tokens that cannot come. A vocabulary of more than 32768 uses the workspace. Of a row that has no others every log probability is -infinity and the entropy 0; a row with
- * a NaN or +infinity has no log probabilities (NaN), and its top tokens are ordered with NaN above all. */
+ * are tokens that cannot come. Of a row that has no others every log probability is -infinity and the entropy 0; a row with
+ * a NaN or +infinity has no log probabilities (NaN), and its top tokens are ordered with NaN above all. Calls with V over
+ * 32768 use the workspace. */
 typedef struct {
   int dtype;
   float temperature;
