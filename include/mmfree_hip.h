@@ -224,7 +224,8 @@ int mmf_selective_scan(mmf_ctx* ctx, const mmf_scan_args* args);
  * workspace, capture. No counterparts in the reference. */
 
 /* Register weights codes [N, K] of 8 bits with scales [N] (host memory): a weight is code * scale of its output. K is at
- * most 131071, so that sums fit 32 bits. They are repacked on the device; the id is mmf_w8_linear's. */
+ * most 131071, so that sums fit 32 bits, and N * K at most 2^34. They are repacked on the device; the id is
+ * mmf_w8_linear's. */
 int mmf_w8_register(mmf_ctx* ctx, const int8_t* codes, const float* scales, size_t N, size_t K, int* w8_id);
 int mmf_w8_shape(mmf_ctx* ctx, int w8_id, size_t* N, size_t* K);
 /* Free registered weights; the id is invalid afterwards (calls that pass it fail with MMF_ERR_ARG). */
@@ -281,7 +282,8 @@ typedef struct {
 } mmf_block_args;
 int mmf_block_norm_q8(mmf_ctx* ctx, const mmf_block_args* args);
 
-/* Log probabilities under softmax(logits / temperature), row by row of logits [rows, V] of dtype:
+/* Log probabilities under softmax(logits / temperature), of a finite temperature of 1e-38 or more, row by row of logits
+ * [rows, V] of dtype:
  *   logprobs[row] = log p(ids[row])      (an id outside 0..V-1: NaN)
  *   entropy[row]  = -sum p log p
  *   top_ids, top_logprobs [rows, top]    the `top` (0..64, at most V) most likely tokens, likeliest first, equal logits by

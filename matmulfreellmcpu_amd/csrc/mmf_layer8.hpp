@@ -22,10 +22,12 @@ constexpr const char* kBadAlign = "a pointer is not aligned to its type";
 struct W8Geom {
   int N, K, nt, nk;  // tiles of 32 outputs, runs of 32 inputs
 };
-constexpr size_t kW8MaxK = 131071;  // 128 * 128 * K fits 32 bits
+constexpr size_t kW8MaxK = 131071;             // 128 * 128 * K fits 32 bits
+constexpr size_t kW8MaxCodes = size_t{1} << 34;  // a thread for 16 of them: a grid has fewer than 2^32
 inline const char* check_w8(size_t N, size_t K) {
   if (!N || !K || N > kMaxCols) return "invalid 8-bit weight shape";
   if (K > kW8MaxK) return "more than 131071 inputs: their sums would not fit 32 bits";
+  if (N * K > kW8MaxCodes) return "more than 2^34 weights";
   return nullptr;
 }
 inline W8Geom w8_geom(size_t N, size_t K) {
@@ -269,11 +271,13 @@ R each_decay(const DecayArgs& a, R ok, Steps&& steps, Tiles&& tiles) {
 }
 // Whether a call needs the workspace.
 inline bool decay_splits(const DecayArgs& a) {
+  if (!a.lens && a.rows <= a.seqs) return false;
   return each_decay(a, 0, [](const DecayTab&) { return 0; }, [](const DecayTab& t) { return t.many ? 1 : 0; }) != 0;
 }
 
 // ---- log probabilities of tokens ------------------------------------------------------------------
 constexpr size_t kMaxTop = 64;
+constexpr float kMinTemperature = 1e-38f;  // log2(e) over it is finite
 struct LogpArgs {
   int dtype;
   const void* x;                     // [rows, V]
@@ -289,8 +293,7 @@ inline const char* check(LogpArgs& a) {
   if (a.rows > kMaxRows) return "too many rows";
   if (!a.V || a.V > kMaxCols) return "the vocabulary must be 1..1048576";
   if (a.top > kMaxTop || a.top > a.V) return "top must be 0..64 and no more than the vocabulary";
-  if (!(a.temperature > 0.0f) || !(a.temperature < 3.4e38f) || !(1.0f / a.temperature < 3.4e38f))
-    return "the temperature must be positive and finite";
+  if (!(a.temperature >= kMinTemperature) || !(a.temperature < 3.4e38f)) return "the temperature must be positive and finite, 1e-38 or more";
   if (!ld_ok(a.ld, a.V)) return kBadLd;
   if (!a.rows) return nullptr;
   if (!a.x) return "null argument";

@@ -35,6 +35,8 @@ static void products() {
   want("w8 no outputs", check_w8(0, 77), "shape");
   want("w8 no inputs", check_w8(7, 0), "shape");
   want("w8 too many outputs", check_w8(kMaxCols + 1, 7), "shape");
+  want("w8 most weights", check_w8(kMaxCols, 16384), nullptr);
+  want("w8 too many weights", check_w8(kMaxCols, 16385), "2^34");
   auto go = [](const char* what, const char* part, auto&& change) {
     W8Args a{kF32, at<int8_t>(0x10001), at<float>(0x900), nullptr, at<float>(0x20000), 4, 0, 0};
     change(a);
@@ -203,7 +205,8 @@ static void logps() {
   go("logp large vocabulary", "vocabulary", [](LogpArgs& a) { a.V = kMaxCols + 1; });
   go("logp top", "top", [](LogpArgs& a) { a.top = 65; });
   go("logp top of few", "top", [](LogpArgs& a) { a.V = 4; });
-  for (float t : {0.0f, -1.0f, INFINITY, NAN, 1e-39f}) go("logp temperature", "temperature", [&](LogpArgs& a) { a.temperature = t; });
+  for (float t : {1e-38f, 3e38f}) go("logp temperature", nullptr, [&](LogpArgs& a) { a.temperature = t; });
+  for (float t : {0.0f, -1.0f, INFINITY, NAN, 1e-39f, 4e-39f}) go("logp temperature", "temperature", [&](LogpArgs& a) { a.temperature = t; });
   go("logp stride", "stride", [](LogpArgs& a) { a.ld = 99; });
   go("logp null", "null", [](LogpArgs& a) { a.x = nullptr; });
   go("logp ids alone", "together", [](LogpArgs& a) { a.logprobs = nullptr; });

@@ -180,6 +180,14 @@ def test_logprobs_plans(eng, units, rows, t):  # noqa: F811
         run_logp(eng, rng, t, 3 * rng.standard_normal((rows, n)), 7)
 
 
+@pytest.mark.parametrize("T", [1e-38, 1e-6, 1e30])
+@pytest.mark.parametrize("V", [50, 40000])
+def test_logprobs_temperatures(eng, V, T):  # noqa: F811
+    """The smallest temperature leaves all to the largest logit, whose z of 0 it may not turn into a NaN."""
+    rng = np.random.default_rng(V)
+    run_logp(eng, rng, F32, 0.2 * rng.standard_normal((5, V)), 3, T=T)
+
+
 @pytest.mark.parametrize("t", FLOATS)
 @pytest.mark.parametrize("waves", [1, 2, 3, 4, 5, 7, 8, 9, 12, 16, 17, 32])
 def test_block_many_rows_of_each_width(eng, waves, t):  # noqa: F811
