@@ -713,10 +713,9 @@ hipError_t tiles_of(const DecayArgs& a, const DecayTab& t, float* ws, hipStream_
     return tiles_launch<DT, 256, NW, EVEN>(d, t, s);
   };
   const bool even = a.Dk % 8 == 0 && a.Dv % 8 == 0;
-  // Blocks of 64 columns where each has a compute unit of its own (us: 2048 rows of a head of 128 x 128 bf16 20.6, of 128
-  // columns 22.2; 1000 x 777 fp32 32.6 and 36.4), else of 128, which read q and k once (2048 x 16 heads 38.2, and 40.1).
-  const bool wide = a.Dv > 64 && static_cast<size_t>(t.tiles) * a.heads * ((a.Dv + 63) / 64) > 256;
-  if (wide) return even ? sized(std::true_type{}, std::true_type{}) : sized(std::true_type{}, std::false_type{});
+  // Blocks of 128 columns read q and k once. (Blocks of 64 are sooner done where each has a compute unit of its own, 1000 x 777
+  // fp32 32.6 us and 36.4, but take more of the chip: of three contexts at once 21.5 us a call, and 15.5 by these.)
+  if (a.Dv > 64) return even ? sized(std::true_type{}, std::true_type{}) : sized(std::true_type{}, std::false_type{});
   return even ? sized(std::false_type{}, std::true_type{}) : sized(std::false_type{}, std::false_type{});
 }
 

@@ -140,7 +140,7 @@ def test_decay_tiles_of_each_width(eng, Dk, Dv, t):  # noqa: F811
 @pytest.mark.parametrize("t", FLOATS)
 @pytest.mark.parametrize("Dk,Dv", [(64, 96), (60, 70), (96, 128), (90, 127), (128, 72), (120, 130), (160, 136), (200, 129)])
 def test_decay_tiles_of_many_heads(eng, Dk, Dv, t):  # noqa: F811
-    """As above, of so many heads that blocks take 128 columns."""
+    """As above, of many heads that share their queries and keys."""
     run_decay(eng, np.random.default_rng(Dk + Dv), t, [300, 1, 0, 40], 68, Dk, Dv, q_heads=17, k_heads=34)
 
 
