@@ -725,7 +725,7 @@ hipError_t launch_decay(const DecayArgs& a, float* ws, hipStream_t s) {
   if (!a.rows) return hipSuccess;
   return with_type(a.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (!a.lens && a.rows == a.seqs) {  // a row of each
+    if (row_each(a)) {
       for (size_t q = 0; q < a.seqs; q += 65535) {
         const hipError_t e = steps_launch<DT>(a, NoTab{}, q, static_cast<int>(a.seqs - q < 65535 ? a.seqs - q : 65535), s);
         if (e != hipSuccess) return e;

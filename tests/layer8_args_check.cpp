@@ -192,6 +192,20 @@ static void attention() {
   });
 }
 
+static void steps() {
+  DecayArgs a{};
+  const size_t ones[] = {1, 1, 1, 1}, other[] = {1, 2, 0, 1};
+  a.seqs = 4;
+  a.rows = 4;
+  is("a row of each without lengths", row_each(a), 1);
+  a.lens = ones;
+  is("a row of each", row_each(a), 1);
+  a.lens = other;
+  is("as many rows as sequences", row_each(a), 0);
+  a.lens = nullptr;
+  a.rows = 8;
+  is("two rows of each", row_each(a), 0);
+}
 static void logps() {
   auto go = [](const char* what, const char* part, auto&& change) {
     LogpArgs a{kF32, at<float>(0x10000), at<int64_t>(0x20000), at<float>(0x30000), at<float>(0x40000), at<int64_t>(0x50000), at<float>(0x60000),
@@ -240,6 +254,7 @@ int main() {
   ways();
   blocks();
   attention();
+  steps();
   logps();
   return bad;
 }
