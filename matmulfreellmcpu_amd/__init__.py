@@ -379,7 +379,11 @@ class Engine:
 
     def register_w8(self, codes, scales) -> int:
         """8-bit weights: codes int8 [N, K], scales float32 [N]."""
-        codes, cp = _np(codes, np.int8)
+        given = np.asarray(codes)
+        with np.errstate(invalid="ignore"):
+            codes, cp = _np(given, np.int8)
+        if given.dtype != np.int8 and not np.array_equal(codes, given):
+            raise ValueError(f"codes of {given.dtype} that are no int8 numbers")
         scales, sp = _np(scales, np.float32)
         if codes.ndim != 2 or scales.shape != codes.shape[:1]:
             raise ValueError(f"codes {codes.shape} and scales {scales.shape} are not [N, K] and [N]")

@@ -57,3 +57,13 @@ def test_types_of_tensors(eng):  # noqa: F811
                  lambda: eng.w8_linear(0, f, f, f, 1), lambda: eng.w8_linear(0, c, b, f, 1), lambda: eng.w8_linear(0, c, f, f, 1, bias=b)):
         with pytest.raises(ValueError, match="place of"):
             call()
+
+
+def test_w8_codes_are_int8(eng):  # noqa: F811
+    """Weights of another type are taken where they are int8 numbers, and never wrapped or cut."""
+    import numpy as np
+    for codes in ([[128]], [[-129]], [[1.5]], [[float("nan")]], np.array([[200]], np.uint8), np.array([[1 << 40]])):
+        with pytest.raises(ValueError, match="no int8 numbers"):
+            eng.register_w8(codes, [1.0])
+    for codes in ([[127, -128]], np.array([[3.0, -4.0]]), np.array([[7, 100]], np.uint8), np.array([[1, -1]], np.int8)):
+        eng.register_w8(codes, [1.0])
