@@ -172,13 +172,21 @@ def _rows(x, t):
 
 def _own_type(x):
     """The row type of a tensor; an address alone is of F32."""
-    return max(_row_type(x) or F32, F32)
+    return F32 if x.__class__ is int else max(_row_type(x) or F32, F32)
+
+
+_id_types = {}  # whether a dtype object is int64, entered as they are met
 
 
 def _ids(x):
     """As _ptr, of 64-bit integers: a tensor of another type is refused."""
-    if getattr(x, "dtype", None) is not None and str(x.dtype).rpartition(".")[2] != "int64":
-        raise ValueError(f"a tensor of {x.dtype} in the place of int64 ids")
+    if x is None or x.__class__ is int:
+        return x
+    d = getattr(x, "dtype", None)
+    if d not in _id_types:
+        _id_types[d] = d is None or str(d).rpartition(".")[2] == "int64"
+    if not _id_types[d]:
+        raise ValueError(f"a tensor of {d} in the place of int64 ids")
     return _ptr(x)
 
 
