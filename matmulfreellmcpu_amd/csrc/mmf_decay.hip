@@ -139,14 +139,13 @@ hipError_t steps_launch(const DecayArgs& a, const Tab& t, size_t first_seq, int 
 // these rows, as are the weights of a chunk's rows (k q^T): neither goes through LDS to change its layout. An operand's 32
 // inputs then are, for lane group g = l / 16, 4 g + 0..3 and 16 + 4 g + 0..3 of them, in this order, in all products.
 //
-// Rows stand in LDS as bf16: fp32 in three parts (24 bits), fp16 in two, which is exact; parts a and b of two operands
-// are multiplied where a + b is less than the more of them, the others are below the last kept digit. The state and
-// the weights, which are fp32, enter outputs of 16 bits in two parts (2^-17 of each), of fp32 in three; what is added
-// to the state is always cut into three.
+// Rows stand in LDS as bf16: fp32 in three parts (24 bits), fp16 in two, which is exact. The state, the weights and what is
+// added to the state are fp32, in three parts, whatever the rows' type. All pairs of parts are multiplied but the last
+// by the last of two numbers of three parts: the parts are cut off, not rounded, so that the second is up to 2^-7 of the number
+// and the third up to 2^-14, and what is left out up to 2^-28 of the product, where (second, third) would be 2^-21.
 template <int DT>
 inline constexpr int kParts = DT == kF32 ? 3 : DT == kF16 ? 2 : 1;
-template <int DT>
-inline constexpr int kSumParts = DT == kF32 ? 3 : 2;  // of the state and the weights
+constexpr int kSumParts = 3;  // of the state, the weights and what is added to the state
 constexpr int kChunk = kDecayChunk;
 enum DecayPass { kEnds = 0, kOutputs = 1 };
 
@@ -168,7 +167,7 @@ __device__ __forceinline__ T& at_bytes(T* base, uint32_t bytes) {
   return *reinterpret_cast<T*>(reinterpret_cast<Byte*>(base) + bytes);
 }
 
-// v in N bf16 parts: the first ones cut off, the last one rounded (of three: exact).
+// v in N bf16 parts: the first ones cut off, the last one what is left (of three, and of an fp16 number's two, exactly).
 template <int N>
 __device__ __forceinline__ void cut(float v, uint16_t* to) {
 #pragma unroll
@@ -218,12 +217,11 @@ __device__ __forceinline__ bf16x8 by_rows(const uint16_t* at, int c0) {
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(at + 16 * kStride<COLS> + c0));
   return join(__builtin_bit_cast(u16x4, a), __builtin_bit_cast(u16x4, b));
 }
-// c += a b over all pairs of parts that count.
+// c += a b over all pairs of parts but the third by the third.
 template <int NA, int NB>
 __device__ __forceinline__ void mma(const bf16x8* a, const bf16x8* b, f32x4& c) {
-  constexpr int M = NA > NB ? NA : NB;
 #pragma unroll
-  for (int s = M - 1; s >= 0; --s)  // the small products first
+  for (int s = NA + NB - 2 < 3 ? NA + NB - 2 : 3; s >= 0; --s)  // the small products first
 #pragma unroll
     for (int i = 0; i < NA; ++i)
       if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
@@ -312,7 +310,7 @@ __device__ __forceinline__ double running_sum(double x) {
 
 template <int DT, int DKP, int NW>
 struct DecayShape {
-  static constexpr int DVP = 16 * NW, N = kParts<DT>, NS = kSumParts<DT>;
+  static constexpr int DVP = 16 * NW, N = kParts<DT>, NS = kSumParts;
   static constexpr int kRowPart = kChunk * kStride<DKP>, kColPart = kChunk * kStride<DVP>;
   static constexpr int kRowTile = kRowPart * N, kColTile = kColPart * N, kWeights = 2 * NS * 512;
   static constexpr int kEndsOne = kRowTile + kColTile, kOutOne = 2 * kRowTile + kColTile + kWeights;
@@ -587,7 +585,7 @@ __global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVE
         for (int k = 0; k < KT; ++k) S[k] *= keep;
       }
       any = true;
-      bf16x8 w[3];
+      bf16x8 w[NS];
       float f[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -596,13 +594,13 @@ __global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVE
         for (int i = N - 1; i >= 0; --i) f[e] += Elem<kBF16>::up(__builtin_bit_cast(u16x8, v[i])[e]);
         f[e] *= sTo[b][(e >> 2) * 16 + 4 * g + (e & 3)];
       }
-      cut8<3>(f, w);
+      cut8<NS>(f, w);
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         bf16x8 kk[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) kk[i] = by_rows<DKP>(kr + i * Sh::kRowPart, k * 16);
-        mma<N, 3>(kk, w, S[k]);
+        mma<N, NS>(kk, w, S[k]);
       }
       if (some && from_row < C) {
 #pragma unroll
