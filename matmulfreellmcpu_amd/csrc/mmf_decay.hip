@@ -19,9 +19,20 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The log decay of a row in powers of two. 2^-300 times any fp32 number is 0, as 2^-infinity is, and leaves the sums
 // that it stands in their digits.
+constexpr double kForgets = -300.0;
 __device__ __forceinline__ double log2_step(double a) {
   a *= 1.4426950408889634;
-  return a < -300.0 ? -300.0 : a;
+  return a < kForgets ? kForgets : a;
+}
+
+// The decay over a tile, part * 2^power: it may be outside fp32's range where the states before and after it are not.
+struct Keep {
+  float part, power;
+};
+__device__ __forceinline__ Keep keep_of(double log2_total) {
+  if (log2_total < kForgets) return {0.0f, 0.0f};
+  const double n = __builtin_fmin(__builtin_rint(log2_total), 1e6);
+  return {exp2_fast(static_cast<float>(log2_total - n)), static_cast<float>(n)};
 }
 
 // ---- a row of each sequence ----------------------------------------------------------------------
@@ -326,8 +337,9 @@ struct DecayDev {
   const void *q, *k, *v;
   void* out;
   const float *decay, *gates;
-  float *state, *ends, *keeps;  // ends [slot][head][Dk][Dv]: the states from zeros at the tiles' ends, then those
-  size_t ldq, ldk, ldv, ldo, ldg;  // before the tiles; keeps [slot][head]: the decay over a tile
+  float *state, *ends;             // ends [slot][head][Dk][Dv]: the states from zeros at the tiles' ends, then those
+  Keep* keeps;                     // before the tiles; keeps [slot][head]: the decay over a tile
+  size_t ldq, ldk, ldv, ldo, ldg;
   int heads, q_each, k_each, v_each, Dk, Dv;
   float scale;
 };
@@ -394,8 +406,8 @@ __global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVE
   };
   auto sums = [&](int p, float gate) {
     const bool in = lane < C && p + wave * C + lane < rows;
-    const double x = running_sum(in ? log2_step(decay + gate) : 0.0), end = __shfl(x, C - 1);
-    total += end;
+    const double step = in ? log2_step(decay + gate) : 0.0, x = running_sum(step), end = __shfl(x, C - 1);
+    total += __ballot(step == kForgets) ? -__builtin_inf() : end;  // what is forgotten does not grow back by later rows
     if (lane < C) {
       sG[wave][lane] = x;
       sFrom[wave][lane] = exp2_fast(static_cast<float>(x));
@@ -632,7 +644,7 @@ __global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVE
     if (threadIdx.x == 0) {
       total = 0.0;
       for (int w = 0; w < NW; ++w) total += sG[w][0];
-      a.keeps[static_cast<size_t>(blockIdx.x) * a.heads + head] = exp2_fast(static_cast<float>(total));
+      a.keeps[static_cast<size_t>(blockIdx.x) * a.heads + head] = keep_of(total);
     }
   }
 }
@@ -649,12 +661,12 @@ __global__ __launch_bounds__(256) void k_decay_carry(DecayDev a, DecayTab t) {
   const int tiles = (seq.len + t.step - 1) / t.step;
   const size_t head = blockIdx.y, step = a.heads * n;
   float* ends = a.ends + (static_cast<size_t>(seq.tile) * a.heads + head) * n + i;
-  const float* keeps = a.keeps + static_cast<size_t>(seq.tile) * a.heads + head;
+  const Keep* keeps = a.keeps + static_cast<size_t>(seq.tile) * a.heads + head;
   Vec h = {};
   if (a.state) h = *reinterpret_cast<const Vec*>(a.state + (static_cast<size_t>(seq.seq) * a.heads + head) * n + i);
   for (int j = 0; j < tiles; j += kBatch) {
     Vec e[kBatch];
-    float f[kBatch];
+    Keep f[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const size_t q = min(j + k, tiles - 2);  // (the last tile's end is not needed)
@@ -665,9 +677,15 @@ __global__ __launch_bounds__(256) void k_decay_carry(DecayDev a, DecayTab t) {
     for (int k = 0; k < kBatch; ++k) {
       if (j + k >= tiles) break;
       *reinterpret_cast<Vec*>(ends + (j + k) * step) = h;
-      // a state of 0 stays out of the product: a growing head's factor may be infinite over a tile where no row's is
+      // a power past what a factor holds is taken of the state first: exactly, as far as the result is a number of fp32
+      const int power = static_cast<int>(f[k].power), in = min(max(power, -125), 125);
+      const float factor = __builtin_ldexpf(f[k].part, in);
+      if (power != in) {
 #pragma unroll
-      for (int c = 0; c < V; ++c) h[c] = h[c] != 0.0f ? __builtin_fmaf(f[k], h[c], e[k][c]) : e[k][c];
+        for (int c = 0; c < V; ++c) h[c] = __builtin_ldexpf(h[c], power - in);
+      }
+#pragma unroll
+      for (int c = 0; c < V; ++c) h[c] = __builtin_fmaf(factor, h[c], e[k][c]);
     }
   }
 }
@@ -701,7 +719,7 @@ hipError_t tiles_of(const DecayArgs& a, const DecayTab& t, float* ws, hipStream_
   DecayDev d{a.q, a.k, a.v, a.out, a.decay, a.gates, a.state, ws, nullptr, a.ldq, a.ldk, a.ldv, a.ldo, a.ldg,
              static_cast<int>(a.heads), static_cast<int>(a.heads / a.q_heads), static_cast<int>(a.heads / a.k_heads),
              static_cast<int>(a.heads / a.v_heads), static_cast<int>(a.Dk), static_cast<int>(a.Dv), a.scale};
-  if (t.many) d.keeps = ws + static_cast<size_t>(t.cut_tiles) * a.heads * a.Dk * a.Dv;
+  if (t.many) d.keeps = reinterpret_cast<Keep*>(ws + static_cast<size_t>(t.cut_tiles) * a.heads * a.Dk * a.Dv);
   auto sized = [&](auto wide, auto even) {
     constexpr int NW = decltype(wide)::value ? 8 : 4;
     constexpr bool EVEN = decltype(even)::value;

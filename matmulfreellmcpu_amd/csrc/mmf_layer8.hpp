@@ -226,7 +226,7 @@ inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
     chunks += (s[i].len + chunk - 1) / chunk;
     most = s[i].len > most ? s[i].len : most;
   }
-  const size_t blocks = a.heads * ((a.Dv + 127) / 128), per = a.heads * (a.Dk * a.Dv + 1);
+  const size_t blocks = a.heads * ((a.Dv + 127) / 128), per = a.heads * (a.Dk * a.Dv + 2);
   size_t step = (chunks * blocks + 511) / 512 * chunk;
   const size_t least = chunks * blocks <= 512 ? 64 : 128;
   if (step < least) step = least;

@@ -6,7 +6,8 @@ U = 2^-24 is fp32's half step.
 import numpy as np
 import pytest
 
-from test_gpu_layer import BF16, F16, F32, FLOATS, U, Rows, coded, out_rows, value
+from test_gpu_layer import BF16, F16, F32, FLOATS, U, Rows, close, coded, out_rows, value
+from test_gpu_layer8 import decay_ref
 from test_gpu_parity import Dev, eng  # noqa: F401  (module fixture)
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +108,58 @@ def test_long_prompts_repeat_themselves(eng, t):  # noqa: F811
         got = O.get().view(np.uint8), S.get().view(np.uint8)
         first = first or got
         assert (got[0] == first[0]).all() and (got[1] == first[1]).all()
+
+
+# ---- range ----------------------------------------------------------------------------------
+
+
+def far_states(eng, t, H, lens, log_decay, state, scale, keys=5, q_from=0):  # noqa: F811
+    """Rows whose keys are 0 but for the last `keys` of each sequence, and whose queries are 0 before row q_from of it, at
+    log decays [rows]; against the recurrence.
+
+    An exponent of a chunk of 32 rows rounds to fp32, half a step (U) relative of at most 32 * 2 / ln 2, which is 64 U of its
+    exponential (a factor between tiles: 2 U), and the recurrence's own bound counts 3 U a row, 96 U a chunk."""
+    rng, D, rows, f = np.random.default_rng(t + H + len(lens)), 8, sum(lens), np.float32
+    print(f"far states t={t} H={H} lens={lens} scale={scale}", flush=True)
+    q, k, v = (value(coded(rng.standard_normal((rows, H, D)), t), t) for _ in range(3))
+    at = np.concatenate([np.arange(n) for n in lens])
+    k[at < np.repeat(lens, lens) - keys] = 0
+    q[at < q_from] = 0
+    gates = np.broadcast_to(np.asarray(log_decay, f)[:, None], (rows, H))
+    st = (state * (1 + rng.random((len(lens), H, D, D)))).astype(f)
+    out, got = attention(eng, t, q, k, v, lens, state=st, gates=np.ascontiguousarray(gates), scale=scale)
+    want, bound, new, err = decay_ref(q, k, v, gates, st, lens, float(f(scale)))
+    most = np.abs(new).max(), np.abs(want).max()
+    assert most[0] < 3e38 and most[1] < 60000
+    close(out, want, bound, t, "out")
+    close(got, new, err, F32, "state")
+
+
+# one tile, tiles of 64 rows, both in a call, tiles of 128 rows
+FAR = [(1, [128]), (1, [256]), (1, [128, 300]), (16, [2048])]
+
+
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("H,lens", FAR)
+def test_states_that_grow_past_a_tile(eng, H, lens, t):  # noqa: F811
+    """A small state grows by e^126 over a tile's rows, more than fp32 holds, and stays finite; it is e^126 smaller in the end."""
+    a = np.concatenate([np.where(np.arange(n) < 63, 2.0, np.where(np.arange(n) < 126, -2.0, 0.0)) for n in lens])
+    far_states(eng, t, H, lens, a, 1e-30, 1e-25)
+    a = np.concatenate([np.where(np.arange(n) < 63, 2.0, 0.0) for n in lens])
+    far_states(eng, t, H, lens, a, 1e-30, 1e-25)
+
+
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("H,lens", FAR)
+def test_states_that_shrink_past_a_tile(eng, H, lens, t):  # noqa: F811
+    """A large state shrinks by e^-96 over a tile's rows, less than fp32 holds, and is still a number."""
+    a = np.concatenate([np.where(np.arange(n) < 64, -1.5, 0.0) for n in lens])
+    far_states(eng, t, H, lens, a, 1e30, 1e12, keys=0, q_from=64)
+
+
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("H,lens", FAR)
+def test_forgotten_states_do_not_grow_back(eng, H, lens, t):  # noqa: F811
+    """A log decay of -infinity before rows that grow."""
+    a = np.concatenate([np.where(np.arange(n) < 1, -np.inf, np.where(np.arange(n) < 128, 2.0, 0.0)) for n in lens])
+    far_states(eng, t, H, lens, a, 1e35, 1.0)
