@@ -267,8 +267,9 @@ int mmf_decay_attention(mmf_ctx* ctx, const mmf_decay_args* args);
  * and codes and scales of y as mmf_add_rmsnorm_q8 makes them (both or neither). b, x, gate, h, y [rows, cols] of dtype;
  * w_post, w_pre, channels [cols] fp32; act an MMF_ACT_* (of a gate; sigmoid(g), or silu(g) = g * sigmoid(g)). All steps are
  * in 64 bits but h, which is rounded to fp32 before the second norm. h (may be NULL) may be b, x or the gate itself with the
- * same stride; y may be NULL; one of h, y and codes is needed. Rows whose h or y holds an infinity or NaN have codes 0 and
- * the scale NaN. */
+ * same stride; y may be NULL; one of h, y and codes is needed. A row whose h (in fp32) or w_pre holds an infinity or NaN,
+ * or whose scale would pass fp32, has codes 0 and the scale NaN. A finite h or y past its own type's range is stored as an
+ * infinity, with the codes and the scale of the number that it was. */
 enum { MMF_ACT_NONE = 0, MMF_ACT_SIGMOID = 1, MMF_ACT_SILU = 2 };
 typedef struct {
   int dtype, act;

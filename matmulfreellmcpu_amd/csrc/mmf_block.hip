@@ -111,6 +111,10 @@ __device__ __forceinline__ void block_reduce(RowSums& s, int& slot, double& sum,
   slot ^= 1;
 }
 
+// Whether a row whose largest |y| is m has a scale m / 127 in fp32.
+__device__ __forceinline__ bool scale_fits(double m) { return m < 127.0 * 0x1.ffffffp127; }
+__device__ __forceinline__ float scale_of(double m) { return __builtin_fminf(static_cast<float>(m / 127.0), 0x1.fffffep127f); }
+
 // A block goes through rows, NV vectors of 16 bytes a thread. One vector's weights stay in registers, and the next row's
 // vector is on its way meanwhile; two would not fit there. EVEN: rows are whole vectors.
 template <int DT, int NV, bool EVEN>
@@ -262,10 +266,10 @@ __global__ __launch_bounds__(1024, 4) void k_block(BlockArgs a) {
     if (norm2) {
       sum += fine;
       block_reduce<true>(s, slot, sum, top);
-      bad = !(sum < __builtin_inf());
       if (a.w_pre) rstd2 = rsqrt_mean(sum, inv_cols, eps);
       const double m = larger(top * rstd2, 1e-5);
-      if (a.codes && threadIdx.x == 0) a.scales[row] = bad ? __builtin_nanf("") : static_cast<float>(m / 127.0);
+      bad = !(sum < __builtin_inf()) || !scale_fits(m);
+      if (a.codes && threadIdx.x == 0) a.scales[row] = bad ? __builtin_nanf("") : scale_of(m);
       double r = __builtin_amdgcn_rcp(m);
       r = __builtin_fma(r, __builtin_fma(-m, r, 1.0), r);
       r = __builtin_fma(r, __builtin_fma(-m, r, 1.0), r);
@@ -343,10 +347,10 @@ __global__ __launch_bounds__(512) void k_block_long(BlockArgs a) {
     top = larger(top, __builtin_fabs(d * w));
   }
   block_reduce<true>(s, slot, sum, top);
-  const bool bad = !(sum < __builtin_inf());
   const double rstd2 = a.w_pre ? rsqrt_mean(sum, inv_cols, a.eps) : 1.0;
   const double m = larger(top * rstd2, 1e-5), inv = 127.0 * rstd2 / m;
-  if (a.codes && threadIdx.x == 0) a.scales[row] = bad ? __builtin_nanf("") : static_cast<float>(m / 127.0);
+  const bool bad = !(sum < __builtin_inf()) || !scale_fits(m);
+  if (a.codes && threadIdx.x == 0) a.scales[row] = bad ? __builtin_nanf("") : scale_of(m);
   for (size_t i = threadIdx.x; i < a.cols; i += 512) {
     const float h = h_at(i);
     const double hw = a.w_pre ? static_cast<double>(h) * static_cast<double>(a.w_pre[i]) : static_cast<double>(h);
