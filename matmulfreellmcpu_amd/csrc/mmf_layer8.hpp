@@ -285,7 +285,7 @@ inline bool decay_splits(const DecayArgs& a) {
 
 // ---- log probabilities of tokens ------------------------------------------------------------------
 constexpr size_t kMaxTop = 64;
-constexpr float kMinTemperature = 1e-38f;  // log2(e) over it is finite
+constexpr float kMinTemperature = 1e-38f;  // 2 log2(e) over it is finite
 struct LogpArgs {
   int dtype;
   const void* x;                     // [rows, V]

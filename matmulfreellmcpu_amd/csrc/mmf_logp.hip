@@ -32,9 +32,13 @@ struct Sums {
   float top, sum, weighted;  // the maximum, sum e^z, sum z e^z
 };
 
+// (v - m) / 2, for logits whose difference may pass fp32; as exact as the difference. It goes with twice the temperature's
+// inverse, two_t, which is finite also times log2(e).
+__device__ __forceinline__ float half_less(float v, float half_m) { return __builtin_fmaf(v, 0.5f, -half_m); }
+
 // log p of a token whose logit is v.
-__device__ __forceinline__ float logp_of(const Sums& t, float inv_t, float log_sum, float v) {
-  return t.sum == 0.0f ? -__builtin_inff() : (v - t.top) * inv_t - log_sum;  // a row of -infinity alone has no tokens
+__device__ __forceinline__ float logp_of(const Sums& t, float two_t, float log_sum, float v) {
+  return t.sum == 0.0f ? -__builtin_inff() : half_less(v, 0.5f * t.top) * two_t - log_sum;  // a row of -infinity alone has no tokens
 }
 __device__ __forceinline__ float entropy_of(const Sums& t, float log_sum) {
   return t.sum == 0.0f ? 0.0f : log_sum - t.weighted / t.sum;
@@ -49,9 +53,9 @@ __device__ __forceinline__ float given(const LogpArgs& a, size_t row) {
   return in ? E::up(static_cast<const typename E::T*>(a.x)[row * a.ld + id]) : __builtin_nanf("");
 }
 // The outputs of a row but its top tokens, by one thread.
-__device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Sums& t, float inv_t, float log_sum, float logit) {
+__device__ __forceinline__ void finish(const LogpArgs& a, size_t row, const Sums& t, float two_t, float log_sum, float logit) {
   if (a.entropy) a.entropy[row] = entropy_of(t, log_sum);
-  if (a.logprobs) a.logprobs[row] = logit != logit ? logit : logp_of(t, inv_t, log_sum, logit);
+  if (a.logprobs) a.logprobs[row] = logit != logit ? logit : logp_of(t, two_t, log_sum, logit);
 }
 
 // The top tokens of a part with more candidates than the list holds, or with numbers that are none: one at a time, the
@@ -84,7 +88,7 @@ __device__ __forceinline__ void one_by_one(const typename Elem<DT>::T* x, int fr
 // bf16 (131 MB) 45 us, 27.6 at a copy's rate, with the vector ALUs 0.61 busy: two passes over a row's registers and three
 // barriers stand between its loads; without top tokens 36.
 template <int DT, int TH, int NV, bool WHOLE>
-__global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float inv_t, float* ws, uint32_t segs) {
+__global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float two_t, float* ws, uint32_t segs) {
   using E = Elem<DT>;
   using T = typename E::T;
   using Vec = typename E::Vec;
@@ -183,15 +187,15 @@ __global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float 
       if (lane == 0) s_bound = least;
     }
     // (of -infinity alone the shift is 0, so that the sum is 0, or NaN by a NaN)
-    const float shift = top == -__builtin_inff() ? 0.0f : top, scale = inv_t * 1.44269504f;
-    float sum = 0.0f, weighted = 0.0f;
+    const float half = top == -__builtin_inff() ? 0.0f : 0.5f * top, scale = two_t * 1.44269504f;
+    float sum = 0.0f, weighted = 0.0f;  // (sum z log2(e) e^z)
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float z = E::up(v[i][j]) - shift, e = exp2_fast(z * scale);
+        const float z = half_less(E::up(v[i][j]), half) * scale, e = exp2_fast(z);
         sum += e;
-        weighted = __builtin_fmaf(__builtin_fmaxf(z, -1e30f), e, weighted);  // -infinity has e = 0
+        weighted = __builtin_fmaf(__builtin_fmaxf(z, -1e30f), e, weighted);  // (below -150 e is 0, and -infinity times it not)
       }
     narrow(v);
 #pragma unroll
@@ -211,12 +215,12 @@ __global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float 
       sum += __shfl_xor(sum, n);
       weighted += __shfl_xor(weighted, n);
     }
-    const Sums t{top, sum, weighted * inv_t};
+    const Sums t{top, sum, weighted * 0.693147181f};
     const float log_sum = logf(sum);
     float* out = ws + static_cast<size_t>(part) * (4 + 2 * k);
     if (tid == TH - 1) {
       if (WHOLE) {
-        finish(a, row, t, inv_t, log_sum, logit);
+        finish(a, row, t, two_t, log_sum, logit);
       } else {
         out[0] = t.top;
         out[1] = t.sum;
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float 
         reinterpret_cast<uint64_t*>(out + 4)[rank] = p;
       } else {
         a.top_ids[row * k + rank] = index_of(p);
-        a.top_logprobs[row * k + rank] = logp_of(t, inv_t, log_sum, value_of(static_cast<uint32_t>(p >> 32)));
+        a.top_logprobs[row * k + rank] = logp_of(t, two_t, log_sum, value_of(static_cast<uint32_t>(p >> 32)));
       }
     };
     // candidates, in an order that does not matter: of the few threads that hold any. A NaN or +infinity (the sum is NaN) has
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float 
 
 // The parts of a row joined.
 template <int DT>
-__global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, float inv_t, const float* ws, int segs) {
+__global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, float two_t, const float* ws, int segs) {
   __shared__ uint64_t list[2048];
   const size_t row = blockIdx.x;
   const int k = static_cast<int>(a.top), step = 4 + 2 * k;
@@ -318,12 +322,12 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, float inv_t, cons
   for (int i = 0; i < segs; ++i) {
     const float s = part[i * step + 1], w = part[i * step + 2];
     if (s == 0.0f) continue;
-    const float d = (part[i * step] - t.top) * inv_t, f = exp2_fast(d * 1.44269504f);
+    const float d = half_less(part[i * step], 0.5f * t.top) * two_t, f = exp2_fast(d * 1.44269504f);
     t.sum = __builtin_fmaf(f, s, t.sum);
     t.weighted = __builtin_fmaf(f, __builtin_fmaf(f > 0.0f ? d : 0.0f, s, w), t.weighted);
   }
   const float log_sum = logf(t.sum);
-  if (threadIdx.x == 0) finish(a, row, t, inv_t, log_sum, a.ids ? given<DT>(a, row) : 0.0f);
+  if (threadIdx.x == 0) finish(a, row, t, two_t, log_sum, a.ids ? given<DT>(a, row) : 0.0f);
   if (!k) return;
   const int n = segs * k;
   for (int i = threadIdx.x; i < n; i += 256) list[i] = reinterpret_cast<const uint64_t*>(part + i / k * step + 4)[i % k];
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, float inv_t, cons
     for (int o = 0; o < n; ++o) rank += list[o] > mine;
     if (rank >= k) continue;
     a.top_ids[row * k + rank] = index_of(mine);
-    a.top_logprobs[row * k + rank] = logp_of(t, inv_t, log_sum, value_of(static_cast<uint32_t>(mine >> 32)));
+    a.top_logprobs[row * k + rank] = logp_of(t, two_t, log_sum, value_of(static_cast<uint32_t>(mine >> 32)));
   }
 }
 
@@ -345,7 +349,7 @@ hipError_t launch_logp(const LogpArgs& all, float* ws, hipStream_t s) {
   return with_type(all.dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const LogpPlan p = logp_plan(DT, all.V, all.rows);
-    const float inv_t = 1.0f / all.temperature;
+    const float two_t = 2.0f / all.temperature;
     size_t most = logp_rows_most(p, all.top);
     if (most > size_t{1} << 20) most = size_t{1} << 20;  // a grid has fewer than 2^32 threads
     for (size_t r = 0; r < all.rows; r += most) {
@@ -365,9 +369,9 @@ hipError_t launch_logp(const LogpArgs& all, float* ws, hipStream_t s) {
         if constexpr ((TH == 512 && NV < 8) || TH * NV * Elem<DT>::V > kLogpPart) return false;  // no plan's
         if (p.threads != TH || p.vecs != NV) return false;
         if (p.segs == 1)
-          k_logp<DT, TH, NV, true><<<grid, TH, 0, s>>>(a, inv_t, ws, 1);
+          k_logp<DT, TH, NV, true><<<grid, TH, 0, s>>>(a, two_t, ws, 1);
         else if constexpr (TH * NV * Elem<DT>::V == kLogpPart)
-          k_logp<DT, TH, NV, false><<<grid, TH, 0, s>>>(a, inv_t, ws, p.segs);
+          k_logp<DT, TH, NV, false><<<grid, TH, 0, s>>>(a, two_t, ws, p.segs);
         return true;
       };
       auto any = [&](auto threads) {
@@ -379,7 +383,7 @@ hipError_t launch_logp(const LogpArgs& all, float* ws, hipStream_t s) {
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       if (p.segs > 1) {
-        k_logp_join<DT><<<static_cast<unsigned>(a.rows), 256, 0, s>>>(a, inv_t, ws, p.segs);
+        k_logp_join<DT><<<static_cast<unsigned>(a.rows), 256, 0, s>>>(a, two_t, ws, p.segs);
         if ((e = hipGetLastError()) != hipSuccess) return e;
       }
     }
