@@ -37,35 +37,31 @@ __device__ __forceinline__ Keep keep_of(double log2_total) {
 
 // ---- a row of each sequence ----------------------------------------------------------------------
 // A block takes kCols columns of one head's state of one sequence, in registers: 8 lanes of 4 columns, 32 strips of
-// rows, row strip + 32 i each. Step by step down the sequence. Bound by the state, read and written once: 64 rows of 20 heads of
-// 128 x 128 (168 MB) 34 us, 4.9 TB/s.
+// rows, row strip + 32 i each. Bound by the state, read and written once: 64 rows of 20 heads of 128 x 128 (168 MB) 34 us,
+// 4.9 TB/s.
 constexpr int kCols = 32, kStrips = 32;
 struct NoTab {};
 template <int DT, int NK, class Tab>
-__global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, Tab t, size_t first_seq) {
+__global__ __launch_bounds__(256) void k_decay_row(DecayArgs a, Tab t, size_t first_seq) {
   using E = Elem<DT>;
   using T = typename E::T;
   typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-  __shared__ float sums[2][4][kCols];
+  __shared__ float sums[4][kCols];
   const int slices = static_cast<int>((a.Dv + kCols - 1) / kCols);
   const size_t head = blockIdx.x / slices;
   const int c0 = blockIdx.x % slices * kCols + (threadIdx.x & 7) * 4, strip = threadIdx.x >> 3;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int Dk = static_cast<int>(a.Dk), Dv = static_cast<int>(a.Dv);
-  size_t first = first_seq + blockIdx.y, seq = first;  // a row of each, where there is no table
-  int len = 1;
+  size_t row = first_seq + blockIdx.y, seq = row;  // a row of each, where there is no table
   if constexpr (std::is_same_v<Tab, DecayTab>) {
-    first = t.of[blockIdx.y].row;
+    row = t.of[blockIdx.y].row;
     seq = t.of[blockIdx.y].seq;
-    len = t.of[blockIdx.y].len;
   }
   float* state = a.state ? a.state + (seq * a.heads + head) * a.Dk * a.Dv : nullptr;
-  const T* q = static_cast<const T*>(a.q) + first * a.ldq + head / (a.heads / a.q_heads) * a.Dk;
-  const T* k = static_cast<const T*>(a.k) + first * a.ldk + head / (a.heads / a.k_heads) * a.Dk;
-  const T* v = static_cast<const T*>(a.v) + first * a.ldv + head / (a.heads / a.v_heads) * a.Dv;
-  const float* gates = a.gates ? a.gates + first * a.ldg + head : nullptr;
-  T* out = static_cast<T*>(a.out) + first * a.ldo + head * a.Dv;
-  const double decay = a.decay ? a.decay[head] : 0.0;
+  const T* q = static_cast<const T*>(a.q) + row * a.ldq + head / (a.heads / a.q_heads) * a.Dk;
+  const T* k = static_cast<const T*>(a.k) + row * a.ldk + head / (a.heads / a.k_heads) * a.Dk;
+  const T* v = static_cast<const T*>(a.v) + row * a.ldv + head / (a.heads / a.v_heads) * a.Dv;
+  const double decay = a.decay ? a.decay[head] : 0.0, gate = a.gates ? a.gates[row * a.ldg + head] : 0.0;
   const bool whole = c0 + 4 <= Dv;
 
   float S[NK][4] = {};
@@ -83,37 +79,34 @@ __global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, Tab t, size_t 
       for (int j = 0; j < 4; ++j) S[i][j] = c0 + j < Dv ? p[j] : 0.0f;
     }
   }
-  for (int r = 0; r < len; ++r) {
-    const float keep = static_cast<float>(exp(decay + (gates ? gates[r * a.ldg] : 0.0)));
-    float vv[4], y[4] = {};
+  const float keep = static_cast<float>(exp(decay + gate));
+  float vv[4], y[4] = {};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = c0 + j < Dv ? E::up(v[r * a.ldv + c0 + j]) : 0.0f;
+  for (int j = 0; j < 4; ++j) vv[j] = c0 + j < Dv ? E::up(v[c0 + j]) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int d = strip + kStrips * i;
-      if (d >= Dk) continue;
-      const float kk = E::up(k[r * a.ldk + d]), qq = E::up(q[r * a.ldq + d]);
+  for (int i = 0; i < NK; ++i) {
+    const int d = strip + kStrips * i;
+    if (d >= Dk) continue;
+    const float kk = E::up(k[d]), qq = E::up(q[d]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        S[i][j] = __builtin_fmaf(keep, S[i][j], kk * vv[j]);
-        y[j] = __builtin_fmaf(qq, S[i][j], y[j]);
-      }
+    for (int j = 0; j < 4; ++j) {
+      S[i][j] = __builtin_fmaf(keep, S[i][j], kk * vv[j]);
+      y[j] = __builtin_fmaf(qq, S[i][j], y[j]);
     }
+  }
 #pragma unroll
-    for (int n = 8; n < 64; n *= 2)
+  for (int n = 8; n < 64; n *= 2)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] += __shfl_xor(y[j], n);
-    float (&s)[4][kCols] = sums[r & 1];
-    if (lane < 8) {
+    for (int j = 0; j < 4; ++j) y[j] += __shfl_xor(y[j], n);
+  if (lane < 8) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[wave][lane * 4 + j] = y[j];
-    }
-    __syncthreads();
-    const int c = blockIdx.x % slices * kCols + threadIdx.x;
-    if (threadIdx.x < kCols && c < Dv) {
-      const float o = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
-      out[r * a.ldo + c] = E::down(o * a.scale);
-    }
+    for (int j = 0; j < 4; ++j) sums[wave][lane * 4 + j] = y[j];
+  }
+  __syncthreads();
+  const int c = blockIdx.x % slices * kCols + threadIdx.x;
+  if (threadIdx.x < kCols && c < Dv) {
+    const float o = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+    static_cast<T*>(a.out)[row * a.ldo + head * a.Dv + c] = E::down(o * a.scale);
   }
   if (!state) return;
 #pragma unroll
@@ -131,15 +124,16 @@ __global__ __launch_bounds__(256) void k_decay_steps(DecayArgs a, Tab t, size_t 
   }
 }
 
+// The rows of n sequences of one row each: those of a table, or from first_seq on.
 template <int DT, class Tab>
-hipError_t steps_launch(const DecayArgs& a, const Tab& t, size_t first_seq, int n, hipStream_t s) {
+hipError_t rows_launch(const DecayArgs& a, const Tab& t, size_t first_seq, int n, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.heads * ((a.Dv + kCols - 1) / kCols)), n);
   if (a.Dk <= 64)
-    k_decay_steps<DT, 2, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
+    k_decay_row<DT, 2, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
   else if (a.Dk <= 128)
-    k_decay_steps<DT, 4, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
+    k_decay_row<DT, 4, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
   else
-    k_decay_steps<DT, 8, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
+    k_decay_row<DT, 8, Tab><<<grid, 256, 0, s>>>(a, t, first_seq);
   return hipGetLastError();
 }
 
@@ -743,12 +737,12 @@ hipError_t launch_decay(const DecayArgs& a, float* ws, hipStream_t s) {
     constexpr int DT = decltype(dt)::value;
     if (row_each(a)) {
       for (size_t q = 0; q < a.seqs; q += 65535) {
-        const hipError_t e = steps_launch<DT>(a, NoTab{}, q, static_cast<int>(a.seqs - q < 65535 ? a.seqs - q : 65535), s);
+        const hipError_t e = rows_launch<DT>(a, NoTab{}, q, static_cast<int>(a.seqs - q < 65535 ? a.seqs - q : 65535), s);
         if (e != hipSuccess) return e;
       }
       return hipSuccess;
     }
-    return each_decay(a, hipSuccess, [&](const DecayTab& t) { return steps_launch<DT>(a, t, 0, t.n, s); },
+    return each_decay(a, hipSuccess, [&](const DecayTab& t) { return rows_launch<DT>(a, t, 0, t.n, s); },
                       [&](const DecayTab& t) { return tiles_of<DT>(a, t, ws, s); });
   });
 }

@@ -238,33 +238,31 @@ inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
     if (slots * per <= kLayerWsBytes / 4) return static_cast<int>(step);
   }
 }
-// Calls steps(tab) for sequences of up to kDecayShort rows and tiles(tab) for longer ones, up to kDecaySeqs at a time,
-// until one returns a value other than `ok`. (Steps of two rows are slower already: 32 streams of some two rows, 16 heads of
-// 128 x 128 bf16, 24.9 us, and 20.5 by tiles.)
-constexpr int kDecayShort = 1;
-template <class R, class Steps, class Tiles>
-R each_decay(const DecayArgs& a, R ok, Steps&& steps, Tiles&& tiles) {
-  DecaySeq few[kDecaySeqs], many[kDecaySeqs];
-  int nf = 0, nm = 0, row = 0;
+// Calls ones(tab) for sequences of one row and tiles(tab) for longer ones, up to kDecaySeqs at a time, until one returns a
+// value other than `ok`. (Row after row is slower for two already: 32 streams of some two rows, 16 heads of 128 x 128 bf16,
+// 24.9 us, and 20.5 by tiles.)
+template <class R, class Ones, class Tiles>
+R each_decay(const DecayArgs& a, R ok, Ones&& ones, Tiles&& tiles) {
+  DecaySeq one[kDecaySeqs], many[kDecaySeqs];
+  int n1 = 0, nm = 0, row = 0;
   DecayTab t;
   R r = ok;
-  auto flush = [&](bool of_few) {
-    if (of_few ? nf : nm) {
-      if (of_few)
-        fill_decay(t, few, nf, 1 << 25);
+  auto flush = [&](bool of_ones) {
+    if (of_ones ? n1 : nm) {
+      if (of_ones)
+        fill_decay(t, one, n1, 1);
       else
         fill_decay(t, many, nm, decay_step(a, many, nm));
-      r = of_few ? steps(t) : tiles(t);
+      r = of_ones ? ones(t) : tiles(t);
     }
-    (of_few ? nf : nm) = 0;
+    (of_ones ? n1 : nm) = 0;
   };
   for (size_t i = 0; i < a.seqs && r == ok; ++i) {
     const int len = static_cast<int>(a.lens ? a.lens[i] : a.rows / a.seqs);
     if (!len) continue;
-    const bool is_few = len <= kDecayShort;
-    (is_few ? few[nf++] : many[nm++]) = {row, len, static_cast<int>(i), 0};
+    (len == 1 ? one[n1++] : many[nm++]) = {row, len, static_cast<int>(i), 0};
     row += len;
-    if ((is_few ? nf : nm) == kDecaySeqs) flush(is_few);
+    if ((len == 1 ? n1 : nm) == kDecaySeqs) flush(len == 1);
   }
   if (r == ok) flush(true);
   if (r == ok) flush(false);
