@@ -12,17 +12,16 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v4iu __attribute__((ext_vector_type(4), aligned(1)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-// codes [N, K] -> the layout, a thread 16 bytes of it.
+// codes [N, K] -> the layout, a thread 16 neighbouring inputs of an output, with zeros behind the weights.
 __global__ __launch_bounds__(256) void k_w8_pack(const int8_t* codes, W8Geom g, int8_t* out) {
   const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= static_cast<size_t>(g.nt) * g.nk * 64) return;
-  const int lane = i & 63;
-  const size_t run = i >> 6;
-  const int k0 = static_cast<int>(run % g.nk) * 32 + 16 * (lane >> 5);
-  const size_t n = run / g.nk * 32 + (lane & 31);
+  const size_t run = i >> 6, n = run / g.nk * 32 + i % 32;
+  const int k0 = static_cast<int>(run % g.nk) * 32 + 16 * (i >> 5 & 1);
+  int8_t* to = out + w8_at(g, n, k0);
 #pragma unroll
   for (int j = 0; j < 16; ++j)
-    out[i * 16 + j] = n < static_cast<size_t>(g.N) && k0 + j < g.K ? codes[n * g.K + k0 + j] : static_cast<int8_t>(0);
+    to[j] = n < static_cast<size_t>(g.N) && k0 + j < g.K ? codes[n * g.K + k0 + j] : static_cast<int8_t>(0);
 }
 
 // 16 inputs of a row from k on; what stands past the row's end meets weights of 0 and is not read.
