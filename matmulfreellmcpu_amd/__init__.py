@@ -421,7 +421,7 @@ class Engine:
         [heads] and gates [rows, heads] are log decays, scale None is Dk ** -0.5 (mmf_decay_attention)."""
         _keep, lp, n = _lens(lens, seqs)
         t = _own_type(q) if dtype is None else dtype
-        a = _DECAY_ARGS.pack(t, Dk ** -0.5 if scale is None else scale, _rows(out, t) or 0, _rows(q, t) or 0, _rows(k, t) or 0,
+        a = _DECAY_ARGS.pack(t, max(Dk, 1) ** -0.5 if scale is None else scale, _rows(out, t) or 0, _rows(q, t) or 0, _rows(k, t) or 0,
                              _rows(v, t) or 0, _rows(decay, F32) or 0, _rows(gates, F32) or 0, _rows(state, F32) or 0, lp or 0,
                              n, rows, heads, q_heads, k_heads, v_heads, Dk, Dv, ldo, ldq, ldk, ldv, ldg)
         rc = self.lib.mmf_decay_attention(self.h, a)

@@ -67,3 +67,9 @@ def test_w8_codes_are_int8(eng):  # noqa: F811
             eng.register_w8(codes, [1.0])
     for codes in ([[127, -128]], np.array([[3.0, -4.0]]), np.array([[7, 100]], np.uint8), np.array([[1, -1]], np.int8)):
         eng.register_w8(codes, [1.0])
+
+
+def test_heads_of_no_size_are_refused_by_the_library(eng):  # noqa: F811
+    """The default scale of a head of 0 is no division by 0: the call reaches the library, which says what is wrong."""
+    eng.decay_attention(64, 64, 64, 64, 1, 1, 0, 8)
+    assert eng.lib.args
