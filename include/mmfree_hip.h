@@ -242,7 +242,7 @@ int mmf_w8_linear(mmf_ctx* ctx, int w8_id, const int8_t* x, const float* xscales
  * q [rows, q_heads * Dk], k [rows, k_heads * Dk], v [rows, v_heads * Dv] and out [rows, heads * Dv] of dtype, Dk and Dv
  * 1..256; decay [heads], gates [rows, heads] and state [seqs, heads, Dk, Dv] (may be NULL) in fp32. q_heads, k_heads and
  * v_heads (0: heads) divide heads, and neighbouring heads share one: head h takes the h / (heads / k_heads)-th of k. A log
- * decay of -infinity forgets the state for good. Log decays above 0 are taken as they are: states, outputs and the growth
+ * decay of -infinity forgets a finite state for good. Log decays above 0 are taken as they are: states, outputs and the growth
  * over any 32 rows, by itself and times a product of q and k or a value of v, have to be finite in fp32. Over 32 rows a state
  * counts down to 2^-126 of itself. A row whose q, k or v holds an infinity or NaN does not touch the rows before it. Calls with
  * a sequence of more than 128 rows may use the workspace. */

@@ -7,7 +7,7 @@
 // and the code are taken in fp64, at fp32's rate on this chip.
 //
 // What bounds it: of many rows the vector ALUs, 84 instructions an element of bf16 with silu, 30 of them the sigmoid's: 2048 x 2560
-// 24.7 us with them 0.57 busy (47 MB: 9.9 at a copy's rate), without a gate 15.2; 2048 x 8192 without 32.7 (168 MB, 5.1 TB/s).
+// 24.7 us with them 0.57 busy (47 MB: 9.9 at a copy's rate), without a gate 15.2; 2048 x 8192 without 32.7 (117 MB, 3.6 TB/s).
 #include <algorithm>
 
 #include "mmf_layer_dev.hpp"

@@ -339,8 +339,8 @@ struct DecayDev {
 };
 
 // What bounds it: neither rate. 2048 rows of 16 heads of 128 x 128 bf16 take 11 us (ends) and 20 (outputs), with the matrix cores
-// 0.15 and the vector ALUs 0.3 busy: four chunks a tile, each a line of LDS reads, products and two barriers, of eight waves a compute
-// unit; more tiles would fill it (8 x 1024 rows: 25 and 59), but each writes and reads a state of 64 KB a head.
+// 0.15 and the vector ALUs 0.3 to 0.4 busy: four chunks a tile, each a line of LDS reads, products and two barriers, of eight waves
+// a compute unit; more tiles would fill it (8 x 1024 rows: 25 and 66), but each writes and reads a state of 64 KB a head.
 template <int DT, int DKP, int NW, int PASS, bool EVEN>
 __global__ __launch_bounds__(64 * NW, DT != kF32 && DKP <= 128 && NW == 8 && EVEN ? 4 : 2) void k_decay(DecayDev a, DecayTab t) {
   using Sh = DecayShape<DT, DKP, NW>;
@@ -724,7 +724,7 @@ hipError_t tiles_of(const DecayArgs& a, const DecayTab& t, float* ws, hipStream_
   };
   const bool even = a.Dk % 8 == 0 && a.Dv % 8 == 0;
   // Blocks of 128 columns read q and k once. (Blocks of 64 are sooner done where each has a compute unit of its own, 1000 x 777
-  // fp32 32.6 us and 36.4, but take more of the chip: of three contexts at once 21.5 us a call, and 15.5 by these.)
+  // fp32 33.7 us and 38.0, but take more of the chip: of three contexts at once 22.0 us a call, and 15.9 by these.)
   if (a.Dv > 64) return even ? sized(std::true_type{}, std::true_type{}) : sized(std::true_type{}, std::false_type{});
   return even ? sized(std::false_type{}, std::true_type{}) : sized(std::false_type{}, std::false_type{});
 }

@@ -215,8 +215,8 @@ inline void fill_decay(DecayTab& t, const DecaySeq* s, int n, int step) {
   t.tiles = tiles;
 }
 // Rows of a tile: so many that the tiles of all heads fill the chip twice, and that those of long sequences have room in
-// the workspace. At least 128, as each tile writes a state and reads it three times (2048 rows of 16 heads: 38.8 us, and
-// 44.7 by tiles of 64), but 64 where such tiles have a compute unit each (one head: 22.0 us, and 27.3 by 128). Nothing is
+// the workspace. At least 128, as each tile writes a state and reads it three times (2048 rows of 16 heads: 39.3 us, and
+// 45.2 by tiles of 64), but 64 where such tiles have a compute unit each (one head: 23.1 us, and 28.1 by 128). Nothing is
 // cut where the longest sequence would be cut into two: that would be three launches for one.
 inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
   constexpr int chunk = kDecayChunk;
@@ -240,7 +240,7 @@ inline int decay_step(const DecayArgs& a, const DecaySeq* s, int n) {
 }
 // Calls ones(tab) for sequences of one row and tiles(tab) for longer ones, up to kDecaySeqs at a time, until one returns a
 // value other than `ok`. (Row after row is slower for two already: 32 streams of some two rows, 16 heads of 128 x 128 bf16,
-// 24.9 us, and 20.5 by tiles.)
+// 24.9 us, and 20.8 by tiles.)
 template <class R, class Ones, class Tiles>
 R each_decay(const DecayArgs& a, R ok, Ones&& ones, Tiles&& tiles) {
   DecaySeq one[kDecaySeqs], many[kDecaySeqs];

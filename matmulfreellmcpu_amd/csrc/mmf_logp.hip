@@ -85,7 +85,7 @@ __device__ __forceinline__ void one_by_one(const typename Elem<DT>::T* x, int fr
 }
 
 // A block goes through parts of rows (rows, where one part is a row), the next one's logits on their way meanwhile. 2048 x 32000
-// bf16 (131 MB) 45 us, 27.6 at a copy's rate, with the vector ALUs 0.61 busy: two passes over a row's registers and three
+// bf16 (131 MB) 45 us, 27.6 at a copy's rate, with the vector ALUs 0.56 busy: two passes over a row's registers and three
 // barriers stand between its loads; without top tokens 36.
 template <int DT, int TH, int NV, bool WHOLE>
 __global__ __launch_bounds__(TH, NV <= 2 ? 8 : 4) void k_logp(LogpArgs a, float two_t, float* ws, uint32_t segs) {
